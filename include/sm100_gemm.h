@@ -62,12 +62,15 @@ void gemm_run(int M, int N, int K, const void *X, const void *W, void *Y, float 
 /*
  * Extended arguments for every data type.  No counterpart in the reference (it is
  * BF16-only); gemm_run(M,N,K,X,W,Y,ws,stream) == gemm_run_ex with dtype GEMM_DT_BF16.
+ * A caller that was compiled before w_zero / x_dtype existed passes the smaller struct_size it
+ * knows (up to y_forward) and gets w_zero = NULL, x_dtype = GEMM_X_BF16.
  */
 typedef struct GemmArgs {
     uint32_t struct_size;   /* sizeof(GemmArgs), checked                                   */
     uint32_t dtype;         /* GEMM_DT_*; must match the plugin                            */
     int32_t M, N, K;
-    int32_t group_size;     /* W4A16: K-elements per scale (128); others: ignored          */
+    int32_t group_size;     /* W4A16: K-elements per scale (128; 32, 64 or 128 for the     */
+                            /* matrix-vector plugins); others: ignored                     */
     const void *X;          /* activations, layout per dtype                               */
     const void *W;          /* weights, layout per dtype                                   */
     void *Y;                /* bf16 M x N                                                  */
@@ -113,8 +116,15 @@ typedef struct GemmArgs {
     /* own matrix) and four sender warps forward whole 512-byte rows from L2 while the next tile is computed.  The   */
     /* 512 x 256 plugins always forward; every other plugin ignores the field.                                      */
     int32_t y_forward;
+    /* Matrix-vector plugins of the W4A16 family (`w4a16_bm128_bn<8|16>_bk32_...`, M <= bn); every other plugin    */
+    /* answers GEMM_ERR_ARG when one of the two is set.                                                            */
+    int32_t x_dtype;        /* GEMM_X_*: type of X, of the scales, of C and bias, and of Y                         */
+    const void *w_zero;     /* zero points: W holds unsigned 0..15, one 4-bit zero point per group, two per byte   */
+                            /* (low nibble = even group), rows of ceil(K / group_size / 2) bytes: the weight is    */
+                            /* (q - zero) * scale.  NULL: W is signed                                              */
 } GemmArgs;
 
+enum { GEMM_X_BF16 = 0, GEMM_X_F16 = 1 };
 enum { GEMM_ACT_NONE = 0, GEMM_ACT_RELU = 1, GEMM_ACT_GELU = 2 /* erf form */, GEMM_ACT_SILU = 3 };
 enum { GEMM_Y_BF16 = 0, GEMM_Y_E4M3 = 1 };
 
@@ -125,6 +135,13 @@ enum { GEMM_Y_BF16 = 0, GEMM_Y_E4M3 = 1 };
  * and inside the atom row r, K-block kb at byte (r%32)*16 + ((r%128)/32)*4 + kb%4.  Rows are
  * padded to a multiple of 128.  libsm100gemm_util.so converts a row-major [rows][K/32] array
  * into this layout (include/sm100_gemm_util.h).  Weights are converted once; K must be a multiple of 128 (MXFP8) / 256 (W4A4).
+ *
+ * Matrix-vector plugins (`w4a16_bm128_bn<8|16>_bk32_...`): 1 <= M <= bn rows of X against int4 weights, any N >= 1, K a
+ * multiple of group_size (32, 64 or 128); X bf16 or fp16 (x_dtype), scales [N][K/group_size] of the same type, signed
+ * weights or zero points (w_zero).  X and W 16-byte aligned, every other pointer aligned to its elements.  They use no
+ * workspace (gemm_workspace_bytes reports the family's figure, so that one workspace serves every W4A16 plugin) and the
+ * first call may be made under stream capture.  `_e2`: with the output transform, in the type of X; y_dtype must be
+ * GEMM_Y_BF16 (= "the type of X" here), amax NULL; C may be Y.  Sums are FP32, rounded once.
  */
 /* Returns GEMM_OK or an error code; asynchronous on success. */
 int gemm_run_ex(const GemmArgs *args);

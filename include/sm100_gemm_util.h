@@ -47,6 +47,81 @@ int gemm_quant_mx(const void *x, void *q, void *sf_tiled, long long rows, int K,
  * s = bf16(max|group| / 7) (1 for a zero group), q = clamp(rint(w * (1 / s)), -8, 7).  K a multiple of 128. */
 int gemm_quant_int4_g128(const void *w, void *q, void *scales, long long rows, int K, void *stream);
 
+/* ---- the operators beside the projections of a decode step (csrc/token_kernels.cu).  No reference counterpart.
+ * Stream-ordered, asynchronous, no allocation, no workspace; both may be captured into a CUDA graph, the first call too.
+ * All pointers are device pointers of the current device.  A refused call launches nothing and returns
+ * cudaErrorInvalidValue; gemm_util_last_error_message() then says why (text of the calling thread's last such call).
+ * x and y are the same buffer (in place) or do not overlap. */
+enum { GEMM_X_F32 = 2 };     /* beside GEMM_X_BF16 = 0 and GEMM_X_F16 = 1 of include/sm100_gemm.h */
+const char *gemm_util_last_error_message(void);
+
+/* Rotary positions on `heads` heads of each of `tokens` tokens: the pair (a, b) number i of a head becomes
+ *     scale * (a cos t - b sin t,  a sin t + b cos t),   t = position * f_i          (backward: t -> -t)
+ * f_i = base^(-2 i / rot_dim), scaled for contexts longer than trained (`scaling`).  Pairs: (i, i + rot_dim / 2) or
+ * (2 i, 2 i + 1) of the head's first rot_dim elements; elements behind them are copied.  A token with a negative position
+ * is padding: its heads are passed through unchanged.  backward = 1 turns the gradient of y into that of x (the transposed
+ * map; its rows are addressed as x -> y too).  Angles are exact modulo a turn at every position.
+ * Strides are in elements, so that q and k are turned in place inside a fused QKV result: heads = q + k heads,
+ * token stride = the row of the whole result. */
+enum { GEMM_ROTARY_HALF = 0, GEMM_ROTARY_INTERLEAVED = 1 };
+enum {
+    GEMM_ROTARY_PLAIN = 0,
+    GEMM_ROTARY_LINEAR = 1,  /* f_i / factor                                                                          */
+    GEMM_ROTARY_NTK = 2,     /* base * factor^(rot_dim / (rot_dim - 2)) in the place of base                          */
+    GEMM_ROTARY_RAMP = 3     /* f_i * w + f_i / factor * (1 - w), w = (original_length * f_i / 2 pi - low_rotations)  */
+                             /* / (high_rotations - low_rotations), clamped to [0, 1]                                 */
+};
+typedef struct GemmRotaryArgs {
+    uint32_t struct_size;   /* sizeof(GemmRotaryArgs), checked                       */
+    int32_t dtype;          /* GEMM_X_BF16, GEMM_X_F16 or GEMM_X_F32: type of x and y */
+    int32_t layout;         /* GEMM_ROTARY_HALF / _INTERLEAVED                       */
+    int32_t backward;       /* 0 / 1                                                 */
+    int64_t tokens;         /* 0: nothing is done                                    */
+    int32_t heads, head_dim;
+    int32_t rot_dim;        /* even, <= head_dim and <= 512                          */
+    int32_t scaling;        /* GEMM_ROTARY_PLAIN ...                                 */
+    const void *x;
+    void *y;
+    int64_t x_token_stride, x_head_stride, y_token_stride, y_head_stride;
+    const int64_t *positions;   /* [tokens]                                          */
+    double base;            /* 10000 in most models                                  */
+    double factor, low_rotations, high_rotations, original_length;
+    float scale;            /* multiplies cos and sin (1 when no attention scaling)  */
+    int32_t reserved;       /* 0                                                     */
+    void *stream;
+} GemmRotaryArgs;
+int gemm_rotary(const GemmRotaryArgs *args);
+
+/* Logits of `rows` sequences before sampling, y[r][v] from x[r][v], in FP32, rounded once to the type of y:
+ *     l = x;  token v in the row's history:  l = l > 0 ? l / repetition : l * repetition
+ *     c = how often v was generated, c > 0:  l -= frequency * c + presence
+ *     v listed in the row's biases:          l += the sum of its listed values, in the order of the list
+ *     mask bit of v is 0:                    l = -inf (whatever it was; a row that allows nothing is all -inf)
+ * History: the first history_len[r] tokens of row r (at most history_ld), the first prompt_len[r] of which are the prompt:
+ * they count as seen, not as generated; without a history (history NULL, a first token) no penalty applies.  Ids outside [0, vocab) are ignored, in the history and in the biases. */
+typedef struct GemmLogitsArgs {
+    uint32_t struct_size;   /* sizeof(GemmLogitsArgs), checked                                             */
+    int32_t x_dtype, y_dtype;   /* GEMM_X_BF16, GEMM_X_F16 or GEMM_X_F32                                   */
+    int32_t rows;           /* 0: nothing is done                                                          */
+    int32_t vocab;
+    int32_t reserved;       /* 0                                                                           */
+    const void *x;
+    void *y;
+    int64_t x_ld, y_ld;     /* row pitches in elements, >= vocab                                           */
+    const int32_t *history; /* [rows][history_ld], or NULL                                                 */
+    int64_t history_ld;
+    const int32_t *history_len;     /* [rows], with history                                                */
+    const int32_t *prompt_len;      /* [rows], or NULL: everything was generated                           */
+    const float *repetition, *presence, *frequency;     /* [rows] each, or NULL: 1, 0, 0                   */
+    const int32_t *bias_ids;        /* biases of row r: entries bias_begin[r] .. bias_begin[r + 1] - 1     */
+    const float *bias_values;
+    const int32_t *bias_begin;      /* [rows + 1], not decreasing, or NULL (all three)                     */
+    const uint32_t *mask;   /* [rows][mask_ld], bit v % 32 of word v / 32: 1 = allowed; or NULL            */
+    int64_t mask_ld;        /* >= ceil(vocab / 32)                                                         */
+    void *stream;
+} GemmLogitsArgs;
+int gemm_logits(const GemmLogitsArgs *args);
+
 /* ---- offline weight packing and the weight file (host memory, host code).  No reference counterpart. */
 enum {
     GEMM_FILE_ERR_ARG = -5,      /* null pointer, value out of range, K not a multiple the layout needs */

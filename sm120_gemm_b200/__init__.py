@@ -21,6 +21,7 @@ KERNEL_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "kernels")
 GEMM_OK = 0
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3       # GEMM_ACT_* of include/sm100_gemm.h
 Y_BF16, Y_E4M3 = 0, 1                                     # GEMM_Y_*
+X_BF16, X_F16, X_F32 = 0, 1, 2                            # GEMM_X_* (X_F32: rotary and logits only)
 ERROR_NAMES = {0: "GEMM_OK", 1: "GEMM_ERR_SHAPE", 2: "GEMM_ERR_CUDA", 3: "GEMM_ERR_DRIVER", 4: "GEMM_ERR_WORKSPACE",
                5: "GEMM_ERR_DEVICE_TIMEOUT", 6: "GEMM_ERR_ARG"}
 
@@ -53,6 +54,7 @@ class GemmArgs(ctypes.Structure):
         ("C", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("alpha", ctypes.c_float), ("beta", ctypes.c_float),
         ("activation", ctypes.c_int32), ("y_dtype", ctypes.c_int32), ("y_scale", ctypes.c_float), ("amax", ctypes.c_void_p),
         ("y_forward", ctypes.c_int32),
+        ("x_dtype", ctypes.c_int32), ("w_zero", ctypes.c_void_p),
     ]
 
     def __init__(self, *a, **kw):
@@ -71,12 +73,55 @@ class GemmWeightFileInfo(ctypes.Structure):
                 ("scale_bytes", ctypes.c_uint64), ("tensor_scale", ctypes.c_float), ("checksum", ctypes.c_uint32)]
 
 
+ROTARY_HALF, ROTARY_INTERLEAVED = 0, 1                                    # GEMM_ROTARY_* of include/sm100_gemm_util.h
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_NTK, ROTARY_RAMP = 0, 1, 2, 3
+
+
+class GemmRotaryArgs(ctypes.Structure):
+    """``struct GemmRotaryArgs`` of include/sm100_gemm_util.h."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("dtype", ctypes.c_int32), ("layout", ctypes.c_int32), ("backward", ctypes.c_int32),
+        ("tokens", ctypes.c_int64), ("heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("rot_dim", ctypes.c_int32), ("scaling", ctypes.c_int32),
+        ("x", ctypes.c_void_p), ("y", ctypes.c_void_p),
+        ("x_token_stride", ctypes.c_int64), ("x_head_stride", ctypes.c_int64), ("y_token_stride", ctypes.c_int64), ("y_head_stride", ctypes.c_int64),
+        ("positions", ctypes.c_void_p),
+        ("base", ctypes.c_double), ("factor", ctypes.c_double), ("low_rotations", ctypes.c_double), ("high_rotations", ctypes.c_double),
+        ("original_length", ctypes.c_double), ("scale", ctypes.c_float), ("reserved", ctypes.c_int32), ("stream", ctypes.c_void_p),
+    ]
+
+    def __init__(self, *a, **kw):
+        super().__init__(*a, **kw)
+        self.struct_size = ctypes.sizeof(GemmRotaryArgs)
+        for name, value in (("base", 10000.0), ("factor", 1.0), ("scale", 1.0)):
+            if name not in kw:
+                setattr(self, name, value)
+
+
+class GemmLogitsArgs(ctypes.Structure):
+    """``struct GemmLogitsArgs`` of include/sm100_gemm_util.h."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("x_dtype", ctypes.c_int32), ("y_dtype", ctypes.c_int32), ("rows", ctypes.c_int32),
+        ("vocab", ctypes.c_int32), ("reserved", ctypes.c_int32), ("x", ctypes.c_void_p), ("y", ctypes.c_void_p),
+        ("x_ld", ctypes.c_int64), ("y_ld", ctypes.c_int64), ("history", ctypes.c_void_p), ("history_ld", ctypes.c_int64),
+        ("history_len", ctypes.c_void_p), ("prompt_len", ctypes.c_void_p),
+        ("repetition", ctypes.c_void_p), ("presence", ctypes.c_void_p), ("frequency", ctypes.c_void_p),
+        ("bias_ids", ctypes.c_void_p), ("bias_values", ctypes.c_void_p), ("bias_begin", ctypes.c_void_p),
+        ("mask", ctypes.c_void_p), ("mask_ld", ctypes.c_int64), ("stream", ctypes.c_void_p),
+    ]
+
+    def __init__(self, *a, **kw):
+        super().__init__(*a, **kw)
+        self.struct_size = ctypes.sizeof(GemmLogitsArgs)
+
+
 # every symbol include/sm100_gemm_util.h declares
 UTIL_SYMBOLS = ("gemm_interleave_blocks", "gemm_spacer", "gemm_mx_tiled_scale_bytes", "gemm_mx_scales_to_tiled",
                 "gemm_quant_e4m3_per_tensor", "gemm_quant_mx", "gemm_quant_int4_g128", "gemm_packed_weight_bytes",
                 "gemm_packed_scale_bytes", "gemm_pack_int4_host", "gemm_unpack_int4_host", "gemm_pack_fp4_host", "gemm_unpack_fp4_host",
                 "gemm_mx_scales_to_tiled_host", "gemm_mx_scales_from_tiled_host", "gemm_weight_file_write", "gemm_weight_file_info",
-                "gemm_weight_file_read")
+                "gemm_weight_file_read", "gemm_rotary", "gemm_logits", "gemm_util_last_error_message")
 
 
 @dataclass
@@ -292,9 +337,28 @@ def util_lib() -> ctypes.CDLL:
         lib.gemm_weight_file_write.argtypes = [ctypes.c_char_p, ci, ll, ci, ctypes.c_float, vp, vp]
         lib.gemm_weight_file_info.argtypes = [ctypes.c_char_p, ctypes.POINTER(GemmWeightFileInfo)]
         lib.gemm_weight_file_read.argtypes = [ctypes.c_char_p, vp, ctypes.c_size_t, vp, ctypes.c_size_t]
+        lib.gemm_rotary.argtypes = [ctypes.POINTER(GemmRotaryArgs)]
+        lib.gemm_logits.argtypes = [ctypes.POINTER(GemmLogitsArgs)]
+        lib.gemm_util_last_error_message.restype = ctypes.c_char_p
         _UTIL = lib
     return _UTIL
 
 
+def _util_call(fn, args) -> None:
+    rc = fn(args)
+    if rc != 0:
+        raise GemmError(6 if rc == 1 else 2, util_lib().gemm_util_last_error_message().decode())     # cudaErrorInvalidValue: a refused argument
+
+
+def rotary(args: GemmRotaryArgs) -> None:
+    """Rotary positions (``gemm_rotary``): queued on ``args.stream``; GemmError when the call is refused."""
+    _util_call(util_lib().gemm_rotary, args)
+
+
+def logits(args: GemmLogitsArgs) -> None:
+    """Penalties, biases and grammar masks on logits (``gemm_logits``): queued on ``args.stream``; GemmError when the call is refused."""
+    _util_call(util_lib().gemm_logits, args)
+
+
 __all__ = ["heuristic_config", "heuristic_ms", "GemmWeightFileInfo", "UTIL_SYMBOLS", "util_lib", "GemmConfig", "generate_configs", "KernelRegistry", "AutotuneCache", "LoadedKernel", "GemmArgs", "GemmError",
-           "dispatch", "dispatch_ex", "load_plugin", "KERNEL_DIR", "ABI_SYMBOLS"]
+           "GemmRotaryArgs", "GemmLogitsArgs", "rotary", "logits", "dispatch", "dispatch_ex", "load_plugin", "KERNEL_DIR", "ABI_SYMBOLS"]

@@ -91,9 +91,9 @@ UTIL_LIB = os.path.join(KERNEL_DIR, "libsm100gemm_util.so")
 
 
 def build_util(force: bool = False) -> str:
-    """The utility library: quantisation kernels, weight packers and file format, block interleave for the
+    """The utility library: quantisation kernels, rotary positions, logits operators, weight packers and file format, block interleave for the
     N-sharded run, MX scale tiling, timing spacer."""
-    srcs = [os.path.join(CSRC, f) for f in ("gemm_util.cu", "quant_kernels.cu", "weight_file.cpp")]
+    srcs = [os.path.join(CSRC, f) for f in ("gemm_util.cu", "quant_kernels.cu", "token_kernels.cu", "weight_file.cpp")]
     if not force and os.path.exists(UTIL_LIB) and os.path.getmtime(UTIL_LIB) >= _deps_mtime():
         return UTIL_LIB
     os.makedirs(KERNEL_DIR, exist_ok=True)

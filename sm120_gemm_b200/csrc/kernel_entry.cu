@@ -9,6 +9,7 @@
 #include "bf16_gemm.cuh"
 #include "w4a16_gemm.cuh"
 #include "w4a16_tmem_gemm.cuh"
+#include "w4_matvec.cuh"
 
 #ifndef GEMM_DT
 #error "configuration macros missing: build through sm120_gemm_b200/build.py"
@@ -33,7 +34,12 @@ constexpr int MB = GEMM_MB;          // 128-row blocks of X per CTA
 constexpr int BM = 128 * CG * MB;
 
 #if GEMM_DT == 3
-// W4A16: operands swapped (AB = 1), BN is M padded, work is always cut stream-K fashion (SK = 0)
+#if GEMM_BK == 32    // matrix-vector products: weights stream through registers, M <= BN
+static_assert(AB == 1 && SK == 1 && CG == 1 && (EPI == 0 || EPI == 2), "matrix-vector plugins are w4a16_bm128_bn<8|16>_bk32_s<S>_cg1_sk1_ab1_e<0|2>");
+using Traits = sm100::W4MatvecTraits<BN, STAGES, EPI>;
+using Launcher = sm100::W4MatvecLauncher<Traits>;
+#else
+// W4A16 on the tensor memory: operands swapped (AB = 1), BN is M padded, work is always cut stream-K fashion (SK = 0)
 static_assert(AB == 1 && SK == 0 && CG == 1 && EPI == 0, "W4A16 plugins are <dt>_bm128_bn<MPAD>_bk<64|128>_s<S>_cg1_sk0_ab1_e0");
 #if GEMM_BK == 128   // dequantised weights through tensor memory
 using Traits = sm100::W4A16TmemTraits<BN, STAGES>;
@@ -41,6 +47,7 @@ using Launcher = sm100::W4A16TmemLauncher<Traits>;
 #else                // dequantised weights through shared memory
 using Traits = sm100::W4A16Traits<BN, STAGES>;
 using Launcher = sm100::W4A16Launcher<Traits>;
+#endif
 #endif
 #elif GEMM_DT == 0
 // BF16: through the reference's two entry-point classes, chosen at compile time exactly as its entry template
@@ -103,8 +110,22 @@ void gemm_run(int M, int N, int K, const void *X, const void *W, void *Y, float 
 int gemm_run_ex(const GemmArgs *a)
 {
     sm100::clear_error();
-    if (!a || a->struct_size != sizeof(GemmArgs)) return sm100::set_error(GEMM_ERR_ARG, "GemmArgs is null or has the wrong struct_size");
+    // the struct grew at its end: a caller compiled before that passes the size up to y_forward (padded to 8 bytes)
+    constexpr size_t kOldBytes = offsetof(GemmArgs, x_dtype), kOldSize = (kOldBytes + 7) / 8 * 8;
+    if (!a || (a->struct_size != sizeof(GemmArgs) && a->struct_size != kOldSize))
+        return sm100::set_error(GEMM_ERR_ARG, "GemmArgs is null or has the wrong struct_size");
+    GemmArgs widened;
+    if (a->struct_size == kOldSize) {
+        memset(&widened, 0, sizeof(widened));
+        memcpy(&widened, a, kOldBytes);
+        a = &widened;
+    }
     if ((int)a->dtype != DT) return sm100::set_error(GEMM_ERR_ARG, "dtype %u does not match plugin %s", a->dtype, kConfigName);
+#if GEMM_DT == 3 && GEMM_BK == 32
+    if (a->y_num_peers > 0) return sm100::set_error(GEMM_ERR_ARG, "peer destinations are not supported by %s", kConfigName);
+    return Launcher::run(*a);
+#else
+    if (a->x_dtype || a->w_zero) return sm100::set_error(GEMM_ERR_ARG, "x_dtype and w_zero need a matrix-vector configuration (w4a16 ..._bk32_...), not %s", kConfigName);
 #if GEMM_DT == 3
     if (a->y_num_peers > 0) return sm100::set_error(GEMM_ERR_ARG, "peer destinations are not supported by %s", kConfigName);
     if (a->C || a->bias || a->amax || a->activation || a->y_dtype) return sm100::set_error(GEMM_ERR_ARG, "%s has no fused output transform", kConfigName);
@@ -147,6 +168,7 @@ int gemm_run_ex(const GemmArgs *a)
 #endif
 #else
     return Launcher::run(a->M, a->N, a->K, a->X, a->W, a->Y, static_cast<float *>(a->workspace), a->workspace_bytes, a->stream, ex);
+#endif
 #endif
 #endif
 }

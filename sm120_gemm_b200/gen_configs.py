@@ -10,7 +10,8 @@ shared-memory cap for the mma.sync kernel), re-derived for the tcgen05 design:
   bn       multiple of 16 up to 256  (UMMA N; two FP32 accumulator buffers need 2*bn <= 512 TMEM columns;
            the TMA-store epilogue needs a multiple of 64)
   bk       one 128-byte swizzle span of K per stage: 64 bf16, 128 fp8, 256 fp4 elements
-           (w4a16: 64 = dequantised tiles in shared memory, 128 = dequantised scale groups in tensor memory)
+           (w4a16: 64 = dequantised tiles in shared memory, 128 = dequantised scale groups in tensor memory,
+           32 = matrix-vector products for M <= bn: groups of 32, 64 or 128, zero points, bf16 or fp16)
   s        TMA ring stages, bounded by the 227 KB of shared memory one CTA may use
   cg       CTA group (1 | 2)
   sk       split-K factor (FP32 partials + reduce kernel); 0 = stream-K: the tiles x k-blocks work is
@@ -70,6 +71,8 @@ class GemmConfig:
 
     def smem_bytes(self) -> int:
         """Dynamic shared memory of the kernel; must equal the traits' SMEM_ALLOC."""
+        if self.dt == "w4a16" and self.bk == 32:
+            return 0
         if self.dt == "w4a16" and self.bk == 128:   # W4A16TmemTraits: load ring only (16 KB packed + 4 activation boxes per stage); s = group slots in TMEM
             load_stage = 128 * 128 + 4 * (-(-self.bn * 128 // 1024) * 1024)
             load_stages = min(8, 200 * 1024 // load_stage)
@@ -99,6 +102,8 @@ class GemmConfig:
         """The plugin's own gemm_can_run, restated (reference: src/gemm_config.h:34-38)."""
         if M <= 0 or N <= 0 or K <= 0:
             return False
+        if self.dt == "w4a16" and self.bk == 32:   # matrix-vector plugins (K must also be whole scale groups)
+            return M <= self.bn and K % 32 == 0
         if self.dt == "w4a16":   # decode kernel: M fits the padded UMMA N, whole 128-element scale groups
             return M <= self.bn and N % 8 == 0 and K % 128 == 0
         if (K * ELEM_BITS[self.dt]) % 128 != 0 or N % 8 != 0:
@@ -203,8 +208,12 @@ def generate_block_scaled(dt: str, max_smem: int) -> list[GemmConfig]:
 def generate_w4a16(max_smem: int) -> list[GemmConfig]:
     """W4A16 decode kernels: operands swapped (ab=1), bn = M padded to 16/32/64/128, stream-K work split.
     bk128: dequantised weights go through tensor memory (A operand of the MMA read from TMEM), s = group slots;
-    bk64: dequantised weights go through shared memory, s = group ring slots."""
+    bk64: dequantised weights go through shared memory, s = group ring slots.
+    bk32: matrix-vector products (sk1: the whole K in one CTA), s = 16-byte weight loads in flight per thread."""
     out = []
+    for rows in (8, 16):
+        for epi in (0, 2):
+            out.append(GemmConfig("w4a16", 128, rows, 32, 8, 1, 1, 1, epi))
     for mpad, slots in ((16, 6), (32, 5), (64, 4), (128, 2)):
         c = GemmConfig("w4a16", 128, mpad, 128, slots, 1, 0, 1, 0)
         if c.smem_bytes() <= max_smem:
