@@ -8,6 +8,26 @@
 //
 // u - z is an integer of at most 5 bits, exact in bf16 and fp16, and the products and sums are FP32: the only rounding to
 // fewer bits is the last one, of y.
+//
+// What it has to do is read N * K / 2 bytes once, so the weights go from global memory straight to registers (16 bytes per
+// lane and load, several in flight, no shared memory, no barrier on their way) and the sums are taken by the warp-level
+// matrix instruction m16n8k16 with the 16 weight rows of a tile as A and the rows of X as the 8 columns of B: FP32 FMAs
+// alone would need 1.9 G of them per row of X at 28672 x 8192, six times the time of the bytes for M = 8.
+//
+// The order of k inside a sum is free, so it follows the packing: lane (g, c) = (lane / 4, lane % 4) of a warp reads
+// 16 bytes = 32 consecutive k of weight rows g and g + 8, the four lanes of a quad 128 k (a UNIT).  Of a word's eight
+// nibbles the pairs (0,4), (1,5), (2,6), (3,7) come out of one mask each as two 16-bit numbers, and X is staged in shared
+// memory in that order, fragment by fragment, so that one 16-byte load feeds two matrix instructions.
+//
+// Scales belong to (row, group) and are applied to FP32 sums, one multiply-add per group and accumulator.  A group of 128
+// is a unit.  Of smaller groups a unit holds GPU = 2 or 4, lane c's 32 elements in group c * GPU / 4: then a column of B is
+// a (row of X, group) pair, zero where the lane's elements are of another group, and the sums of the groups stay apart in
+// different columns.  NB column blocks of 8 hold the M * GPU columns.
+//
+// Work: CTA i takes the rows N * i / grid .. N * (i + 1) / grid (any boundary: every SM reads the same number of bytes),
+// cut into tiles of 16.  Its 16 (or 8) warps are WR groups over the tiles times WK slices over the units of K; the WK partial sums
+// of a tile meet in shared memory and are added in the order of the slices -- no atomics, the same result every run.
+// X is staged whole when it fits, else in passes over K with the partial sums kept.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -27,17 +47,47 @@ struct W4MatvecParams {
     const void *C, *bias;        // output transform
     float alpha, beta;
     int act;
+    // the launch's plan
+    int block_rows;              // rows of W whose partial sums shared memory holds
+    int units_per_pass;          // units (128 K-elements) of X that shared memory holds
+    int wk_shift;                // log2(WK)
 };
 
+// mma D += A * B, m16n8k16, A and B of the type E, D FP32;  dequantisation of two nibbles (bits 0-3 and 16-19 of a word):
+// placed in the low mantissa bits of MAGIC (128 in bf16, 1024 in fp16) they are that number plus the nibble, exactly.
 template <class T>
 struct W4Type;
 template <>
 struct W4Type<__nv_bfloat16> {
+    static constexpr uint32_t MAGIC = 0x43004300u;
+    static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+    {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+    static __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b)
+    {
+        uint32_t r;
+        asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
     static __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
     static __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
 };
 template <>
 struct W4Type<__half> {
+    static constexpr uint32_t MAGIC = 0x64006400u;
+    static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+    {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+    static __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b)
+    {
+        uint32_t r;
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
     static __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
     static __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
 };
@@ -47,8 +97,13 @@ struct W4MatvecTraits {
     static constexpr int MPAD = MPAD_;       // most rows of X
     static constexpr int STAGES = STAGES_;
     static constexpr int EPI = EPI_;
-    static constexpr int THREADS = 256;
-    static constexpr int SMEM_ALLOC = 0;
+    // 16 warps of 128 registers; the 4 and 8 column blocks of small groups and many rows need more registers: 8 warps
+    template <int NB>
+    static constexpr int WARPS = NB <= 2 ? 16 : 8;
+    static constexpr int TILE = 16, UNIT = 128;
+    static constexpr int PART_BYTES = 52 * 1024;     // partial sums
+    static constexpr int X_BYTES = 160 * 1024;       // staged X
+    static constexpr int SMEM_ALLOC = PART_BYTES + X_BYTES;
     static_assert(MPAD_ == 8 || MPAD_ == 16, "rows of X: up to 8 or 16");
 };
 
@@ -68,44 +123,223 @@ __device__ __forceinline__ void w4_store(const W4MatvecParams &p, int m, int n, 
     static_cast<E *>(p.Y)[at] = W4Type<E>::from_f32(v);
 }
 
-// One warp per weight row: lane l takes the 32-element blocks l, l + 32, ... (16 bytes of W each).
-template <class E, class T>
-__global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4MatvecParams p)
+// the eight k of one packed word as four 16-bit pairs (0,4), (1,5), (2,6), (3,7), each nibble minus its zero point
+template <class E, bool ZERO>
+__device__ __forceinline__ void w4_dequant(uint32_t w, uint32_t bias, uint32_t (&out)[4])
 {
-    const int lane = threadIdx.x & 31;
-    const int warps = gridDim.x * (T::THREADS / 32);
-    const int groups = p.K >> p.group_shift;
+    constexpr uint32_t MERGE = W4Type<E>::MAGIC | (ZERO ? 0u : 0x00080008u);      // signed: the xor also flips the nibble's sign bit
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        uint32_t y;
+        asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(y) : "r"(w >> (4 * j)), "n"(0x000f000f), "n"(MERGE));      // (a & b) ^ c
+        out[j] = W4Type<E>::sub2(y, bias);
+    }
+}
+
+// one unit of one tile for one lane, as loaded
+template <int GPU>
+struct W4Unit {
+    static constexpr int SCALES = GPU == 1 ? 1 : 2;
+    uint4 a, b;                      // rows g and g + 8
+    uint16_t sa[SCALES], sb[SCALES];
+    uint8_t za, zb;
+};
+
+__device__ __forceinline__ uint4 w4_stream_load(const uint8_t *p)
+{
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// place of one warp in its share of a pass: tiles WR apart, units WK apart
+struct W4Place {
+    int tile, unit;
+};
+
+template <class E, int NB, int GPU, bool ZERO, class T>
+__global__ void __launch_bounds__(32 * T::template WARPS<NB>, 1) w4_matvec_kernel(const W4MatvecParams p)
+{
+    constexpr int WARPS = T::template WARPS<NB>, THREADS = 32 * WARPS;
+    constexpr int DEPTH = NB == 2 && GPU > 1 ? 3 : 4;      // units in flight per warp (what the registers hold)
+    extern __shared__ __align__(16) uint8_t smem[];
+    float *part = reinterpret_cast<float *>(smem);                                  // [WK][M][block_rows]
+    uint4 *xs = reinterpret_cast<uint4 *>(smem + T::PART_BYTES);                    // [unit][word 0..3][m][c]: 8 values of X
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int g = lane >> 2, c = lane & 3;
+    const int WK = 1 << p.wk_shift, WR = WARPS >> p.wk_shift;
+    const int wk = warp & (WK - 1), wr = warp >> p.wk_shift;
+    const int M = p.M, K = p.K;
+    const int groups = K >> p.group_shift;
+    const int zero_pitch = (groups + 1) >> 1;
+    const int units = (K + T::UNIT - 1) / T::UNIT;
+    const size_t row_bytes = (size_t)(K >> 1);
+    const int row_begin = (int)((long long)p.N * blockIdx.x / gridDim.x), row_end = (int)((long long)p.N * (blockIdx.x + 1) / gridDim.x);
     const E *X = static_cast<const E *>(p.X), *S = static_cast<const E *>(p.scales);
-    for (int n = blockIdx.x * (T::THREADS / 32) + (threadIdx.x >> 5); n < p.N; n += warps) {
-        float acc[T::MPAD];
+
+    // this lane's column of B in column block nb: row m of X, for the lane's own group only
+    int xoff[NB];
 #pragma unroll
-        for (int m = 0; m < T::MPAD; m++) acc[m] = 0.f;
-        for (int k = lane * 32; k < p.K; k += 1024) {
-            const uint4 w = __ldcs(reinterpret_cast<const uint4 *>(p.W + (size_t)n * (p.K / 2) + k / 2));
-            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-            const int g = k >> p.group_shift;
-            const float s = W4Type<E>::to_f32(S[(size_t)n * groups + g]);
-            const int z = p.zeros ? (p.zeros[(size_t)n * ((groups + 1) / 2) + g / 2] >> (4 * (g & 1))) & 15 : 8;
-            const uint32_t flip = p.zeros ? 0u : 8u;
+    for (int nb = 0; nb < NB; nb++) {
+        const int col = nb * 8 + g, m = col / GPU;
+        xoff[nb] = (m < M && col % GPU == c * GPU / 4) ? m * 4 + c : -1;
+    }
+
+    for (int row0 = row_begin; row0 < row_end; row0 += p.block_rows) {
+        const int rows = min(p.block_rows, row_end - row0);
+        const int tiles = (rows + T::TILE - 1) / T::TILE;
+        for (int u0 = 0; u0 < units; u0 += p.units_per_pass) {
+            const int nu = min(p.units_per_pass, units - u0);       // units of this pass
+            // the slices of a tile start rotated from tile to tile, so that a last, partial round of units falls on other warps
+            const int turn = nu & (WK - 1);
+            auto settle = [&](W4Place &at) {
+                while (at.tile < tiles && at.unit >= nu) { at.tile += WR; at.unit = (wk + at.tile * turn) & (WK - 1); }
+            };
+            auto load = [&](W4Unit<GPU> &r, const W4Place &at) {
+                r.a = r.b = make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int m = 0; m < T::MPAD; m++) {
-                if (m >= p.M) break;
-                float part = 0.f;
+                for (int i = 0; i < W4Unit<GPU>::SCALES; i++) r.sa[i] = r.sb[i] = 0;
+                r.za = r.zb = 0;
+                if (at.tile >= tiles) return;
+                const int ra = at.tile * T::TILE + g, rb = ra + 8;
+                const int u = u0 + at.unit;
+                const bool in_k = u * T::UNIT + c * 32 < K;
+                const uint8_t *w = p.W + (size_t)(row0 + ra) * row_bytes + (size_t)u * (T::UNIT / 2) + c * 16;
+                if (in_k && ra < rows) r.a = w4_stream_load(w);
+                if (in_k && rb < rows) r.b = w4_stream_load(w + 8 * row_bytes);
+                // scales of the groups of this lane's two accumulator columns (2c, 2c + 1)
+                const int s0 = GPU == 1 ? u : GPU == 2 ? 2 * u : 4 * u + 2 * (c & 1);
+                const uint16_t *sp = reinterpret_cast<const uint16_t *>(S) + (size_t)(row0 + ra) * groups + s0;
 #pragma unroll
-                for (int j = 0; j < 32; j++) {
-                    const int u = (int)(((words[j / 8] >> (4 * (j % 8))) & 15u) ^ flip);
-                    part = fmaf((float)(u - z), W4Type<E>::to_f32(X[(size_t)m * p.K + k + j]), part);
+                for (int i = 0; i < W4Unit<GPU>::SCALES; i++) {
+                    if (s0 + i < groups && ra < rows) r.sa[i] = __ldg(sp + i);
+                    if (s0 + i < groups && rb < rows) r.sb[i] = __ldg(sp + (size_t)8 * groups + i);
                 }
-                acc[m] = fmaf(s, part, acc[m]);
+                if (ZERO) {
+                    const int zg = u * GPU + c * GPU / 4;          // group of this lane's elements
+                    const uint8_t *zp = p.zeros + (size_t)(row0 + ra) * zero_pitch + (zg >> 1);
+                    if (zg < groups && ra < rows) r.za = __ldg(zp) >> (4 * (zg & 1));
+                    if (zg < groups && rb < rows) r.zb = __ldg(zp + (size_t)8 * zero_pitch) >> (4 * (zg & 1));
+                }
+            };
+            W4Place ahead = {wr, (wk + wr * turn) & (WK - 1)};
+            settle(ahead);
+            W4Place at = ahead;
+            W4Unit<GPU> ring[DEPTH];
+#pragma unroll
+            for (int d = 0; d < DEPTH; d++) {
+                load(ring[d], ahead);
+                ahead.unit += WK;
+                settle(ahead);
+            }
+            // stage X while the first weights are on their way; the pass before has to be through with its own
+            if (units > p.units_per_pass || row0 == row_begin) {
+                __syncthreads();
+                const int pieces = nu * 2 * M * 4;                  // (unit, half of the words, m, c): 16 values, 32 bytes each
+                for (int i = threadIdx.x; i < pieces; i += THREADS) {
+                    const int xc = i & 3, m = (i >> 2) % M, uh = (i >> 2) / M;
+                    const int k = (u0 + (uh >> 1)) * T::UNIT + xc * 32 + (uh & 1) * 16;
+                    uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+                    if (k < K) {
+                        const uint4 *src = reinterpret_cast<const uint4 *>(X + (size_t)m * K + k);
+                        v[0] = __ldg(src);
+                        v[1] = __ldg(src + 1);
+                    }
+                    uint4 *dst = xs + ((uh * 2) * M + m) * 4 + xc;
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+                        dst[h * M * 4] = make_uint4(__byte_perm(v[h].x, v[h].z, 0x5410), __byte_perm(v[h].x, v[h].z, 0x7632),
+                                                    __byte_perm(v[h].y, v[h].w, 0x5410), __byte_perm(v[h].y, v[h].w, 0x7632));
+                }
+                __syncthreads();
+            }
+            float total[NB][4];
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) total[nb][i] = 0.f;
+            while (at.tile < tiles) {
+#pragma unroll
+                for (int d = 0; d < DEPTH; d++) {
+                    if (at.tile >= tiles) break;
+                    W4Unit<GPU> &r = ring[d];
+                    const uint32_t bias_a = ZERO ? W4Type<E>::MAGIC + (uint32_t)(r.za & 15) * 0x00010001u : W4Type<E>::MAGIC | 0x00080008u;
+                    const uint32_t bias_b = ZERO ? W4Type<E>::MAGIC + (uint32_t)(r.zb & 15) * 0x00010001u : W4Type<E>::MAGIC | 0x00080008u;
+                    const uint32_t wa[4] = {r.a.x, r.a.y, r.a.z, r.a.w}, wb[4] = {r.b.x, r.b.y, r.b.z, r.b.w};
+                    float acc[NB][4];
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[nb][i] = 0.f;
+                    const uint4 *xu = xs + at.unit * (16 * M);
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        uint32_t qa[4], qb[4];
+                        w4_dequant<E, ZERO>(wa[w], bias_a, qa);
+                        w4_dequant<E, ZERO>(wb[w], bias_b, qb);
+#pragma unroll
+                        for (int nb = 0; nb < NB; nb++) {
+                            uint4 x = make_uint4(0, 0, 0, 0);
+                            if (xoff[nb] >= 0) x = xu[w * (4 * M) + xoff[nb]];
+                            W4Type<E>::mma(acc[nb], qa[0], qb[0], qa[1], qb[1], x.x, x.y);
+                            W4Type<E>::mma(acc[nb], qa[2], qb[2], qa[3], qb[3], x.z, x.w);
+                        }
+                    }
+                    constexpr int S1 = W4Unit<GPU>::SCALES - 1;
+                    auto scale = [](uint16_t bits) { return W4Type<E>::to_f32(*reinterpret_cast<const E *>(&bits)); };
+                    const float sa0 = scale(r.sa[0]), sa1 = scale(r.sa[S1]), sb0 = scale(r.sb[0]), sb1 = scale(r.sb[S1]);
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++) {
+                        total[nb][0] = fmaf(sa0, acc[nb][0], total[nb][0]);
+                        total[nb][1] = fmaf(sa1, acc[nb][1], total[nb][1]);
+                        total[nb][2] = fmaf(sb0, acc[nb][2], total[nb][2]);
+                        total[nb][3] = fmaf(sb1, acc[nb][3], total[nb][3]);
+                    }
+                    load(r, ahead);
+                    ahead.unit += WK;
+                    settle(ahead);
+                    const int tile = at.tile;
+                    at.unit += WK;
+                    settle(at);
+                    if (at.tile != tile) {
+                        // the warp's share of this tile is complete: its partial sums go to its own slot
+                        float *slot = part + (size_t)wk * M * p.block_rows + tile * T::TILE + g;
+                        auto put = [&](int m, int row, float v) {
+                            if (m >= M || tile * T::TILE + g + row >= rows) return;
+                            float *q = slot + m * p.block_rows + row;
+                            *q = u0 == 0 ? v : *q + v;
+                        };
+#pragma unroll
+                        for (int nb = 0; nb < NB; nb++) {
+                            if constexpr (GPU == 1) {
+                                put(nb * 8 + 2 * c, 0, total[nb][0]);
+                                put(nb * 8 + 2 * c + 1, 0, total[nb][1]);
+                                put(nb * 8 + 2 * c, 8, total[nb][2]);
+                                put(nb * 8 + 2 * c + 1, 8, total[nb][3]);
+                            } else if constexpr (GPU == 2) {
+                                put(nb * 4 + c, 0, total[nb][0] + total[nb][1]);
+                                put(nb * 4 + c, 8, total[nb][2] + total[nb][3]);
+                            } else {
+                                float v0 = total[nb][0] + total[nb][1], v1 = total[nb][2] + total[nb][3];
+                                v0 += __shfl_xor_sync(0xffffffffu, v0, 1);
+                                v1 += __shfl_xor_sync(0xffffffffu, v1, 1);
+                                put(nb * 2 + (c >> 1), (c & 1) * 8, (c & 1) ? v1 : v0);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 4; i++) total[nb][i] = 0.f;
+                        }
+                    }
+                }
             }
         }
-#pragma unroll
-        for (int m = 0; m < T::MPAD; m++) {
-            if (m >= p.M) break;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) acc[m] += __shfl_xor_sync(0xffffffffu, acc[m], o);
-            if (lane == 0) w4_store<E, T::EPI>(p, m, n, acc[m]);
+        __syncthreads();
+        for (int i = threadIdx.x; i < rows * M; i += THREADS) {
+            const int m = i / rows, r = i - m * rows;
+            float v = 0.f;
+            for (int w = 0; w < WK; w++) v += part[((size_t)w * M + m) * p.block_rows + r];
+            w4_store<E, T::EPI>(p, m, row0 + r, v);
         }
+        __syncthreads();
     }
 }
 
@@ -143,11 +377,83 @@ struct W4MatvecLauncher {
         p.alpha = a.alpha;
         p.beta = a.beta;
         p.act = a.activation;
-        long long grid = ((long long)a.N + T::THREADS / 32 - 1) / (T::THREADS / 32);
-        const long long most = a.sm_limit > 0 ? a.sm_limit : 148 * 8;
-        if (grid > most) grid = most;
-        if (a.x_dtype == GEMM_X_F16) w4_matvec_kernel<__half, T><<<(unsigned)grid, T::THREADS, 0, a.stream>>>(p);
-        else w4_matvec_kernel<__nv_bfloat16, T><<<(unsigned)grid, T::THREADS, 0, a.stream>>>(p);
+        int sms = 0;
+        int rc = sm_count(&sms);
+        if (rc != GEMM_OK) return rc;
+        int grid = a.sm_limit > 0 && a.sm_limit < sms ? a.sm_limit : sms;
+        if (grid > a.N) grid = a.N;
+        // partial sums: rows of a CTA x M x WK floats; as many K slices as fit (a tile's bytes then arrive soonest), blocks of
+        // rows when not even one slice of all rows does
+        const int rows = (a.N + grid - 1) / grid, units = (a.K + T::UNIT - 1) / T::UNIT;
+        const int most_units = T::X_BYTES / (a.M * T::UNIT * 2), passes = (units + most_units - 1) / most_units;
+        p.units_per_pass = (units + passes - 1) / passes;
+        const int slots = T::PART_BYTES / (int)sizeof(float) / a.M;
+        const int columns = a.M * (T::UNIT >> p.group_shift);
+        p.wk_shift = columns <= 16 ? 4 : 3;
+        while (p.wk_shift > 0 && ((1 << p.wk_shift) > p.units_per_pass || (rows << p.wk_shift) > slots)) p.wk_shift--;
+        p.block_rows = rows;
+        if (rows > slots) {
+            const int blocks = (rows + slots / T::TILE * T::TILE - 1) / (slots / T::TILE * T::TILE);
+            p.block_rows = ((rows + blocks - 1) / blocks + T::TILE - 1) / T::TILE * T::TILE;
+        }
+        const int smem = T::PART_BYTES + p.units_per_pass * a.M * T::UNIT * 2;
+        if (a.x_dtype == GEMM_X_F16) return launch<__half>(p, grid, smem, a.stream);
+        return launch<__nv_bfloat16>(p, grid, smem, a.stream);
+    }
+
+private:
+    static int sm_count(int *out)
+    {
+        static std::atomic<int> counts[MAX_DEVICES];
+        int dev = 0;
+        SM100_CUDA_TRY(cudaGetDevice(&dev));
+        if (dev < 0 || dev >= MAX_DEVICES) return set_error(GEMM_ERR_ARG, "device ordinal %d out of range", dev);
+        int n = counts[dev].load(std::memory_order_relaxed);
+        if (n == 0) {
+            SM100_CUDA_TRY(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+            counts[dev].store(n, std::memory_order_relaxed);
+        }
+        *out = n;
+        return GEMM_OK;
+    }
+
+    template <class E>
+    static int launch(const W4MatvecParams &p, int grid, int smem, cudaStream_t stream)
+    {
+        if (p.zeros) return launch_groups<E, true>(p, grid, smem, stream);
+        return launch_groups<E, false>(p, grid, smem, stream);
+    }
+    template <class E, bool ZERO>
+    static int launch_groups(const W4MatvecParams &p, int grid, int smem, cudaStream_t stream)
+    {
+        if (p.group_shift == 7) return launch_columns<E, ZERO, 1>(p, grid, smem, stream);
+        if (p.group_shift == 6) return launch_columns<E, ZERO, 2>(p, grid, smem, stream);
+        return launch_columns<E, ZERO, 4>(p, grid, smem, stream);
+    }
+    template <class E, bool ZERO, int GPU>
+    static int launch_columns(const W4MatvecParams &p, int grid, int smem, cudaStream_t stream)
+    {
+        const int columns = p.M * GPU;
+        if (columns <= 8) return launch_kernel<E, ZERO, GPU, 1>(p, grid, smem, stream);
+        if constexpr (T::MPAD * GPU >= 16)
+            if (columns <= 16) return launch_kernel<E, ZERO, GPU, 2>(p, grid, smem, stream);
+        if constexpr (T::MPAD * GPU >= 32)
+            if (columns <= 32) return launch_kernel<E, ZERO, GPU, 4>(p, grid, smem, stream);
+        if constexpr (T::MPAD * GPU >= 64) return launch_kernel<E, ZERO, GPU, 8>(p, grid, smem, stream);
+        return set_error(GEMM_ERR_SHAPE, "%d rows do not fit this configuration", p.M);
+    }
+    template <class E, bool ZERO, int GPU, int NB>
+    static int launch_kernel(const W4MatvecParams &p, int grid, int smem, cudaStream_t stream)
+    {
+        static std::atomic<bool> attr_set[MAX_DEVICES];
+        int dev = 0;
+        SM100_CUDA_TRY(cudaGetDevice(&dev));
+        auto *kernel = w4_matvec_kernel<E, NB, GPU, ZERO, T>;
+        if (!attr_set[dev].load(std::memory_order_acquire)) {
+            SM100_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM_ALLOC));
+            attr_set[dev].store(true, std::memory_order_release);
+        }
+        kernel<<<grid, 32 * T::template WARPS<NB>, smem, stream>>>(p);
         SM100_CUDA_TRY(cudaGetLastError());
         return GEMM_OK;
     }
