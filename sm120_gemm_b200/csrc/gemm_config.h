@@ -73,7 +73,7 @@ struct GemmConfig {
     bool is_valid_for(int M, int N, int K) const
     {
         if (M <= 0 || N <= 0 || K <= 0) return false;
-        if (dt == GEMM_DT_W4A16 && bk == 32) return M <= bn && K % 32 == 0;      // matrix-vector plugins (K must also be whole scale groups)
+        if (dt == GEMM_DT_W4A16 && bk == 32) return M <= bn && K % 32 == 0 && K <= 1 << 28;      // matrix-vector plugins (K must also be whole scale groups)
         if (dt == GEMM_DT_W4A16) return M <= bn && N % 8 == 0 && K % 128 == 0;   // decode kernel, bn = padded M
         if (((long long)K * sm100::elem_bits(dt)) % 128 != 0 || N % 8 != 0) return false;
         if ((dt == GEMM_DT_MXFP8 || dt == GEMM_DT_W4A4) && K % bk != 0) return false;
@@ -85,7 +85,7 @@ struct GemmConfig {
     // a plugin reports the exact figure through gemm_smem_bytes()).
     size_t smem_bytes() const
     {
-        if (dt == GEMM_DT_W4A16 && bk == 32) return (52 + 160) * 1024;   // matrix-vector plugins: partial sums + staged X (the largest launch)
+        if (dt == GEMM_DT_W4A16 && bk == 32) return (52 + 160) * 1024 + 256;   // matrix-vector plugins: partial sums + staged X (the largest launch)
         if (dt == GEMM_DT_W4A16 && bk == 128) {   // tensor-memory family: load ring only (16 KB packed + 4 activation boxes per stage)
             const size_t load_stage = 128 * 128 + 4 * (((size_t)bn * 128 + 1023) / 1024 * 1024);
             const size_t fit = (200 * 1024) / load_stage;

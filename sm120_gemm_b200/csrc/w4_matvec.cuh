@@ -18,6 +18,10 @@
 // 16 bytes = 32 consecutive k of weight rows g and g + 8, the four lanes of a quad 128 k (a UNIT).  Of a word's eight
 // nibbles the pairs (0,4), (1,5), (2,6), (3,7) come out of one mask each as two 16-bit numbers, and X is staged in shared
 // memory in that order, fragment by fragment, so that one 16-byte load feeds two matrix instructions.
+// The masked bits are not moved into place: read as 16-bit floating point, a pattern below twice the smallest normal number
+// is that integer times the smallest subnormal, so bits 0-3 are q and bits 4-7 are 16 q of those, and one packed multiply-add
+// by a power of two turns either into (q - z) * 2^-6 (bf16; fp16: 2^-9), exactly: one shift, four logic instructions and
+// four multiply-adds for eight weights.  The sums are multiplied by 2^6 (2^9) at the end.
 //
 // Scales belong to (row, group) and are applied to FP32 sums, one multiply-add per group and accumulator.  A group of 128
 // is a unit.  Of smaller groups a unit holds GPU = 2 or 4, lane c's 32 elements in group c * GPU / 4: then a column of B is
@@ -53,22 +57,29 @@ struct W4MatvecParams {
     int wk_shift;                // log2(WK)
 };
 
-// mma D += A * B, m16n8k16, A and B of the type E, D FP32;  dequantisation of two nibbles (bits 0-3 and 16-19 of a word):
-// placed in the low mantissa bits of MAGIC (128 in bf16, 1024 in fp16) they are that number plus the nibble, exactly.
+// What depends on the 16-bit type: mma D = A * B + D (m16n8k16, D FP32; `first`: D = A * B), the packed multiply-add, and
+// the constants of the conversion: LOW * (q in bits 0-3) = HIGH * (q in bits 4-7) = q / OUT as packed numbers.
 template <class T>
 struct W4Type;
 template <>
 struct W4Type<__nv_bfloat16> {
-    static constexpr uint32_t MAGIC = 0x43004300u;
+    static constexpr uint32_t LOW = 0x7f007f00u, HIGH = 0x7d007d00u, NEG_LOW = 0xff00ff00u;      // 2^127, 2^123, -2^127
+    static constexpr uint32_t MINUS_8 = 0xbe00be00u;                                             // -8 / OUT
+    static constexpr float OUT = 64.f;
     static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
     {
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     }
-    static __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b)
+    static __device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+    {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    }
+    static __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c)
     {
         uint32_t r;
-        asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
         return r;
     }
     static __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -76,16 +87,23 @@ struct W4Type<__nv_bfloat16> {
 };
 template <>
 struct W4Type<__half> {
-    static constexpr uint32_t MAGIC = 0x64006400u;
+    static constexpr uint32_t LOW = 0x78007800u, HIGH = 0x68006800u, NEG_LOW = 0xf800f800u;      // 2^15, 2^11, -2^15
+    static constexpr uint32_t MINUS_8 = 0xa400a400u;                                             // -8 / OUT
+    static constexpr float OUT = 512.f;
     static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
     {
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     }
-    static __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b)
+    static __device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+    {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    }
+    static __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c)
     {
         uint32_t r;
-        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
         return r;
     }
     static __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
@@ -97,13 +115,16 @@ struct W4MatvecTraits {
     static constexpr int MPAD = MPAD_;       // most rows of X
     static constexpr int STAGES = STAGES_;
     static constexpr int EPI = EPI_;
-    // 16 warps of 128 registers; the 4 and 8 column blocks of small groups and many rows need more registers: 8 warps
+    // 16 warps of 128 registers; more column blocks need more registers: 8 warps
     template <int NB>
-    static constexpr int WARPS = NB <= 2 ? 16 : 8;
+    static constexpr int WARPS = NB == 1 ? 16 : 8;
     static constexpr int TILE = 16, UNIT = 128;
     static constexpr int PART_BYTES = 52 * 1024;     // partial sums
     static constexpr int X_BYTES = 160 * 1024;       // staged X
-    static constexpr int SMEM_ALLOC = PART_BYTES + X_BYTES;
+    static constexpr int ZERO_BYTES = 256;           // zeros that are read in the place of X
+    static constexpr int SMEM_ALLOC = PART_BYTES + ZERO_BYTES + X_BYTES;
+    static constexpr int X_ROW = 256 + 64;           // staged X, one unit of one row
+    static __host__ __device__ constexpr int x_unit_bytes(int M) { return M * X_ROW; }      // staged X, one unit
     static_assert(MPAD_ == 8 || MPAD_ == 16, "rows of X: up to 8 or 16");
 };
 
@@ -123,17 +144,22 @@ __device__ __forceinline__ void w4_store(const W4MatvecParams &p, int m, int n, 
     static_cast<E *>(p.Y)[at] = W4Type<E>::from_f32(v);
 }
 
-// the eight k of one packed word as four 16-bit pairs (0,4), (1,5), (2,6), (3,7), each nibble minus its zero point
+// the eight k of one packed word as four 16-bit pairs (0,4), (1,5), (2,6), (3,7), each (nibble - zero point) / OUT;
+// `minus` is the packed -zero point / OUT
 template <class E, bool ZERO>
-__device__ __forceinline__ void w4_dequant(uint32_t w, uint32_t bias, uint32_t (&out)[4])
+__device__ __forceinline__ void w4_dequant(uint32_t w, uint32_t minus, uint32_t (&out)[4])
 {
-    constexpr uint32_t MERGE = W4Type<E>::MAGIC | (ZERO ? 0u : 0x00080008u);      // signed: the xor also flips the nibble's sign bit
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
+    constexpr uint32_t FLIP = ZERO ? 0u : 0x00080008u;      // signed weights: flipping the top bit of a nibble adds 8
+    const uint32_t v = w >> 8;
+    auto pick = [](uint32_t x, uint32_t mask, uint32_t flip) {
         uint32_t y;
-        asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(y) : "r"(w >> (4 * j)), "n"(0x000f000f), "n"(MERGE));      // (a & b) ^ c
-        out[j] = W4Type<E>::sub2(y, bias);
-    }
+        asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(y) : "r"(x), "r"(mask), "r"(flip));      // (x & mask) ^ flip
+        return y;
+    };
+    out[0] = W4Type<E>::fma2(pick(w, 0x000f000fu, FLIP), W4Type<E>::LOW, minus);
+    out[1] = W4Type<E>::fma2(pick(w, 0x00f000f0u, FLIP << 4), W4Type<E>::HIGH, minus);
+    out[2] = W4Type<E>::fma2(pick(v, 0x000f000fu, FLIP), W4Type<E>::LOW, minus);
+    out[3] = W4Type<E>::fma2(pick(v, 0x00f000f0u, FLIP << 4), W4Type<E>::HIGH, minus);
 }
 
 // one unit of one tile for one lane, as loaded
@@ -152,20 +178,18 @@ __device__ __forceinline__ uint4 w4_stream_load(const uint8_t *p)
     return v;
 }
 
-// place of one warp in its share of a pass: tiles WR apart, units WK apart
-struct W4Place {
-    int tile, unit;
-};
-
 template <class E, int NB, int GPU, bool ZERO, class T>
 __global__ void __launch_bounds__(32 * T::template WARPS<NB>, 1) w4_matvec_kernel(const W4MatvecParams p)
 {
     constexpr int WARPS = T::template WARPS<NB>, THREADS = 32 * WARPS;
-    constexpr int DEPTH = NB == 2 && GPU > 1 ? 3 : 4;      // units in flight per warp (what the registers hold)
+    constexpr int BATCH = NB == 8 ? 1 : NB == 1 ? 2 : 4;    // units that are loaded together; two batches in flight per warp
     extern __shared__ __align__(16) uint8_t smem[];
-    float *part = reinterpret_cast<float *>(smem);                                  // [WK][M][block_rows]
-    uint4 *xs = reinterpret_cast<uint4 *>(smem + T::PART_BYTES);                    // [unit][word 0..3][m][c]: 8 values of X
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float *part = reinterpret_cast<float *>(smem);       // [WK][M][block_rows]
+    // X: 256 bytes per unit and m ([word 0..3][c]: 8 values), 320 apart, so that the eight lanes of a 16-byte access
+    // (two m) reach all banks; in front of it zeros for the lanes whose column is another group's
+    uint8_t *xs = smem + T::PART_BYTES + T::ZERO_BYTES;
+    const int lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);                 // uniform over the warp, and known to be
     const int g = lane >> 2, c = lane & 3;
     const int WK = 1 << p.wk_shift, WR = WARPS >> p.wk_shift;
     const int wk = warp & (WK - 1), wr = warp >> p.wk_shift;
@@ -173,16 +197,20 @@ __global__ void __launch_bounds__(32 * T::template WARPS<NB>, 1) w4_matvec_kerne
     const int groups = K >> p.group_shift;
     const int zero_pitch = (groups + 1) >> 1;
     const int units = (K + T::UNIT - 1) / T::UNIT;
-    const size_t row_bytes = (size_t)(K >> 1);
+    const uint32_t row_bytes = (uint32_t)K >> 1;
+    const uint32_t unit_bytes = T::x_unit_bytes(M);
     const int row_begin = (int)((long long)p.N * blockIdx.x / gridDim.x), row_end = (int)((long long)p.N * (blockIdx.x + 1) / gridDim.x);
-    const E *X = static_cast<const E *>(p.X), *S = static_cast<const E *>(p.scales);
 
-    // this lane's column of B in column block nb: row m of X, for the lane's own group only
-    int xoff[NB];
+    // this lane's column of B in column block nb: row m of X, for the lane's own group only.  Columns behind the last may
+    // hold anything (they only reach their own sums, which nobody reads): they repeat the last row's.
+    uint32_t xaddr[NB], xstep[NB];
+    if (threadIdx.x < T::ZERO_BYTES / 16) reinterpret_cast<uint4 *>(smem + T::PART_BYTES)[threadIdx.x] = make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
-        const int col = nb * 8 + g, m = col / GPU;
-        xoff[nb] = (m < M && col % GPU == c * GPU / 4) ? m * 4 + c : -1;
+        const int col = nb * 8 + g, m = min(col / GPU, M - 1);
+        const bool own = GPU == 1 || col % GPU == c * GPU / 4;
+        xaddr[nb] = own ? T::PART_BYTES + T::ZERO_BYTES + m * T::X_ROW + c * 16 : T::PART_BYTES;
+        xstep[nb] = own ? unit_bytes : 0;
     }
 
     for (int row0 = row_begin; row0 < row_end; row0 += p.block_rows) {
@@ -190,50 +218,90 @@ __global__ void __launch_bounds__(32 * T::template WARPS<NB>, 1) w4_matvec_kerne
         const int tiles = (rows + T::TILE - 1) / T::TILE;
         for (int u0 = 0; u0 < units; u0 += p.units_per_pass) {
             const int nu = min(p.units_per_pass, units - u0);       // units of this pass
-            // the slices of a tile start rotated from tile to tile, so that a last, partial round of units falls on other warps
+            // A warp's share of the pass is a sequence of units, WK apart in a tile, tiles WR apart.  The slices of a tile
+            // start rotated from tile to tile, so that a last, partial round of units falls on other warps.
             const int turn = nu & (WK - 1);
-            auto settle = [&](W4Place &at) {
-                while (at.tile < tiles && at.unit >= nu) { at.tile += WR; at.unit = (wk + at.tile * turn) & (WK - 1); }
-            };
-            auto load = [&](W4Unit<GPU> &r, const W4Place &at) {
-                r.a = r.b = make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < W4Unit<GPU>::SCALES; i++) r.sa[i] = r.sb[i] = 0;
-                r.za = r.zb = 0;
-                if (at.tile >= tiles) return;
-                const int ra = at.tile * T::TILE + g, rb = ra + 8;
-                const int u = u0 + at.unit;
-                const bool in_k = u * T::UNIT + c * 32 < K;
-                const uint8_t *w = p.W + (size_t)(row0 + ra) * row_bytes + (size_t)u * (T::UNIT / 2) + c * 16;
-                if (in_k && ra < rows) r.a = w4_stream_load(w);
-                if (in_k && rb < rows) r.b = w4_stream_load(w + 8 * row_bytes);
+            auto first_unit = [&](int tile) { return (wk + tile * turn) & (WK - 1); };
+            const int tail = K & (T::UNIT - 1) ? units - 1 - u0 : -1;       // the unit that ends behind K
+            // loading side: place, the current tile's addresses (one for the warp) and the lane's offsets to them; rows
+            // behind the block's last are read as the last
+            int ld_tile = wr, ld_unit = 0;
+            const uint8_t *wt = nullptr, *st = nullptr, *zt = nullptr;
+            uint32_t wa = 0, wb = 0, sa = 0, sb = 0, za = 0, zb = 0;
+            auto enter_tile = [&]() {
+                while (ld_tile < tiles && (ld_unit = first_unit(ld_tile)) >= nu) ld_tile += WR;
+                if (ld_tile >= tiles) return;
+                const int last = rows - 1 - ld_tile * T::TILE;
+                const uint32_t ra = min(g, last), rb = min(g + 8, last);
+                const size_t r = row0 + ld_tile * T::TILE;
+                wt = p.W + r * row_bytes + (size_t)u0 * (T::UNIT / 2);
+                wa = ra * row_bytes + c * 16;
+                wb = rb * row_bytes + c * 16;
                 // scales of the groups of this lane's two accumulator columns (2c, 2c + 1)
-                const int s0 = GPU == 1 ? u : GPU == 2 ? 2 * u : 4 * u + 2 * (c & 1);
-                const uint16_t *sp = reinterpret_cast<const uint16_t *>(S) + (size_t)(row0 + ra) * groups + s0;
-#pragma unroll
-                for (int i = 0; i < W4Unit<GPU>::SCALES; i++) {
-                    if (s0 + i < groups && ra < rows) r.sa[i] = __ldg(sp + i);
-                    if (s0 + i < groups && rb < rows) r.sb[i] = __ldg(sp + (size_t)8 * groups + i);
-                }
+                st = static_cast<const uint8_t *>(p.scales) + (r * groups + (size_t)u0 * GPU) * 2;
+                sa = (ra * groups + (GPU == 4 ? 2 * (c & 1) : 0)) * 2;
+                sb = (rb * groups + (GPU == 4 ? 2 * (c & 1) : 0)) * 2;
                 if (ZERO) {
-                    const int zg = u * GPU + c * GPU / 4;          // group of this lane's elements
-                    const uint8_t *zp = p.zeros + (size_t)(row0 + ra) * zero_pitch + (zg >> 1);
-                    if (zg < groups && ra < rows) r.za = __ldg(zp) >> (4 * (zg & 1));
-                    if (zg < groups && rb < rows) r.zb = __ldg(zp + (size_t)8 * zero_pitch) >> (4 * (zg & 1));
+                    zt = p.zeros + r * zero_pitch;
+                    za = ra * zero_pitch + (GPU == 4 ? c >> 1 : 0);
+                    zb = rb * zero_pitch + (GPU == 4 ? c >> 1 : 0);
                 }
             };
-            W4Place ahead = {wr, (wk + wr * turn) & (WK - 1)};
-            settle(ahead);
-            W4Place at = ahead;
-            W4Unit<GPU> ring[DEPTH];
+            auto load_unit = [&](W4Unit<GPU> &r, int u) {
+                const uint8_t *w = wt + (size_t)u * (T::UNIT / 2), *s = st + (size_t)u * (GPU * 2);
+                // zero points: byte of the lane's group, (u * GPU + c * GPU / 4) / 2
+                const uint8_t *z = ZERO ? zt + (GPU == 4 ? 2 * (u0 + u) : GPU == 2 ? u0 + u : (u0 + u) >> 1) : nullptr;
+                if (u != tail) {
+                    r.a = w4_stream_load(w + wa);
+                    r.b = w4_stream_load(w + wb);
 #pragma unroll
-            for (int d = 0; d < DEPTH; d++) {
-                load(ring[d], ahead);
-                ahead.unit += WK;
-                settle(ahead);
-            }
+                    for (int i = 0; i < W4Unit<GPU>::SCALES; i++) {
+                        r.sa[i] = __ldg(reinterpret_cast<const uint16_t *>(s + sa) + i);
+                        r.sb[i] = __ldg(reinterpret_cast<const uint16_t *>(s + sb) + i);
+                    }
+                    if (ZERO) {
+                        r.za = __ldg(z + za);
+                        r.zb = __ldg(z + zb);
+                    }
+                } else {
+                    r.a = r.b = make_uint4(0, 0, 0, 0);
+                    r.za = r.zb = 0;
+                    if ((u0 + u) * T::UNIT + c * 32 < K) {
+                        r.a = w4_stream_load(w + wa);
+                        r.b = w4_stream_load(w + wb);
+                        if (ZERO) {
+                            r.za = __ldg(z + za);
+                            r.zb = __ldg(z + zb);
+                        }
+                    }
+                    const int left = groups - (u0 + u) * GPU - (GPU == 4 ? 2 * (c & 1) : 0);
+#pragma unroll
+                    for (int i = 0; i < W4Unit<GPU>::SCALES; i++) {
+                        r.sa[i] = i < left ? __ldg(reinterpret_cast<const uint16_t *>(s + sa) + i) : (uint16_t)0;
+                        r.sb[i] = i < left ? __ldg(reinterpret_cast<const uint16_t *>(s + sb) + i) : (uint16_t)0;
+                    }
+                }
+            };
+            auto load = [&](W4Unit<GPU> (&r)[BATCH]) {
+                if (ld_tile >= tiles) return;
+                load_unit(r[0], ld_unit);
+#pragma unroll
+                for (int i = 1; i < BATCH; i++)
+                    if (ld_unit + i * WK < nu) load_unit(r[i], ld_unit + i * WK);
+                ld_unit += BATCH * WK;
+                if (ld_unit >= nu) {
+                    ld_tile += WR;
+                    enter_tile();
+                }
+            };
+            enter_tile();
+            int tile = ld_tile, unit = ld_unit;                             // computing side
+            W4Unit<GPU> ring[2][BATCH];
+            load(ring[0]);
+            load(ring[1]);
             // stage X while the first weights are on their way; the pass before has to be through with its own
             if (units > p.units_per_pass || row0 == row_begin) {
+                const E *X = static_cast<const E *>(p.X);
                 __syncthreads();
                 const int pieces = nu * 2 * M * 4;                  // (unit, half of the words, m, c): 16 values, 32 bytes each
                 for (int i = threadIdx.x; i < pieces; i += THREADS) {
@@ -245,11 +313,11 @@ __global__ void __launch_bounds__(32 * T::template WARPS<NB>, 1) w4_matvec_kerne
                         v[0] = __ldg(src);
                         v[1] = __ldg(src + 1);
                     }
-                    uint4 *dst = xs + ((uh * 2) * M + m) * 4 + xc;
+                    uint4 *dst = reinterpret_cast<uint4 *>(xs + (uh >> 1) * unit_bytes + m * T::X_ROW + (uh & 1) * 128 + xc * 16);
 #pragma unroll
                     for (int h = 0; h < 2; h++)
-                        dst[h * M * 4] = make_uint4(__byte_perm(v[h].x, v[h].z, 0x5410), __byte_perm(v[h].x, v[h].z, 0x7632),
-                                                    __byte_perm(v[h].y, v[h].w, 0x5410), __byte_perm(v[h].y, v[h].w, 0x7632));
+                        dst[h * 4] = make_uint4(__byte_perm(v[h].x, v[h].z, 0x5410), __byte_perm(v[h].x, v[h].z, 0x7632),
+                                                __byte_perm(v[h].y, v[h].w, 0x5410), __byte_perm(v[h].y, v[h].w, 0x7632));
                 }
                 __syncthreads();
             }
@@ -258,54 +326,55 @@ __global__ void __launch_bounds__(32 * T::template WARPS<NB>, 1) w4_matvec_kerne
             for (int nb = 0; nb < NB; nb++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) total[nb][i] = 0.f;
-            while (at.tile < tiles) {
+            auto compute_unit = [&](const W4Unit<GPU> &r, int u) {
+                uint32_t minus_a = W4Type<E>::MINUS_8, minus_b = W4Type<E>::MINUS_8;
+                if (ZERO) {
+                    const int shift = GPU == 4 ? 4 * (c & 1) : GPU == 2 ? 4 * (c >> 1) : 4 * ((u0 + u) & 1);
+                    minus_a = W4Type<E>::fma2(((uint32_t)(r.za >> shift) & 15u) * 0x00010001u, W4Type<E>::NEG_LOW, 0u);
+                    minus_b = W4Type<E>::fma2(((uint32_t)(r.zb >> shift) & 15u) * 0x00010001u, W4Type<E>::NEG_LOW, 0u);
+                }
+                const uint32_t qwa[4] = {r.a.x, r.a.y, r.a.z, r.a.w}, qwb[4] = {r.b.x, r.b.y, r.b.z, r.b.w};
+                float acc[NB][4];
 #pragma unroll
-                for (int d = 0; d < DEPTH; d++) {
-                    if (at.tile >= tiles) break;
-                    W4Unit<GPU> &r = ring[d];
-                    const uint32_t bias_a = ZERO ? W4Type<E>::MAGIC + (uint32_t)(r.za & 15) * 0x00010001u : W4Type<E>::MAGIC | 0x00080008u;
-                    const uint32_t bias_b = ZERO ? W4Type<E>::MAGIC + (uint32_t)(r.zb & 15) * 0x00010001u : W4Type<E>::MAGIC | 0x00080008u;
-                    const uint32_t wa[4] = {r.a.x, r.a.y, r.a.z, r.a.w}, wb[4] = {r.b.x, r.b.y, r.b.z, r.b.w};
-                    float acc[NB][4];
-#pragma unroll
-                    for (int nb = 0; nb < NB; nb++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) acc[nb][i] = 0.f;
-                    const uint4 *xu = xs + at.unit * (16 * M);
-#pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        uint32_t qa[4], qb[4];
-                        w4_dequant<E, ZERO>(wa[w], bias_a, qa);
-                        w4_dequant<E, ZERO>(wb[w], bias_b, qb);
-#pragma unroll
-                        for (int nb = 0; nb < NB; nb++) {
-                            uint4 x = make_uint4(0, 0, 0, 0);
-                            if (xoff[nb] >= 0) x = xu[w * (4 * M) + xoff[nb]];
-                            W4Type<E>::mma(acc[nb], qa[0], qb[0], qa[1], qb[1], x.x, x.y);
-                            W4Type<E>::mma(acc[nb], qa[2], qb[2], qa[3], qb[3], x.z, x.w);
-                        }
-                    }
-                    constexpr int S1 = W4Unit<GPU>::SCALES - 1;
-                    auto scale = [](uint16_t bits) { return W4Type<E>::to_f32(*reinterpret_cast<const E *>(&bits)); };
-                    const float sa0 = scale(r.sa[0]), sa1 = scale(r.sa[S1]), sb0 = scale(r.sb[0]), sb1 = scale(r.sb[S1]);
+                for (int w = 0; w < 4; w++) {
+                    uint32_t qa[4], qb[4];
+                    w4_dequant<E, ZERO>(qwa[w], minus_a, qa);
+                    w4_dequant<E, ZERO>(qwb[w], minus_b, qb);
 #pragma unroll
                     for (int nb = 0; nb < NB; nb++) {
-                        total[nb][0] = fmaf(sa0, acc[nb][0], total[nb][0]);
-                        total[nb][1] = fmaf(sa1, acc[nb][1], total[nb][1]);
-                        total[nb][2] = fmaf(sb0, acc[nb][2], total[nb][2]);
-                        total[nb][3] = fmaf(sb1, acc[nb][3], total[nb][3]);
+                        const uint4 x = *reinterpret_cast<const uint4 *>(smem + xaddr[nb] + u * xstep[nb] + w * 64);
+                        if (w == 0) W4Type<E>::mma_first(acc[nb], qa[0], qb[0], qa[1], qb[1], x.x, x.y);
+                        else W4Type<E>::mma(acc[nb], qa[0], qb[0], qa[1], qb[1], x.x, x.y);
+                        W4Type<E>::mma(acc[nb], qa[2], qb[2], qa[3], qb[3], x.z, x.w);
                     }
-                    load(r, ahead);
-                    ahead.unit += WK;
-                    settle(ahead);
-                    const int tile = at.tile;
-                    at.unit += WK;
-                    settle(at);
-                    if (at.tile != tile) {
+                }
+                constexpr int S1 = W4Unit<GPU>::SCALES - 1;
+                auto scale = [](uint16_t bits) { return W4Type<E>::to_f32(*reinterpret_cast<const E *>(&bits)); };
+                const float sa0 = scale(r.sa[0]), sa1 = scale(r.sa[S1]), sb0 = scale(r.sb[0]), sb1 = scale(r.sb[S1]);
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++) {
+                    total[nb][0] = fmaf(sa0, acc[nb][0], total[nb][0]);
+                    total[nb][1] = fmaf(sa1, acc[nb][1], total[nb][1]);
+                    total[nb][2] = fmaf(sb0, acc[nb][2], total[nb][2]);
+                    total[nb][3] = fmaf(sb1, acc[nb][3], total[nb][3]);
+                }
+            };
+            while (tile < tiles) {
+#pragma unroll
+                for (int d = 0; d < 2; d++) {
+                    if (tile >= tiles) break;
+                    compute_unit(ring[d][0], unit);
+#pragma unroll
+                    for (int i = 1; i < BATCH; i++)
+                        if (unit + i * WK < nu) compute_unit(ring[d][i], unit + i * WK);
+                    load(ring[d]);
+                    unit += BATCH * WK;
+                    if (unit >= nu) {
                         // the warp's share of this tile is complete: its partial sums go to its own slot
                         float *slot = part + (size_t)wk * M * p.block_rows + tile * T::TILE + g;
                         auto put = [&](int m, int row, float v) {
                             if (m >= M || tile * T::TILE + g + row >= rows) return;
+                            v *= W4Type<E>::OUT;
                             float *q = slot + m * p.block_rows + row;
                             *q = u0 == 0 ? v : *q + v;
                         };
@@ -328,6 +397,8 @@ __global__ void __launch_bounds__(32 * T::template WARPS<NB>, 1) w4_matvec_kerne
 #pragma unroll
                             for (int i = 0; i < 4; i++) total[nb][i] = 0.f;
                         }
+                        do tile += WR;
+                        while (tile < tiles && (unit = first_unit(tile)) >= nu);
                     }
                 }
             }
@@ -345,7 +416,7 @@ __global__ void __launch_bounds__(32 * T::template WARPS<NB>, 1) w4_matvec_kerne
 
 template <class T>
 struct W4MatvecLauncher {
-    static bool can_run(int M, int N, int K) { return M >= 1 && M <= T::MPAD && N >= 1 && K >= 32 && K % 32 == 0; }
+    static bool can_run(int M, int N, int K) { return M >= 1 && M <= T::MPAD && N >= 1 && K >= 32 && K % 32 == 0 && K <= 1 << 28; }
     // the family's figure, so that one workspace serves whichever W4A16 plugin is picked; nothing here touches it
     static size_t workspace_bytes(int, int, int) { return (size_t)2 * STREAMK_MAX_CTAS * 128 * 128 * sizeof(float); }
 
@@ -385,18 +456,17 @@ struct W4MatvecLauncher {
         // partial sums: rows of a CTA x M x WK floats; as many K slices as fit (a tile's bytes then arrive soonest), blocks of
         // rows when not even one slice of all rows does
         const int rows = (a.N + grid - 1) / grid, units = (a.K + T::UNIT - 1) / T::UNIT;
-        const int most_units = T::X_BYTES / (a.M * T::UNIT * 2), passes = (units + most_units - 1) / most_units;
+        const int most_units = T::X_BYTES / T::x_unit_bytes(a.M), passes = (units + most_units - 1) / most_units;
         p.units_per_pass = (units + passes - 1) / passes;
         const int slots = T::PART_BYTES / (int)sizeof(float) / a.M;
-        const int columns = a.M * (T::UNIT >> p.group_shift);
-        p.wk_shift = columns <= 16 ? 4 : 3;
+        p.wk_shift = a.M * (T::UNIT >> p.group_shift) <= 8 ? 4 : 3;
         while (p.wk_shift > 0 && ((1 << p.wk_shift) > p.units_per_pass || (rows << p.wk_shift) > slots)) p.wk_shift--;
         p.block_rows = rows;
         if (rows > slots) {
             const int blocks = (rows + slots / T::TILE * T::TILE - 1) / (slots / T::TILE * T::TILE);
             p.block_rows = ((rows + blocks - 1) / blocks + T::TILE - 1) / T::TILE * T::TILE;
         }
-        const int smem = T::PART_BYTES + p.units_per_pass * a.M * T::UNIT * 2;
+        const int smem = T::PART_BYTES + T::ZERO_BYTES + p.units_per_pass * T::x_unit_bytes(a.M);
         if (a.x_dtype == GEMM_X_F16) return launch<__half>(p, grid, smem, a.stream);
         return launch<__nv_bfloat16>(p, grid, smem, a.stream);
     }

@@ -72,7 +72,7 @@ class GemmConfig:
     def smem_bytes(self) -> int:
         """Dynamic shared memory of the kernel; must equal the traits' SMEM_ALLOC."""
         if self.dt == "w4a16" and self.bk == 32:   # W4MatvecTraits: partial sums + staged X (the largest launch)
-            return (52 + 160) * 1024
+            return (52 + 160) * 1024 + 256
         if self.dt == "w4a16" and self.bk == 128:   # W4A16TmemTraits: load ring only (16 KB packed + 4 activation boxes per stage); s = group slots in TMEM
             load_stage = 128 * 128 + 4 * (-(-self.bn * 128 // 1024) * 1024)
             load_stages = min(8, 200 * 1024 // load_stage)
@@ -103,7 +103,7 @@ class GemmConfig:
         if M <= 0 or N <= 0 or K <= 0:
             return False
         if self.dt == "w4a16" and self.bk == 32:   # matrix-vector plugins (K must also be whole scale groups)
-            return M <= self.bn and K % 32 == 0
+            return M <= self.bn and K % 32 == 0 and K <= 1 << 28
         if self.dt == "w4a16":   # decode kernel: M fits the padded UMMA N, whole 128-element scale groups
             return M <= self.bn and N % 8 == 0 and K % 128 == 0
         if (K * ELEM_BITS[self.dt]) % 128 != 0 or N % 8 != 0:
