@@ -85,7 +85,7 @@ struct GemmConfig {
     // a plugin reports the exact figure through gemm_smem_bytes()).
     size_t smem_bytes() const
     {
-        if (dt == GEMM_DT_W4A16 && bk == 32) return (52 + 160) * 1024 + 256;   // matrix-vector plugins: partial sums + staged X (the largest launch)
+        if (dt == GEMM_DT_W4A16 && bk == 32) return 232448;   // matrix-vector plugins: partial sums, weight ring, staged X (the largest launch)
         if (dt == GEMM_DT_W4A16 && bk == 128) {   // tensor-memory family: load ring only (16 KB packed + 4 activation boxes per stage)
             const size_t load_stage = 128 * 128 + 4 * (((size_t)bn * 128 + 1023) / 1024 * 1024);
             const size_t fit = (200 * 1024) / load_stage;

@@ -6,32 +6,30 @@
 //     y[m,n] = sum_g s[n,g] * sum_{k in g} (u[n,k] - z[n,g]) * x[m,k]         u = nibble, z = zero point
 //     signed weights: u = nibble ^ 8, z = 8
 //
-// u - z is an integer of at most 5 bits, exact in bf16 and fp16, and the products and sums are FP32: the only rounding to
-// fewer bits is the last one, of y.
+// What it has to do is read N * K / 2 bytes once, so the weights stream through a ring of each warp's own in shared memory
+// (16-byte asynchronous copies, no barrier between warps) and the sums are taken by the warp-level matrix instruction m16n8k16
+// with the 16 weight rows of a tile as A and up to 8 rows of X as the columns of B: FP32 FMAs alone would need 1.9 G of them
+// per row of X at 28672 x 8192, six times the time of the bytes for M = 8.
 //
-// What it has to do is read N * K / 2 bytes once, so the weights go from global memory straight to registers (16 bytes per
-// lane and load, several in flight, no shared memory, no barrier on their way) and the sums are taken by the warp-level
-// matrix instruction m16n8k16 with the 16 weight rows of a tile as A and the rows of X as the 8 columns of B: FP32 FMAs
-// alone would need 1.9 G of them per row of X at 28672 x 8192, six times the time of the bytes for M = 8.
-//
-// The order of k inside a sum is free, so it follows the packing: lane (g, c) = (lane / 4, lane % 4) of a warp reads
-// 16 bytes = 32 consecutive k of weight rows g and g + 8, the four lanes of a quad 128 k (a UNIT).  Of a word's eight
-// nibbles the pairs (0,4), (1,5), (2,6), (3,7) come out of one mask each as two 16-bit numbers, and X is staged in shared
-// memory in that order, fragment by fragment, so that one 16-byte load feeds two matrix instructions.
-// The masked bits are not moved into place: read as 16-bit floating point, a pattern below twice the smallest normal number
-// is that integer times the smallest subnormal, so bits 0-3 are q and bits 4-7 are 16 q of those, and one packed multiply-add
-// by a power of two turns either into (q - z) * 2^-6 (bf16; fp16: 2^-9), exactly: one shift, four logic instructions and
-// four multiply-adds for eight weights.  The sums are multiplied by 2^6 (2^9) at the end.
-//
-// Scales belong to (row, group) and are applied to FP32 sums, one multiply-add per group and accumulator.  A group of 128
-// is a unit.  Of smaller groups a unit holds GPU = 2 or 4, lane c's 32 elements in group c * GPU / 4: then a column of B is
-// a (row of X, group) pair, zero where the lane's elements are of another group, and the sums of the groups stay apart in
-// different columns.  NB column blocks of 8 hold the M * GPU columns.
+// A UNIT is 128 k of a tile: 16 rows of 64 bytes.  ldmatrix hands the 16 bytes of (row g, 32 k) to the four lanes of quad g, a
+// word each: lane (g, c) = (lane / 4, lane % 4) gets the eight k 8c .. 8c + 7 of rows g and g + 8.  The order of k inside a sum
+// is free, so it follows the packing: of a word's eight nibbles one mask takes a pair: (0,4), (1,5), and behind a shift (2,6),
+// (3,7); X is staged in that order, so that one 16-byte load is the B of two matrix instructions, 32 k.
+// The masked word IS two matrix operands: a 16-bit floating-point pattern below twice the smallest normal number is that
+// integer times the smallest subnormal d, and the matrix units take subnormals as they are.  So bits 0-3 are u * d and bits
+// 4-7 are 16 u * d, exactly; the pairs of either kind go to sums of their own (lo, hi) and lo + hi / 16 is sum u * x * d.
+// One shift and four logic instructions make eight weights.  Zero points are taken off as z * (sum of x over the group),
+// which the staging of X computes: lo starts at -z * sum x * d.  All of it is FP32; the only rounding to fewer bits is the last
+// one, of y.  (u and z are at most 15, so the difference loses at most four bits of FP32 against sums of u - z, far below the
+// last rounding.)
+// d = 2^-24 (fp16) leaves FP32 room for every x.  d = 2^-133 (bf16) does not: X is staged as x * 2^k, k = 100 where every
+// |x| is below 2^19 and some |x| of each row above 2^-40, else by row from its largest value.
+// Scales belong to (row, group) and are applied to the FP32 sums of a group, GPU = 1, 2 or 4 groups per unit.
 //
 // Work: CTA i takes the rows N * i / grid .. N * (i + 1) / grid (any boundary: every SM reads the same number of bytes),
-// cut into tiles of 16.  Its 16 (or 8) warps are WR groups over the tiles times WK slices over the units of K; the WK partial sums
-// of a tile meet in shared memory and are added in the order of the slices -- no atomics, the same result every run.
-// X is staged whole when it fits, else in passes over K with the partial sums kept.
+// cut into tiles of 16.  Its 16 warps are WR groups over the tiles times WK slices over K in batches of two units; the WK
+// partial sums of a tile meet in shared memory and are added in the order of the slices -- no atomics, the same result
+// every run.  X is staged whole when it fits, else in passes over K with the partial sums kept.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -55,56 +53,35 @@ struct W4MatvecParams {
     int block_rows;              // rows of W whose partial sums shared memory holds
     int units_per_pass;          // units (128 K-elements) of X that shared memory holds
     int wk_shift;                // log2(WK)
+    int scale_window, zero_window;       // scales / zero points reach the ring in words around them, else they are read when needed
+    const uint8_t *scales_end, *zeros_end;
 };
 
-// What depends on the 16-bit type: mma D = A * B + D (m16n8k16, D FP32; `first`: D = A * B), the packed multiply-add, and
-// the constants of the conversion: LOW * (q in bits 0-3) = HIGH * (q in bits 4-7) = q / OUT as packed numbers.
+// What depends on the 16-bit type: the matrix instruction m16n8k16 (D = A * B + C, C and D FP32), and the scaling of X.
 template <class T>
 struct W4Type;
 template <>
 struct W4Type<__nv_bfloat16> {
-    static constexpr uint32_t LOW = 0x7f007f00u, HIGH = 0x7d007d00u, NEG_LOW = 0xff00ff00u;      // 2^127, 2^123, -2^127
-    static constexpr uint32_t MINUS_8 = 0xbe00be00u;                                             // -8 / OUT
-    static constexpr float OUT = 64.f;
-    static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+    static constexpr bool RESCALE = true;
+    static constexpr int K_USUAL = 100;          // X is staged as x * 2^K_USUAL
+    static constexpr float OUT = 8589934592.f;   // 2^133 / 2^K_USUAL
+    static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3)
     {
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    }
-    static __device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
-    {
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-    }
-    static __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c)
-    {
-        uint32_t r;
-        asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-        return r;
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
     }
     static __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
     static __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
 };
 template <>
 struct W4Type<__half> {
-    static constexpr uint32_t LOW = 0x78007800u, HIGH = 0x68006800u, NEG_LOW = 0xf800f800u;      // 2^15, 2^11, -2^15
-    static constexpr uint32_t MINUS_8 = 0xa400a400u;                                             // -8 / OUT
-    static constexpr float OUT = 512.f;
-    static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+    static constexpr bool RESCALE = false;
+    static constexpr int K_USUAL = 0;
+    static constexpr float OUT = 16777216.f;     // 2^24
+    static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3)
     {
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    }
-    static __device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
-    {
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-    }
-    static __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c)
-    {
-        uint32_t r;
-        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-        return r;
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
     }
     static __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
     static __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
@@ -115,16 +92,23 @@ struct W4MatvecTraits {
     static constexpr int MPAD = MPAD_;       // most rows of X
     static constexpr int STAGES = STAGES_;
     static constexpr int EPI = EPI_;
-    // 16 warps of 128 registers; more column blocks need more registers: 8 warps
-    template <int NB>
-    static constexpr int WARPS = NB == 1 ? 16 : 8;
+    static constexpr int NB = MPAD_ / 8;             // column blocks
+    template <int GPU>
+    static constexpr int WARPS = NB == 1 && GPU < 4 ? 16 : 8;      // as the registers allow
+    static constexpr int IN_FLIGHT = 48;             // batches of two units in flight, all warps together
     static constexpr int TILE = 16, UNIT = 128;
-    static constexpr int PART_BYTES = 52 * 1024;     // partial sums
-    static constexpr int X_BYTES = 160 * 1024;       // staged X
-    static constexpr int ZERO_BYTES = 256;           // zeros that are read in the place of X
-    static constexpr int SMEM_ALLOC = PART_BYTES + ZERO_BYTES + X_BYTES;
-    static constexpr int X_ROW = 256 + 64;           // staged X, one unit of one row
-    static __host__ __device__ constexpr int x_unit_bytes(int M) { return M * X_ROW; }      // staged X, one unit
+    static constexpr int UNIT_BYTES = TILE * UNIT / 2;
+    // a batch in the ring: two units, then per row the scales of its 2 GPU groups and a word in front of them, then per row
+    // two words around its zero points
+    static __host__ __device__ constexpr int scale_pitch(int gpu) { return 8 * gpu; }
+    static __host__ __device__ constexpr int slot_bytes(int gpu) { return 2 * UNIT_BYTES + TILE * scale_pitch(gpu) + TILE * 8; }
+    static __host__ __device__ constexpr int ring_bytes(int gpu) { return IN_FLIGHT * slot_bytes(gpu); }
+    static constexpr int PART_BYTES = 26 * 1024;     // partial sums
+    static constexpr int ROW_BYTES = 256;            // per row of X: scaling, flags
+    static constexpr int SMEM_ALLOC = 227 * 1024;    // the rest: staged X and its sums
+    static __host__ __device__ constexpr int x_bytes(int gpu) { return SMEM_ALLOC - PART_BYTES - ROW_BYTES - ring_bytes(gpu); }
+    // staged X and sums of one unit
+    static __host__ __device__ constexpr int x_unit_bytes(int M, int gpu) { return M * UNIT * 2 + gpu * NB * 32; }
     static_assert(MPAD_ == 8 || MPAD_ == 16, "rows of X: up to 8 or 16");
 };
 
@@ -144,50 +128,139 @@ __device__ __forceinline__ void w4_store(const W4MatvecParams &p, int m, int n, 
     static_cast<E *>(p.Y)[at] = W4Type<E>::from_f32(v);
 }
 
-// the eight k of one packed word as four 16-bit pairs (0,4), (1,5), (2,6), (3,7), each (nibble - zero point) / OUT;
-// `minus` is the packed -zero point / OUT
-template <class E, bool ZERO>
-__device__ __forceinline__ void w4_dequant(uint32_t w, uint32_t minus, uint32_t (&out)[4])
+// asynchronous copies of global memory to shared; of `have` bytes, the rest of the piece is zeros
+__device__ __forceinline__ void w4_copy16(uint32_t dst, const uint8_t *src, int have)
 {
-    constexpr uint32_t FLIP = ZERO ? 0u : 0x00080008u;      // signed weights: flipping the top bit of a nibble adds 8
-    const uint32_t v = w >> 8;
-    auto pick = [](uint32_t x, uint32_t mask, uint32_t flip) {
-        uint32_t y;
-        asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(y) : "r"(x), "r"(mask), "r"(flip));      // (x & mask) ^ flip
-        return y;
-    };
-    out[0] = W4Type<E>::fma2(pick(w, 0x000f000fu, FLIP), W4Type<E>::LOW, minus);
-    out[1] = W4Type<E>::fma2(pick(w, 0x00f000f0u, FLIP << 4), W4Type<E>::HIGH, minus);
-    out[2] = W4Type<E>::fma2(pick(v, 0x000f000fu, FLIP), W4Type<E>::LOW, minus);
-    out[3] = W4Type<E>::fma2(pick(v, 0x00f000f0u, FLIP << 4), W4Type<E>::HIGH, minus);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have) : "memory");
+}
+__device__ __forceinline__ void w4_copy16(uint32_t dst, const uint8_t *src)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void w4_copy4(uint32_t dst, const uint8_t *src, int have)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(have) : "memory");
+}
+template <int BYTES>
+__device__ __forceinline__ void w4_copy_small(uint32_t dst, const uint8_t *src)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void w4_copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void w4_copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+__device__ __forceinline__ void w4_ldmatrix(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
-// one unit of one tile for one lane, as loaded
-template <int GPU>
-struct W4Unit {
-    static constexpr int SCALES = GPU == 1 ? 1 : 2;
-    uint4 a, b;                      // rows g and g + 8
-    uint16_t sa[SCALES], sb[SCALES];
-    uint8_t za, zb;
+// (w & mask) ^ flip: a pair of nibbles; flipping the top bit of a signed nibble makes it unsigned, 8 more
+__device__ __forceinline__ uint32_t w4_pick(uint32_t w, uint32_t mask, uint32_t flip)
+{
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(y) : "r"(w), "r"(mask), "r"(flip));
+    return y;
+}
+
+__device__ __forceinline__ float w4_power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }      // -126 <= e <= 127
+
+// per row of X, for one pass: its scaling, and what decides about it
+struct W4Rows {
+    float up[16];        // staged x = x * up * 2^K_USUAL
+    float down[16];      // 1 / up
+    int ordinary[16];    // some |x| is at least 2^-40 (bf16)
+    int top[16];         // largest finite exponent field
 };
 
-__device__ __forceinline__ uint4 w4_stream_load(const uint8_t *p)
+// Stages `nu` units of X from unit u0 on ([unit][32 k][m][c]: 8 values, 16 bytes), and their sums over the groups times
+// -8 d (signed) or -d ([unit][group][m]); x behind K is 0.  Returns whether this thread saw an |x| of 2^19 or more, or no
+// finite number (bf16).
+template <class E, int GPU, bool ZERO, class T>
+__device__ __forceinline__ bool w4_stage_x(const W4MatvecParams &p, uint4 *xs, float *sums, W4Rows *rows, int u0, int nu, bool usual)
 {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
+    const int M = p.M, K = p.K;
+    const E *X = static_cast<const E *>(p.X);
+    bool far = false;
+    const int pieces = nu * M * 16;                                 // (unit, m, 32 k, c)
+    constexpr int THREADS = 32 * T::template WARPS<GPU>;
+    const int rounds = (pieces + THREADS - 1) / THREADS;
+    for (int it = 0; it < rounds; it++) {
+        const int i = it * THREADS + threadIdx.x;
+        const int at = i & 15, m = (i >> 4) % M, u = (i >> 4) / M;
+        const int k = (u0 + u) * T::UNIT + at * 8;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (i < pieces && k < K) v = __ldg(reinterpret_cast<const uint4 *>(X + (size_t)m * K + k));
+        float sum = 0.f;
+        const float up = usual ? 1.f : rows->up[m];
+        uint32_t most = 0;
+        uint32_t q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float lo = W4Type<E>::to_f32(reinterpret_cast<const E *>(q + j)[0]), hi = W4Type<E>::to_f32(reinterpret_cast<const E *>(q + j)[1]);
+            if (W4Type<E>::RESCALE) {
+                most = max(most, max(q[j] & 0x7fff0000u, (q[j] << 16) & 0x7fff0000u));
+                lo *= up;
+                hi *= up;
+                const __nv_bfloat162 two = __floats2bfloat162_rn(lo * w4_power_of_two(W4Type<E>::K_USUAL), hi * w4_power_of_two(W4Type<E>::K_USUAL));
+                q[j] = *reinterpret_cast<const uint32_t *>(&two);
+            }
+            sum += lo;
+            sum += hi;
+        }
+        if (W4Type<E>::RESCALE && i < pieces) {
+            if (most >= 0x49000000u) far = true;                        // 2^19
+            if (most >= 0x2b800000u) rows->ordinary[m] = 1;             // 2^-40; every thread that gets here writes the same
+        }
+#pragma unroll
+        for (int o = 1; o < 16 / GPU; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (i >= pieces) continue;
+        if (at % (16 / GPU) == 0) sums[(u * GPU + at * GPU / 16) * (T::NB * 8) + m] = sum * (ZERO ? -1.f : -8.f) / W4Type<E>::OUT;
+        // the pairs (0,4), (2,6), (1,5), (3,7) of the eight values: operands of the lo sums, then of the hi sums
+        xs[((u * 4 + (at >> 2)) * M + m) * 4 + (at & 3)] =
+            make_uint4(__byte_perm(q[0], q[2], 0x5410), __byte_perm(q[1], q[3], 0x5410), __byte_perm(q[0], q[2], 0x7632), __byte_perm(q[1], q[3], 0x7632));
+    }
+    return far;
 }
 
-template <class E, int NB, int GPU, bool ZERO, class T>
-__global__ void __launch_bounds__(32 * T::template WARPS<NB>, 1) w4_matvec_kernel(const W4MatvecParams p)
+// The rows' scaling from their largest finite values in this pass (bf16 only; rare): brings them to 2^119 .. 2^120.
+template <class E, int THREADS, class T>
+__device__ __forceinline__ void w4_rescale_rows(const W4MatvecParams &p, W4Rows *rows, int u0, int nu)
 {
-    constexpr int WARPS = T::template WARPS<NB>, THREADS = 32 * WARPS;
-    constexpr int BATCH = NB == 8 ? 1 : NB == 1 ? 2 : 4;    // units that are loaded together; two batches in flight per warp
+    if (threadIdx.x < 16) rows->top[threadIdx.x] = 0;
+    __syncthreads();
+    const uint16_t *X = static_cast<const uint16_t *>(p.X);
+    const int k0 = u0 * T::UNIT, kn = min(nu * T::UNIT, p.K - k0);
+    for (int m = 0; m < p.M; m++) {
+        int top = 0;
+        for (int k = threadIdx.x; k < kn; k += THREADS) {
+            const int e = (X[(size_t)m * p.K + k0 + k] >> 7) & 255;
+            if (e != 255) top = max(top, e);
+        }
+        atomicMax(&rows->top[m], top);
+    }
+    __syncthreads();
+    if (threadIdx.x < p.M) {
+        // x * 2^k <= 2^120: the sum of a group stays finite; subnormal rows (exponent field 0) are below 2^-126
+        const int e = max(rows->top[threadIdx.x], 1) - 127, k = min(119 - e, 190) - W4Type<E>::K_USUAL;
+        rows->up[threadIdx.x] = w4_power_of_two(k);
+        rows->down[threadIdx.x] = w4_power_of_two(-k);
+    }
+    __syncthreads();
+}
+
+// WHOLE: K is whole batches and the scales and zero points are aligned like them, so that nothing is cut and every row's
+// share of a batch is one aligned piece.
+template <class E, int GPU, bool ZERO, bool WHOLE, class T>
+__global__ void __launch_bounds__(32 * T::template WARPS<GPU>, 1) w4_matvec_kernel(const W4MatvecParams p)
+{
+    constexpr int NB = T::NB, WARPS = T::template WARPS<GPU>, THREADS = 32 * WARPS, RING = T::IN_FLIGHT / WARPS;
+    constexpr int GROUP_SUBS = 4 / GPU;                  // pieces of 32 k in a group
+    constexpr int SLOT = T::slot_bytes(GPU), SCALES_AT = 2 * T::UNIT_BYTES, SCALE_PITCH = T::scale_pitch(GPU), ZEROS_AT = SCALES_AT + T::TILE * SCALE_PITCH;
+    constexpr int X_AT = T::PART_BYTES + T::ring_bytes(GPU) + T::ROW_BYTES;
     extern __shared__ __align__(16) uint8_t smem[];
     float *part = reinterpret_cast<float *>(smem);       // [WK][M][block_rows]
-    // X: 256 bytes per unit and m ([word 0..3][c]: 8 values), 320 apart, so that the eight lanes of a 16-byte access
-    // (two m) reach all banks; in front of it zeros for the lanes whose column is another group's
-    uint8_t *xs = smem + T::PART_BYTES + T::ZERO_BYTES;
+    W4Rows *xrows = reinterpret_cast<W4Rows *>(smem + X_AT - T::ROW_BYTES);
     const int lane = threadIdx.x & 31;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);                 // uniform over the warp, and known to be
     const int g = lane >> 2, c = lane & 3;
@@ -198,210 +271,256 @@ __global__ void __launch_bounds__(32 * T::template WARPS<NB>, 1) w4_matvec_kerne
     const int zero_pitch = (groups + 1) >> 1;
     const int units = (K + T::UNIT - 1) / T::UNIT;
     const uint32_t row_bytes = (uint32_t)K >> 1;
-    const uint32_t unit_bytes = T::x_unit_bytes(M);
+    const uint32_t sums_at = X_AT + p.units_per_pass * (M * 256);
     const int row_begin = (int)((long long)p.N * blockIdx.x / gridDim.x), row_end = (int)((long long)p.N * (blockIdx.x + 1) / gridDim.x);
+    const uint8_t *scales = static_cast<const uint8_t *>(p.scales);
 
-    // this lane's column of B in column block nb: row m of X, for the lane's own group only.  Columns behind the last may
-    // hold anything (they only reach their own sums, which nobody reads): they repeat the last row's.
-    uint32_t xaddr[NB], xstep[NB];
-    if (threadIdx.x < T::ZERO_BYTES / 16) reinterpret_cast<uint4 *>(smem + T::PART_BYTES)[threadIdx.x] = make_uint4(0, 0, 0, 0);
+    // The ring holds a unit as 16 rows of four 16-byte pieces; piece j of row r lies at (r, j ^ (r / 2 % 4)), so that the
+    // eight rows of a matrix reach all banks.  Copies: lane (g, c) brings piece c of rows g and g + 8.  ldmatrix: lane l names
+    // row l % 16 and piece l / 16 (then 2 more) of the four matrices (rows 0-7, 8-15) x (piece j, j + 1).
+    const uint32_t ring = smem_u32(smem) + T::PART_BYTES + warp * (RING * SLOT);
+    const uint32_t put_at = g * 64 + ((c ^ (g >> 1 & 3)) << 4);
+    const uint32_t get_at = (lane & 15) * 64 + (((lane >> 4) ^ (lane >> 1 & 3)) << 4);
+    // this lane's column of B in column block nb is row m of X; columns behind the last repeat it (nobody reads their sums)
+    uint32_t xbase[NB];
 #pragma unroll
-    for (int nb = 0; nb < NB; nb++) {
-        const int col = nb * 8 + g, m = min(col / GPU, M - 1);
-        const bool own = GPU == 1 || col % GPU == c * GPU / 4;
-        xaddr[nb] = own ? T::PART_BYTES + T::ZERO_BYTES + m * T::X_ROW + c * 16 : T::PART_BYTES;
-        xstep[nb] = own ? unit_bytes : 0;
-    }
+    for (int nb = 0; nb < NB; nb++) xbase[nb] = X_AT + min(nb * 8 + g, M - 1) * 64 + c * 16;
 
     for (int row0 = row_begin; row0 < row_end; row0 += p.block_rows) {
         const int rows = min(p.block_rows, row_end - row0);
         const int tiles = (rows + T::TILE - 1) / T::TILE;
         for (int u0 = 0; u0 < units; u0 += p.units_per_pass) {
             const int nu = min(p.units_per_pass, units - u0);       // units of this pass
-            // A warp's share of the pass is a sequence of units, WK apart in a tile, tiles WR apart.  The slices of a tile
-            // start rotated from tile to tile, so that a last, partial round of units falls on other warps.
-            const int turn = nu & (WK - 1);
-            auto first_unit = [&](int tile) { return (wk + tile * turn) & (WK - 1); };
-            const int tail = K & (T::UNIT - 1) ? units - 1 - u0 : -1;       // the unit that ends behind K
-            // loading side: place, the current tile's addresses (one for the warp) and the lane's offsets to them; rows
-            // behind the block's last are read as the last
-            int ld_tile = wr, ld_unit = 0;
-            const uint8_t *wt = nullptr, *st = nullptr, *zt = nullptr;
-            uint32_t wa = 0, wb = 0, sa = 0, sb = 0, za = 0, zb = 0;
+            const int batches = (nu + 1) >> 1;
+            // A warp's share of the pass is a sequence of batches, WK apart in a tile, tiles WR apart.  The slices of a tile
+            // start rotated from tile to tile, so that a last, partial round of batches falls on other warps.
+            const int turn = batches & (WK - 1);
+            auto first_batch = [&](int tile) { return (wk + tile * turn) & (WK - 1); };
+            // the batch that ends behind K, if one does: its missing pieces are zeros
+            const int cut = !WHOLE && (u0 + 2 * batches) * T::UNIT > K ? batches - 1 : -1;
+            // loading side: place, and this lane's addresses; rows behind the block's last are read as the last
+            int ld_tile = wr, ld_batch = 0;
+            const uint8_t *wa = nullptr, *wb = nullptr, *ls = nullptr, *lz = nullptr;
             auto enter_tile = [&]() {
-                while (ld_tile < tiles && (ld_unit = first_unit(ld_tile)) >= nu) ld_tile += WR;
+                while (ld_tile < tiles && (ld_batch = first_batch(ld_tile)) >= batches) ld_tile += WR;
                 if (ld_tile >= tiles) return;
-                const int last = rows - 1 - ld_tile * T::TILE;
-                const uint32_t ra = min(g, last), rb = min(g + 8, last);
-                const size_t r = row0 + ld_tile * T::TILE;
-                wt = p.W + r * row_bytes + (size_t)u0 * (T::UNIT / 2);
-                wa = ra * row_bytes + c * 16;
-                wb = rb * row_bytes + c * 16;
-                // scales of the groups of this lane's two accumulator columns (2c, 2c + 1)
-                st = static_cast<const uint8_t *>(p.scales) + (r * groups + (size_t)u0 * GPU) * 2;
-                sa = (ra * groups + (GPU == 4 ? 2 * (c & 1) : 0)) * 2;
-                sb = (rb * groups + (GPU == 4 ? 2 * (c & 1) : 0)) * 2;
-                if (ZERO) {
-                    zt = p.zeros + r * zero_pitch;
-                    za = ra * zero_pitch + (GPU == 4 ? c >> 1 : 0);
-                    zb = rb * zero_pitch + (GPU == 4 ? c >> 1 : 0);
-                }
+                const int t0 = ld_tile * T::TILE;
+                const size_t u = u0 + 2 * ld_batch;
+                wa = p.W + (size_t)(row0 + min(t0 + g, rows - 1)) * row_bytes + u * (T::UNIT / 2) + c * 16;
+                wb = p.W + (size_t)(row0 + min(t0 + g + 8, rows - 1)) * row_bytes + u * (T::UNIT / 2) + c * 16;
+                // scales and zero points are brought by lane l for row l % 16 (u is even: whole bytes of zero points)
+                const size_t r = row0 + min(t0 + (lane & 15), rows - 1);
+                ls = scales + (r * groups + u * GPU) * 2;
+                if (ZERO) lz = p.zeros + r * zero_pitch + u * GPU / 2;
             };
-            auto load_unit = [&](W4Unit<GPU> &r, int u) {
-                const uint8_t *w = wt + (size_t)u * (T::UNIT / 2), *s = st + (size_t)u * (GPU * 2);
-                // zero points: byte of the lane's group, (u * GPU + c * GPU / 4) / 2
-                const uint8_t *z = ZERO ? zt + (GPU == 4 ? 2 * (u0 + u) : GPU == 2 ? u0 + u : (u0 + u) >> 1) : nullptr;
-                if (u != tail) {
-                    r.a = w4_stream_load(w + wa);
-                    r.b = w4_stream_load(w + wb);
+            auto load = [&](int slot) {
+                if (ld_tile < tiles) {
+                    const uint32_t dst = ring + slot * SLOT;
 #pragma unroll
-                    for (int i = 0; i < W4Unit<GPU>::SCALES; i++) {
-                        r.sa[i] = __ldg(reinterpret_cast<const uint16_t *>(s + sa) + i);
-                        r.sb[i] = __ldg(reinterpret_cast<const uint16_t *>(s + sb) + i);
-                    }
-                    if (ZERO) {
-                        r.za = __ldg(z + za);
-                        r.zb = __ldg(z + zb);
-                    }
-                } else {
-                    r.a = r.b = make_uint4(0, 0, 0, 0);
-                    r.za = r.zb = 0;
-                    if ((u0 + u) * T::UNIT + c * 32 < K) {
-                        r.a = w4_stream_load(w + wa);
-                        r.b = w4_stream_load(w + wb);
-                        if (ZERO) {
-                            r.za = __ldg(z + za);
-                            r.zb = __ldg(z + zb);
+                    for (int i = 0; i < 2; i++) {
+                        if (WHOLE || ld_batch != cut) {
+                            w4_copy16(dst + put_at + i * T::UNIT_BYTES, wa + i * (T::UNIT / 2));
+                            w4_copy16(dst + put_at + i * T::UNIT_BYTES + 512, wb + i * (T::UNIT / 2));
+                        } else {
+                            const bool in_k = (u0 + 2 * ld_batch + i) * T::UNIT + c * 32 < K;
+                            w4_copy16(dst + put_at + i * T::UNIT_BYTES, in_k ? wa + i * (T::UNIT / 2) : p.W, in_k ? 16 : 0);
+                            w4_copy16(dst + put_at + i * T::UNIT_BYTES + 512, in_k ? wb + i * (T::UNIT / 2) : p.W, in_k ? 16 : 0);
                         }
                     }
-                    const int left = groups - (u0 + u) * GPU - (GPU == 4 ? 2 * (c & 1) : 0);
+                    const uint32_t dst_s = dst + SCALES_AT + (lane & 15) * SCALE_PITCH;
+                    if (WHOLE) {
+                        if (lane < 16) w4_copy_small<4 * GPU>(dst_s, ls);
+                    } else if (p.scale_window) {
+                        // words around them: from the word that holds the first, never behind the array's end
+                        const uint8_t *from = reinterpret_cast<const uint8_t *>(reinterpret_cast<uintptr_t>(ls) & ~(uintptr_t)3);
 #pragma unroll
-                    for (int i = 0; i < W4Unit<GPU>::SCALES; i++) {
-                        r.sa[i] = i < left ? __ldg(reinterpret_cast<const uint16_t *>(s + sa) + i) : (uint16_t)0;
-                        r.sb[i] = i < left ? __ldg(reinterpret_cast<const uint16_t *>(s + sb) + i) : (uint16_t)0;
+                        for (int w = 0; w <= GPU / 2; w++) {
+                            const int word = 2 * w + (lane >> 4);
+                            const long long left = p.scales_end - (from + 4 * word);
+                            if (word <= GPU) w4_copy4(dst_s + 4 * word, left > 0 ? from + 4 * word : scales, left >= 4 ? 4 : left > 0 ? (int)left : 0);
+                        }
+                    }
+                    if (ZERO && WHOLE && GPU == 4) {
+                        if (lane < 16) w4_copy_small<4>(dst + ZEROS_AT + lane * 8, lz);
+                    } else if (ZERO && (WHOLE || p.zero_window)) {
+                        const uint8_t *from = reinterpret_cast<const uint8_t *>(reinterpret_cast<uintptr_t>(lz) & ~(uintptr_t)3) + 4 * (lane >> 4);
+                        const long long left = p.zeros_end - from;
+                        w4_copy4(dst + ZEROS_AT + (lane & 15) * 8 + 4 * (lane >> 4), left > 0 ? from : p.zeros, left >= 4 ? 4 : left > 0 ? (int)left : 0);
+                    }
+                    ld_batch += WK;
+                    wa += WK * T::UNIT;
+                    wb += WK * T::UNIT;
+                    ls += WK * GPU * 4;
+                    if (ZERO) lz += WK * GPU;
+                    if (ld_batch >= batches) {
+                        ld_tile += WR;
+                        enter_tile();
                     }
                 }
-            };
-            auto load = [&](W4Unit<GPU> (&r)[BATCH]) {
-                if (ld_tile >= tiles) return;
-                load_unit(r[0], ld_unit);
-#pragma unroll
-                for (int i = 1; i < BATCH; i++)
-                    if (ld_unit + i * WK < nu) load_unit(r[i], ld_unit + i * WK);
-                ld_unit += BATCH * WK;
-                if (ld_unit >= nu) {
-                    ld_tile += WR;
-                    enter_tile();
-                }
+                w4_copies_commit();
             };
             enter_tile();
-            int tile = ld_tile, unit = ld_unit;                             // computing side
-            W4Unit<GPU> ring[2][BATCH];
-            load(ring[0]);
-            load(ring[1]);
+            int tile = ld_tile, batch = ld_batch;                           // computing side
+#pragma unroll
+            for (int d = 0; d < RING; d++) load(d);
             // stage X while the first weights are on their way; the pass before has to be through with its own
             if (units > p.units_per_pass || row0 == row_begin) {
-                const E *X = static_cast<const E *>(p.X);
-                __syncthreads();
-                const int pieces = nu * 2 * M * 4;                  // (unit, half of the words, m, c): 16 values, 32 bytes each
-                for (int i = threadIdx.x; i < pieces; i += THREADS) {
-                    const int xc = i & 3, m = (i >> 2) % M, uh = (i >> 2) / M;
-                    const int k = (u0 + (uh >> 1)) * T::UNIT + xc * 32 + (uh & 1) * 16;
-                    uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-                    if (k < K) {
-                        const uint4 *src = reinterpret_cast<const uint4 *>(X + (size_t)m * K + k);
-                        v[0] = __ldg(src);
-                        v[1] = __ldg(src + 1);
-                    }
-                    uint4 *dst = reinterpret_cast<uint4 *>(xs + (uh >> 1) * unit_bytes + m * T::X_ROW + (uh & 1) * 128 + xc * 16);
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        dst[h * 4] = make_uint4(__byte_perm(v[h].x, v[h].z, 0x5410), __byte_perm(v[h].x, v[h].z, 0x7632),
-                                                __byte_perm(v[h].y, v[h].w, 0x5410), __byte_perm(v[h].y, v[h].w, 0x7632));
+                if (u0 != 0 || row0 != row_begin) __syncthreads();
+                if (threadIdx.x < 16) {
+                    xrows->ordinary[threadIdx.x] = 0;
+                    xrows->down[threadIdx.x] = 1.f;
                 }
                 __syncthreads();
+#pragma unroll 1
+                for (bool usual = true;; usual = false) {
+                    const bool far = w4_stage_x<E, GPU, ZERO, T>(p, reinterpret_cast<uint4 *>(smem + X_AT), reinterpret_cast<float *>(smem + sums_at), xrows, u0, 2 * batches, usual);
+                    bool again = __syncthreads_or(far) && W4Type<E>::RESCALE;
+                    if (W4Type<E>::RESCALE)
+                        for (int m = 0; m < M; m++) again = again || !xrows->ordinary[m];
+                    if (!again || !usual) break;
+                    w4_rescale_rows<E, THREADS, T>(p, xrows, u0, nu);
+                }
             }
             float total[NB][4];
 #pragma unroll
             for (int nb = 0; nb < NB; nb++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) total[nb][i] = 0.f;
-            auto compute_unit = [&](const W4Unit<GPU> &r, int u) {
-                uint32_t minus_a = W4Type<E>::MINUS_8, minus_b = W4Type<E>::MINUS_8;
-                if (ZERO) {
-                    const int shift = GPU == 4 ? 4 * (c & 1) : GPU == 2 ? 4 * (c >> 1) : 4 * ((u0 + u) & 1);
-                    minus_a = W4Type<E>::fma2(((uint32_t)(r.za >> shift) & 15u) * 0x00010001u, W4Type<E>::NEG_LOW, 0u);
-                    minus_b = W4Type<E>::fma2(((uint32_t)(r.zb >> shift) & 15u) * 0x00010001u, W4Type<E>::NEG_LOW, 0u);
-                }
-                const uint32_t qwa[4] = {r.a.x, r.a.y, r.a.z, r.a.w}, qwb[4] = {r.b.x, r.b.y, r.b.z, r.b.w};
-                float acc[NB][4];
-#pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    uint32_t qa[4], qb[4];
-                    w4_dequant<E, ZERO>(qwa[w], minus_a, qa);
-                    w4_dequant<E, ZERO>(qwb[w], minus_b, qb);
-#pragma unroll
-                    for (int nb = 0; nb < NB; nb++) {
-                        const uint4 x = *reinterpret_cast<const uint4 *>(smem + xaddr[nb] + u * xstep[nb] + w * 64);
-                        if (w == 0) W4Type<E>::mma_first(acc[nb], qa[0], qb[0], qa[1], qb[1], x.x, x.y);
-                        else W4Type<E>::mma(acc[nb], qa[0], qb[0], qa[1], qb[1], x.x, x.y);
-                        W4Type<E>::mma(acc[nb], qa[2], qb[2], qa[3], qb[3], x.z, x.w);
+            // scales of unit u (the i-th of its batch) for row `row` of the tile, row ra of W: GPU times 16 bits
+            auto scales_of = [&](uint32_t (&out)[(GPU + 1) / 2], const uint8_t *slot, int row, size_t ra, int u, int i) {
+                if (WHOLE) {
+                    const uint8_t *at = slot + SCALES_AT + row * SCALE_PITCH + i * GPU * 2;
+                    if constexpr (GPU == 1) out[0] = *reinterpret_cast<const uint16_t *>(at);
+                    else if constexpr (GPU == 2) out[0] = *reinterpret_cast<const uint32_t *>(at);
+                    else {
+                        const uint2 v = *reinterpret_cast<const uint2 *>(at);
+                        out[0] = v.x;
+                        out[(GPU + 1) / 2 - 1] = v.y;
                     }
-                }
-                constexpr int S1 = W4Unit<GPU>::SCALES - 1;
-                auto scale = [](uint16_t bits) { return W4Type<E>::to_f32(*reinterpret_cast<const E *>(&bits)); };
-                const float sa0 = scale(r.sa[0]), sa1 = scale(r.sa[S1]), sb0 = scale(r.sb[0]), sb1 = scale(r.sb[S1]);
+                } else {
+                    // (the window starts with the word that holds the first scale; its base is 4-byte aligned)
+                    const uint16_t *at = p.scale_window ? reinterpret_cast<const uint16_t *>(slot + SCALES_AT + row * SCALE_PITCH + (ra * groups & 1) * 2) + i * GPU
+                                                           : reinterpret_cast<const uint16_t *>(scales) + ra * groups + (size_t)u * GPU;
+                    uint32_t v[4] = {0, 0, 0, 0};
 #pragma unroll
-                for (int nb = 0; nb < NB; nb++) {
-                    total[nb][0] = fmaf(sa0, acc[nb][0], total[nb][0]);
-                    total[nb][1] = fmaf(sa1, acc[nb][1], total[nb][1]);
-                    total[nb][2] = fmaf(sb0, acc[nb][2], total[nb][2]);
-                    total[nb][3] = fmaf(sb1, acc[nb][3], total[nb][3]);
+                    for (int j = 0; j < GPU; j++)
+                        if (u * GPU + j < groups) v[j] = at[j];
+#pragma unroll
+                    for (int w = 0; w < (GPU + 1) / 2; w++) out[w] = v[2 * w] | v[2 * w + 1] << 16;
                 }
             };
-            while (tile < tiles) {
+            // zero points of the unit: GPU nibbles
+            auto zeros_of = [&](const uint8_t *slot, int row, size_t ra, int u, int i) -> uint32_t {
+                if constexpr (WHOLE && GPU == 4) {
+                    return *reinterpret_cast<const uint16_t *>(slot + ZEROS_AT + row * 8 + 2 * i);
+                } else {
+                    // byte of the batch's first group; its low bits say where the window starts
+                    const size_t z = ra * zero_pitch + (size_t)(u - i) * GPU / 2;
+                    const bool window = WHOLE || p.zero_window;
+                    const uint8_t *at = window ? slot + ZEROS_AT + row * 8 + (z & 3) : p.zeros + z;
+                    if (!window && u * GPU >= groups) return 0;                   // (the ring has zeros there or bytes of the array)
+                    if constexpr (GPU == 1) return at[0] >> (4 * i);
+                    else if constexpr (GPU == 2) return at[i];
+                    else return at[2 * i] | (window || u * GPU + 2 < groups ? (uint32_t)at[2 * i + 1] << 8 : 0u);
+                }
+            };
+            auto compute = [&](const uint8_t *slot, uint32_t from, int i) {
+                constexpr uint32_t FLIP = ZERO ? 0u : 0x00080008u;
+                const int u = 2 * batch + i;
+                const size_t ra = row0 + min(tile * T::TILE + g, rows - 1), rb = row0 + min(tile * T::TILE + g + 8, rows - 1);
+                uint32_t sa[(GPU + 1) / 2], sb[(GPU + 1) / 2];
+                scales_of(sa, slot, g, ra, u0 + u, i);
+                scales_of(sb, slot, g + 8, rb, u0 + u, i);
+                uint32_t za = 0, zb = 0;
+                if (ZERO) {
+                    za = zeros_of(slot, g, ra, u0 + u, i);
+                    zb = zeros_of(slot, g + 8, rb, u0 + u, i);
+                }
+                uint32_t xu[NB];
 #pragma unroll
-                for (int d = 0; d < 2; d++) {
-                    if (tile >= tiles) break;
-                    compute_unit(ring[d][0], unit);
+                for (int nb = 0; nb < NB; nb++) xu[nb] = xbase[nb] + u * (256 * M);
+                float lo[NB][4], hi[NB][4];
 #pragma unroll
-                    for (int i = 1; i < BATCH; i++)
-                        if (unit + i * WK < nu) compute_unit(ring[d][i], unit + i * WK);
-                    load(ring[d]);
-                    unit += BATCH * WK;
-                    if (unit >= nu) {
-                        // the warp's share of this tile is complete: its partial sums go to its own slot
-                        float *slot = part + (size_t)wk * M * p.block_rows + tile * T::TILE + g;
-                        auto put = [&](int m, int row, float v) {
-                            if (m >= M || tile * T::TILE + g + row >= rows) return;
-                            v *= W4Type<E>::OUT;
-                            float *q = slot + m * p.block_rows + row;
-                            *q = u0 == 0 ? v : *q + v;
-                        };
+                for (int half = 0; half < 2; half++) {
+                    uint32_t q[4];                       // rows g, g + 8 of piece 2 half, then of piece 2 half + 1
+                    w4_ldmatrix(q, half ? from ^ 32 : from);
+#pragma unroll
+                    for (int sub = 0; sub < 2; sub++) {
+                        const int j = 2 * half + sub;
+                        const uint32_t qa = q[2 * sub], qb = q[2 * sub + 1], va = qa >> 8, vb = qb >> 8;
+                        const uint32_t la0 = w4_pick(qa, 0x000f000fu, FLIP), lb0 = w4_pick(qb, 0x000f000fu, FLIP);
+                        const uint32_t la1 = w4_pick(va, 0x000f000fu, FLIP), lb1 = w4_pick(vb, 0x000f000fu, FLIP);
+                        const uint32_t ha0 = w4_pick(qa, 0x00f000f0u, FLIP << 4), hb0 = w4_pick(qb, 0x00f000f0u, FLIP << 4);
+                        const uint32_t ha1 = w4_pick(va, 0x00f000f0u, FLIP << 4), hb1 = w4_pick(vb, 0x00f000f0u, FLIP << 4);
+                        const int grp = j / GROUP_SUBS;
+                        float fa = 1.f, fb = 1.f;
+                        if (ZERO && j % GROUP_SUBS == 0) {      // 2^23 + z is exact in FP32
+                            fa = __uint_as_float((za >> (4 * grp) & 15u) | 0x4b000000u) - 8388608.f;
+                            fb = __uint_as_float((zb >> (4 * grp) & 15u) | 0x4b000000u) - 8388608.f;
+                        }
 #pragma unroll
                         for (int nb = 0; nb < NB; nb++) {
-                            if constexpr (GPU == 1) {
-                                put(nb * 8 + 2 * c, 0, total[nb][0]);
-                                put(nb * 8 + 2 * c + 1, 0, total[nb][1]);
-                                put(nb * 8 + 2 * c, 8, total[nb][2]);
-                                put(nb * 8 + 2 * c + 1, 8, total[nb][3]);
-                            } else if constexpr (GPU == 2) {
-                                put(nb * 4 + c, 0, total[nb][0] + total[nb][1]);
-                                put(nb * 4 + c, 8, total[nb][2] + total[nb][3]);
+                            const uint4 x = *reinterpret_cast<const uint4 *>(smem + xu[nb] + j * (64 * M));
+                            if (j % GROUP_SUBS == 0) {
+                                const float2 s = *reinterpret_cast<const float2 *>(smem + sums_at + (u * GPU + grp) * (NB * 32) + nb * 32 + c * 8);
+                                W4Type<E>::mma(lo[nb], la0, lb0, la1, lb1, x.x, x.y, fa * s.x, fa * s.y, fb * s.x, fb * s.y);
+                                W4Type<E>::mma(hi[nb], ha0, hb0, ha1, hb1, x.z, x.w, 0.f, 0.f, 0.f, 0.f);
                             } else {
-                                float v0 = total[nb][0] + total[nb][1], v1 = total[nb][2] + total[nb][3];
-                                v0 += __shfl_xor_sync(0xffffffffu, v0, 1);
-                                v1 += __shfl_xor_sync(0xffffffffu, v1, 1);
-                                put(nb * 2 + (c >> 1), (c & 1) * 8, (c & 1) ? v1 : v0);
+                                W4Type<E>::mma(lo[nb], la0, lb0, la1, lb1, x.x, x.y, lo[nb][0], lo[nb][1], lo[nb][2], lo[nb][3]);
+                                W4Type<E>::mma(hi[nb], ha0, hb0, ha1, hb1, x.z, x.w, hi[nb][0], hi[nb][1], hi[nb][2], hi[nb][3]);
                             }
-#pragma unroll
-                            for (int i = 0; i < 4; i++) total[nb][i] = 0.f;
                         }
-                        do tile += WR;
-                        while (tile < tiles && (unit = first_unit(tile)) >= nu);
+                        if ((j + 1) % GROUP_SUBS == 0) {
+                            auto scale = [](uint32_t word, int which) {
+                                const uint16_t bits = (uint16_t)(which ? word >> 16 : word);
+                                return W4Type<E>::to_f32(*reinterpret_cast<const E *>(&bits));
+                            };
+                            const float s_a = scale(sa[grp / 2], grp & 1), s_b = scale(sb[grp / 2], grp & 1);
+#pragma unroll
+                            for (int nb = 0; nb < NB; nb++) {
+                                total[nb][0] = fmaf(s_a, fmaf(hi[nb][0], 0.0625f, lo[nb][0]), total[nb][0]);
+                                total[nb][1] = fmaf(s_a, fmaf(hi[nb][1], 0.0625f, lo[nb][1]), total[nb][1]);
+                                total[nb][2] = fmaf(s_b, fmaf(hi[nb][2], 0.0625f, lo[nb][2]), total[nb][2]);
+                                total[nb][3] = fmaf(s_b, fmaf(hi[nb][3], 0.0625f, lo[nb][3]), total[nb][3]);
+                            }
+                        }
                     }
                 }
+            };
+            int slot = 0;
+            while (tile < tiles) {
+                w4_copies_wait<RING - 1>();
+                __syncwarp();                            // the other lanes' copies too
+#pragma unroll
+                for (int i = 0; i < 2; i++) compute(smem + T::PART_BYTES + (warp * RING + slot) * SLOT, ring + slot * SLOT + get_at + i * T::UNIT_BYTES, i);
+                __syncwarp();                            // every lane has read the slot
+                load(slot);
+                slot = slot == RING - 1 ? 0 : slot + 1;
+                batch += WK;
+                if (batch >= batches) {
+                    // the warp's share of this tile is complete: its partial sums go to its own slot
+                    float *to = part + (size_t)wk * M * p.block_rows + tile * T::TILE + g;
+                    auto put = [&](int m, int row, float v) {
+                        if (m >= M || tile * T::TILE + g + row >= rows) return;
+                        v *= W4Type<E>::OUT;
+                        if (W4Type<E>::RESCALE) v *= xrows->down[m];
+                        float *q = to + m * p.block_rows + row;
+                        *q = u0 == 0 ? v : *q + v;
+                    };
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++) {
+                        put(nb * 8 + 2 * c, 0, total[nb][0]);
+                        put(nb * 8 + 2 * c + 1, 0, total[nb][1]);
+                        put(nb * 8 + 2 * c, 8, total[nb][2]);
+                        put(nb * 8 + 2 * c + 1, 8, total[nb][3]);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) total[nb][i] = 0.f;
+                    }
+                    do tile += WR;
+                    while (tile < tiles && (batch = first_batch(tile)) >= batches);
+                }
             }
+            w4_copies_wait<0>();
         }
         __syncthreads();
         for (int i = threadIdx.x; i < rows * M; i += THREADS) {
@@ -455,20 +574,28 @@ struct W4MatvecLauncher {
         if (grid > a.N) grid = a.N;
         // partial sums: rows of a CTA x M x WK floats; as many K slices as fit (a tile's bytes then arrive soonest), blocks of
         // rows when not even one slice of all rows does
-        const int rows = (a.N + grid - 1) / grid, units = (a.K + T::UNIT - 1) / T::UNIT;
-        const int most_units = T::X_BYTES / T::x_unit_bytes(a.M), passes = (units + most_units - 1) / most_units;
-        p.units_per_pass = (units + passes - 1) / passes;
+        const int gpu = T::UNIT >> p.group_shift, rows = (a.N + grid - 1) / grid, units = (a.K + T::UNIT - 1) / T::UNIT;
+        const int most_units = T::x_bytes(gpu) / T::x_unit_bytes(a.M, gpu) / 2 * 2, passes = (units + most_units - 1) / most_units;
+        p.units_per_pass = ((units + passes - 1) / passes + 1) / 2 * 2;
         const int slots = T::PART_BYTES / (int)sizeof(float) / a.M;
-        p.wk_shift = a.M * (T::UNIT >> p.group_shift) <= 8 ? 4 : 3;
-        while (p.wk_shift > 0 && ((1 << p.wk_shift) > p.units_per_pass || (rows << p.wk_shift) > slots)) p.wk_shift--;
+        p.wk_shift = T::NB == 1 && gpu < 4 ? 4 : 3;
+        while (p.wk_shift > 0 && ((2 << p.wk_shift) > p.units_per_pass || (rows << p.wk_shift) > slots)) p.wk_shift--;
         p.block_rows = rows;
         if (rows > slots) {
             const int blocks = (rows + slots / T::TILE * T::TILE - 1) / (slots / T::TILE * T::TILE);
             p.block_rows = ((rows + blocks - 1) / blocks + T::TILE - 1) / T::TILE * T::TILE;
         }
-        const int smem = T::PART_BYTES + T::ZERO_BYTES + p.units_per_pass * T::x_unit_bytes(a.M);
-        if (a.x_dtype == GEMM_X_F16) return launch<__half>(p, grid, smem, a.stream);
-        return launch<__nv_bfloat16>(p, grid, smem, a.stream);
+        // how scales and zero points come: with whole batches, else in words around them (base 4-byte aligned), else one by one
+        // when they are needed
+        const bool whole = a.K % (2 * T::UNIT) == 0 && bits(a.w_scale) % (4 * gpu) == 0 && bits(a.w_zero) % 4 == 0;
+        p.scale_window = bits(a.w_scale) % 4 == 0;
+        p.zero_window = bits(a.w_zero) % 4 == 0;
+        const size_t groups = (size_t)a.K / a.group_size;
+        p.scales_end = static_cast<const uint8_t *>(a.w_scale) + (size_t)a.N * groups * 2;
+        p.zeros_end = a.w_zero ? p.zeros + (size_t)a.N * ((groups + 1) / 2) : nullptr;
+        const int smem = T::PART_BYTES + T::ring_bytes(gpu) + T::ROW_BYTES + p.units_per_pass * T::x_unit_bytes(a.M, gpu);
+        if (a.x_dtype == GEMM_X_F16) return launch<__half>(p, whole, grid, smem, a.stream);
+        return launch<__nv_bfloat16>(p, whole, grid, smem, a.stream);
     }
 
 private:
@@ -488,42 +615,30 @@ private:
     }
 
     template <class E>
-    static int launch(const W4MatvecParams &p, int grid, int smem, cudaStream_t stream)
+    static int launch(const W4MatvecParams &p, bool whole, int grid, int smem, cudaStream_t stream)
     {
-        if (p.zeros) return launch_groups<E, true>(p, grid, smem, stream);
-        return launch_groups<E, false>(p, grid, smem, stream);
+        if (p.zeros) return whole ? launch_groups<E, true, true>(p, grid, smem, stream) : launch_groups<E, true, false>(p, grid, smem, stream);
+        return whole ? launch_groups<E, false, true>(p, grid, smem, stream) : launch_groups<E, false, false>(p, grid, smem, stream);
     }
-    template <class E, bool ZERO>
+    template <class E, bool ZERO, bool WHOLE>
     static int launch_groups(const W4MatvecParams &p, int grid, int smem, cudaStream_t stream)
     {
-        if (p.group_shift == 7) return launch_columns<E, ZERO, 1>(p, grid, smem, stream);
-        if (p.group_shift == 6) return launch_columns<E, ZERO, 2>(p, grid, smem, stream);
-        return launch_columns<E, ZERO, 4>(p, grid, smem, stream);
+        if (p.group_shift == 7) return launch_kernel<E, ZERO, WHOLE, 1>(p, grid, smem, stream);
+        if (p.group_shift == 6) return launch_kernel<E, ZERO, WHOLE, 2>(p, grid, smem, stream);
+        return launch_kernel<E, ZERO, WHOLE, 4>(p, grid, smem, stream);
     }
-    template <class E, bool ZERO, int GPU>
-    static int launch_columns(const W4MatvecParams &p, int grid, int smem, cudaStream_t stream)
-    {
-        const int columns = p.M * GPU;
-        if (columns <= 8) return launch_kernel<E, ZERO, GPU, 1>(p, grid, smem, stream);
-        if constexpr (T::MPAD * GPU >= 16)
-            if (columns <= 16) return launch_kernel<E, ZERO, GPU, 2>(p, grid, smem, stream);
-        if constexpr (T::MPAD * GPU >= 32)
-            if (columns <= 32) return launch_kernel<E, ZERO, GPU, 4>(p, grid, smem, stream);
-        if constexpr (T::MPAD * GPU >= 64) return launch_kernel<E, ZERO, GPU, 8>(p, grid, smem, stream);
-        return set_error(GEMM_ERR_SHAPE, "%d rows do not fit this configuration", p.M);
-    }
-    template <class E, bool ZERO, int GPU, int NB>
+    template <class E, bool ZERO, bool WHOLE, int GPU>
     static int launch_kernel(const W4MatvecParams &p, int grid, int smem, cudaStream_t stream)
     {
         static std::atomic<bool> attr_set[MAX_DEVICES];
         int dev = 0;
         SM100_CUDA_TRY(cudaGetDevice(&dev));
-        auto *kernel = w4_matvec_kernel<E, NB, GPU, ZERO, T>;
+        auto *kernel = w4_matvec_kernel<E, GPU, ZERO, WHOLE, T>;
         if (!attr_set[dev].load(std::memory_order_acquire)) {
             SM100_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM_ALLOC));
             attr_set[dev].store(true, std::memory_order_release);
         }
-        kernel<<<grid, 32 * T::template WARPS<NB>, smem, stream>>>(p);
+        kernel<<<grid, 32 * T::template WARPS<GPU>, smem, stream>>>(p);
         SM100_CUDA_TRY(cudaGetLastError());
         return GEMM_OK;
     }

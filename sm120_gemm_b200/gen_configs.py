@@ -71,8 +71,8 @@ class GemmConfig:
 
     def smem_bytes(self) -> int:
         """Dynamic shared memory of the kernel; must equal the traits' SMEM_ALLOC."""
-        if self.dt == "w4a16" and self.bk == 32:   # W4MatvecTraits: partial sums + staged X (the largest launch)
-            return (52 + 160) * 1024 + 256
+        if self.dt == "w4a16" and self.bk == 32:   # W4MatvecTraits: partial sums, weight ring, staged X (the largest launch)
+            return MAX_SMEM
         if self.dt == "w4a16" and self.bk == 128:   # W4A16TmemTraits: load ring only (16 KB packed + 4 activation boxes per stage); s = group slots in TMEM
             load_stage = 128 * 128 + 4 * (-(-self.bn * 128 // 1024) * 1024)
             load_stages = min(8, 200 * 1024 // load_stage)
