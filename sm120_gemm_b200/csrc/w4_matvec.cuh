@@ -94,7 +94,7 @@ struct W4MatvecTraits {
     static constexpr int EPI = EPI_;
     static constexpr int NB = MPAD_ / 8;             // column blocks
     template <int GPU>
-    static constexpr int WARPS = NB == 1 && GPU < 4 ? 16 : 8;      // as the registers allow
+    static constexpr int WARPS = NB == 1 && GPU < 2 ? 16 : 8;      // as the registers allow
     static constexpr int IN_FLIGHT = 48;             // batches of two units in flight, all warps together
     static constexpr int TILE = 16, UNIT = 128;
     static constexpr int UNIT_BYTES = TILE * UNIT / 2;
@@ -107,8 +107,9 @@ struct W4MatvecTraits {
     static constexpr int ROW_BYTES = 256;            // per row of X: scaling, flags
     static constexpr int SMEM_ALLOC = 227 * 1024;    // the rest: staged X and its sums
     static __host__ __device__ constexpr int x_bytes(int gpu) { return SMEM_ALLOC - PART_BYTES - ROW_BYTES - ring_bytes(gpu); }
-    // staged X and sums of one unit
-    static __host__ __device__ constexpr int x_unit_bytes(int M, int gpu) { return M * UNIT * 2 + gpu * NB * 32; }
+    // staged X: rows 64 bytes longer than their units, so that the eight lanes of a 16-byte access (two rows) reach all banks
+    static __host__ __device__ constexpr int x_row_bytes(int units) { return units * UNIT * 2 + 64; }
+    static __host__ __device__ constexpr int staged_bytes(int M, int units, int gpu) { return M * x_row_bytes(units) + units * gpu * NB * 32; }
     static_assert(MPAD_ == 8 || MPAD_ == 16, "rows of X: up to 8 or 16");
 };
 
@@ -155,12 +156,20 @@ __device__ __forceinline__ void w4_ldmatrix(uint32_t (&r)[4], uint32_t addr)
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
-// (w & mask) ^ flip: a pair of nibbles; flipping the top bit of a signed nibble makes it unsigned, 8 more
-__device__ __forceinline__ uint32_t w4_pick(uint32_t w, uint32_t mask, uint32_t flip)
+// (w & MASK) ^ flip: a pair of nibbles; flipping the top bit of a signed nibble makes it unsigned, 8 more.  One instruction
+// has room for one constant; `flip` is a register.
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t w4_pick(uint32_t w, uint32_t flip)
 {
     uint32_t y;
-    asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(y) : "r"(w), "r"(mask), "r"(flip));
+    asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(y) : "r"(w), "n"(MASK), "r"(flip));
     return y;
+}
+// a constant that stays in its register (the compiler would make it anew at every use)
+__device__ __forceinline__ uint32_t w4_keep(uint32_t v)
+{
+    asm volatile("" : "+r"(v));
+    return v;
 }
 
 __device__ __forceinline__ float w4_power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }      // -126 <= e <= 127
@@ -173,7 +182,7 @@ struct W4Rows {
     int top[16];         // largest finite exponent field
 };
 
-// Stages `nu` units of X from unit u0 on ([unit][32 k][m][c]: 8 values, 16 bytes), and their sums over the groups times
+// Stages `nu` units of X from unit u0 on ([m][unit][32 k][c]: 8 values, 16 bytes), and their sums over the groups times
 // -8 d (signed) or -d ([unit][group][m]); x behind K is 0.  Returns whether this thread saw an |x| of 2^19 or more, or no
 // finite number (bf16).
 template <class E, int GPU, bool ZERO, class T>
@@ -217,7 +226,7 @@ __device__ __forceinline__ bool w4_stage_x(const W4MatvecParams &p, uint4 *xs, f
         if (i >= pieces) continue;
         if (at % (16 / GPU) == 0) sums[(u * GPU + at * GPU / 16) * (T::NB * 8) + m] = sum * (ZERO ? -1.f : -8.f) / W4Type<E>::OUT;
         // the pairs (0,4), (2,6), (1,5), (3,7) of the eight values: operands of the lo sums, then of the hi sums
-        xs[((u * 4 + (at >> 2)) * M + m) * 4 + (at & 3)] =
+        xs[m * (T::x_row_bytes(p.units_per_pass) / 16) + u * 16 + at] =
             make_uint4(__byte_perm(q[0], q[2], 0x5410), __byte_perm(q[1], q[3], 0x5410), __byte_perm(q[0], q[2], 0x7632), __byte_perm(q[1], q[3], 0x7632));
     }
     return far;
@@ -271,9 +280,10 @@ __global__ void __launch_bounds__(32 * T::template WARPS<GPU>, 1) w4_matvec_kern
     const int zero_pitch = (groups + 1) >> 1;
     const int units = (K + T::UNIT - 1) / T::UNIT;
     const uint32_t row_bytes = (uint32_t)K >> 1;
-    const uint32_t sums_at = X_AT + p.units_per_pass * (M * 256);
+    const uint32_t sums_at = X_AT + M * T::x_row_bytes(p.units_per_pass);
     const int row_begin = (int)((long long)p.N * blockIdx.x / gridDim.x), row_end = (int)((long long)p.N * (blockIdx.x + 1) / gridDim.x);
     const uint8_t *scales = static_cast<const uint8_t *>(p.scales);
+    const uint32_t step_batch = WK * T::UNIT, step_w = WR * T::TILE * row_bytes, step_s = WR * T::TILE * groups * 2, step_z = WR * T::TILE * zero_pitch;      // K <= 2^24
 
     // The ring holds a unit as 16 rows of four 16-byte pieces; piece j of row r lies at (r, j ^ (r / 2 % 4)), so that the
     // eight rows of a matrix reach all banks.  Copies: lane (g, c) brings piece c of rows g and g + 8.  ldmatrix: lane l names
@@ -281,10 +291,11 @@ __global__ void __launch_bounds__(32 * T::template WARPS<GPU>, 1) w4_matvec_kern
     const uint32_t ring = smem_u32(smem) + T::PART_BYTES + warp * (RING * SLOT);
     const uint32_t put_at = g * 64 + ((c ^ (g >> 1 & 3)) << 4);
     const uint32_t get_at = (lane & 15) * 64 + (((lane >> 4) ^ (lane >> 1 & 3)) << 4);
+    const uint32_t flip_lo = ZERO ? 0u : w4_keep(0x00080008u), flip_hi = ZERO ? 0u : w4_keep(0x00800080u);
     // this lane's column of B in column block nb is row m of X; columns behind the last repeat it (nobody reads their sums)
     uint32_t xbase[NB];
 #pragma unroll
-    for (int nb = 0; nb < NB; nb++) xbase[nb] = X_AT + min(nb * 8 + g, M - 1) * 64 + c * 16;
+    for (int nb = 0; nb < NB; nb++) xbase[nb] = X_AT + min(nb * 8 + g, M - 1) * T::x_row_bytes(p.units_per_pass) + c * 16;
 
     for (int row0 = row_begin; row0 < row_end; row0 += p.block_rows) {
         const int rows = min(p.block_rows, row_end - row0);
@@ -292,30 +303,30 @@ __global__ void __launch_bounds__(32 * T::template WARPS<GPU>, 1) w4_matvec_kern
         for (int u0 = 0; u0 < units; u0 += p.units_per_pass) {
             const int nu = min(p.units_per_pass, units - u0);       // units of this pass
             const int batches = (nu + 1) >> 1;
-            // A warp's share of the pass is a sequence of batches, WK apart in a tile, tiles WR apart.  The slices of a tile
-            // start rotated from tile to tile, so that a last, partial round of batches falls on other warps.
-            const int turn = batches & (WK - 1);
-            auto first_batch = [&](int tile) { return (wk + tile * turn) & (WK - 1); };
+            // A warp's share of the pass: of every WR-th tile every WK-th batch.
             // the batch that ends behind K, if one does: its missing pieces are zeros
             const int cut = !WHOLE && (u0 + 2 * batches) * T::UNIT > K ? batches - 1 : -1;
-            // loading side: place, and this lane's addresses; rows behind the block's last are read as the last
-            int ld_tile = wr, ld_batch = 0;
-            const uint8_t *wa = nullptr, *wb = nullptr, *ls = nullptr, *lz = nullptr;
-            auto enter_tile = [&]() {
-                while (ld_tile < tiles && (ld_batch = first_batch(ld_tile)) >= batches) ld_tile += WR;
-                if (ld_tile >= tiles) return;
-                const int t0 = ld_tile * T::TILE;
-                const size_t u = u0 + 2 * ld_batch;
-                wa = p.W + (size_t)(row0 + min(t0 + g, rows - 1)) * row_bytes + u * (T::UNIT / 2) + c * 16;
-                wb = p.W + (size_t)(row0 + min(t0 + g + 8, rows - 1)) * row_bytes + u * (T::UNIT / 2) + c * 16;
-                // scales and zero points are brought by lane l for row l % 16 (u is even: whole bytes of zero points)
-                const size_t r = row0 + min(t0 + (lane & 15), rows - 1);
-                ls = scales + (r * groups + u * GPU) * 2;
-                if (ZERO) lz = p.zeros + r * zero_pitch + u * GPU / 2;
+            // loading side: place, and this lane's addresses; rows behind the block's last are read as the last.  Scales and
+            // zero points are brought by lane l for row l % 16 (batches are whole bytes of zero points).
+            int ld_tile = wr, ld_batch = wk;
+            const uint8_t *wa = p.W + (size_t)(row0 + wr * T::TILE + g) * row_bytes + (size_t)(u0 + 2 * wk) * (T::UNIT / 2) + c * 16;
+            const uint8_t *ls = scales + ((size_t)(row0 + wr * T::TILE + (lane & 15)) * groups + (size_t)(u0 + 2 * wk) * GPU) * 2;
+            const uint8_t *lz = ZERO ? p.zeros + (size_t)(row0 + wr * T::TILE + (lane & 15)) * zero_pitch + (size_t)(u0 + 2 * wk) * GPU / 2 : nullptr;
+            uint32_t eight_rows = 8 * row_bytes;
+            auto clamp_rows = [&]() {
+                const int last = rows - 1 - ld_tile * T::TILE;
+                if (last < T::TILE - 1 && last >= 0) {
+                    eight_rows = (min(g + 8, last) - min(g, last)) * row_bytes;
+                    wa -= (size_t)max(g - last, 0) * row_bytes;
+                    ls -= (size_t)max((lane & 15) - last, 0) * groups * 2;
+                    if (ZERO) lz -= (size_t)max((lane & 15) - last, 0) * zero_pitch;
+                }
             };
-            auto load = [&](int slot) {
+            clamp_rows();
+            auto load = [&](uint32_t slot) {               // slot: byte offset in the ring
                 if (ld_tile < tiles) {
-                    const uint32_t dst = ring + slot * SLOT;
+                    const uint32_t dst = ring + slot;
+                    const uint8_t *wb = wa + eight_rows;
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         if (WHOLE || ld_batch != cut) {
@@ -348,21 +359,25 @@ __global__ void __launch_bounds__(32 * T::template WARPS<GPU>, 1) w4_matvec_kern
                         w4_copy4(dst + ZEROS_AT + (lane & 15) * 8 + 4 * (lane >> 4), left > 0 ? from : p.zeros, left >= 4 ? 4 : left > 0 ? (int)left : 0);
                     }
                     ld_batch += WK;
-                    wa += WK * T::UNIT;
-                    wb += WK * T::UNIT;
+                    wa += step_batch;
                     ls += WK * GPU * 4;
                     if (ZERO) lz += WK * GPU;
-                    if (ld_batch >= batches) {
+                    if (ld_batch >= batches) {           // on to the next tile
+                        const int done = (ld_batch - wk) >> p.wk_shift;
+                        ld_batch = wk;
                         ld_tile += WR;
-                        enter_tile();
+                        wa += (int)(step_w - done * step_batch);
+                        ls += (int)(step_s - done * (WK * GPU * 4));
+                        if (ZERO) lz += (int)(step_z - done * (WK * GPU));
+                        clamp_rows();
                     }
                 }
                 w4_copies_commit();
             };
-            enter_tile();
-            int tile = ld_tile, batch = ld_batch;                           // computing side
+            if (wk >= batches) ld_tile = tiles;              // (a last pass of fewer batches than slices)
+            int tile = ld_tile, batch = wk;                                 // computing side
 #pragma unroll
-            for (int d = 0; d < RING; d++) load(d);
+            for (int d = 0; d < RING; d++) load(d * SLOT);
             // stage X while the first weights are on their way; the pass before has to be through with its own
             if (units > p.units_per_pass || row0 == row_begin) {
                 if (u0 != 0 || row0 != row_begin) __syncthreads();
@@ -425,7 +440,6 @@ __global__ void __launch_bounds__(32 * T::template WARPS<GPU>, 1) w4_matvec_kern
                 }
             };
             auto compute = [&](const uint8_t *slot, uint32_t from, int i) {
-                constexpr uint32_t FLIP = ZERO ? 0u : 0x00080008u;
                 const int u = 2 * batch + i;
                 const size_t ra = row0 + min(tile * T::TILE + g, rows - 1), rb = row0 + min(tile * T::TILE + g + 8, rows - 1);
                 uint32_t sa[(GPU + 1) / 2], sb[(GPU + 1) / 2];
@@ -438,7 +452,7 @@ __global__ void __launch_bounds__(32 * T::template WARPS<GPU>, 1) w4_matvec_kern
                 }
                 uint32_t xu[NB];
 #pragma unroll
-                for (int nb = 0; nb < NB; nb++) xu[nb] = xbase[nb] + u * (256 * M);
+                for (int nb = 0; nb < NB; nb++) xu[nb] = xbase[nb] + u * 256;
                 float lo[NB][4], hi[NB][4];
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
@@ -448,10 +462,10 @@ __global__ void __launch_bounds__(32 * T::template WARPS<GPU>, 1) w4_matvec_kern
                     for (int sub = 0; sub < 2; sub++) {
                         const int j = 2 * half + sub;
                         const uint32_t qa = q[2 * sub], qb = q[2 * sub + 1], va = qa >> 8, vb = qb >> 8;
-                        const uint32_t la0 = w4_pick(qa, 0x000f000fu, FLIP), lb0 = w4_pick(qb, 0x000f000fu, FLIP);
-                        const uint32_t la1 = w4_pick(va, 0x000f000fu, FLIP), lb1 = w4_pick(vb, 0x000f000fu, FLIP);
-                        const uint32_t ha0 = w4_pick(qa, 0x00f000f0u, FLIP << 4), hb0 = w4_pick(qb, 0x00f000f0u, FLIP << 4);
-                        const uint32_t ha1 = w4_pick(va, 0x00f000f0u, FLIP << 4), hb1 = w4_pick(vb, 0x00f000f0u, FLIP << 4);
+                        const uint32_t la0 = w4_pick<0x000f000fu>(qa, flip_lo), lb0 = w4_pick<0x000f000fu>(qb, flip_lo);
+                        const uint32_t la1 = w4_pick<0x000f000fu>(va, flip_lo), lb1 = w4_pick<0x000f000fu>(vb, flip_lo);
+                        const uint32_t ha0 = w4_pick<0x00f000f0u>(qa, flip_hi), hb0 = w4_pick<0x00f000f0u>(qb, flip_hi);
+                        const uint32_t ha1 = w4_pick<0x00f000f0u>(va, flip_hi), hb1 = w4_pick<0x00f000f0u>(vb, flip_hi);
                         const int grp = j / GROUP_SUBS;
                         float fa = 1.f, fb = 1.f;
                         if (ZERO && j % GROUP_SUBS == 0) {      // 2^23 + z is exact in FP32
@@ -460,7 +474,7 @@ __global__ void __launch_bounds__(32 * T::template WARPS<GPU>, 1) w4_matvec_kern
                         }
 #pragma unroll
                         for (int nb = 0; nb < NB; nb++) {
-                            const uint4 x = *reinterpret_cast<const uint4 *>(smem + xu[nb] + j * (64 * M));
+                            const uint4 x = *reinterpret_cast<const uint4 *>(smem + xu[nb] + j * 64);
                             if (j % GROUP_SUBS == 0) {
                                 const float2 s = *reinterpret_cast<const float2 *>(smem + sums_at + (u * GPU + grp) * (NB * 32) + nb * 32 + c * 8);
                                 W4Type<E>::mma(lo[nb], la0, lb0, la1, lb1, x.x, x.y, fa * s.x, fa * s.y, fb * s.x, fb * s.y);
@@ -487,37 +501,37 @@ __global__ void __launch_bounds__(32 * T::template WARPS<GPU>, 1) w4_matvec_kern
                     }
                 }
             };
-            int slot = 0;
+            uint32_t slot = 0;
             while (tile < tiles) {
                 w4_copies_wait<RING - 1>();
                 __syncwarp();                            // the other lanes' copies too
 #pragma unroll
-                for (int i = 0; i < 2; i++) compute(smem + T::PART_BYTES + (warp * RING + slot) * SLOT, ring + slot * SLOT + get_at + i * T::UNIT_BYTES, i);
+                for (int i = 0; i < 2; i++) compute(smem + T::PART_BYTES + warp * (RING * SLOT) + slot, ring + slot + get_at + i * T::UNIT_BYTES, i);
                 __syncwarp();                            // every lane has read the slot
                 load(slot);
-                slot = slot == RING - 1 ? 0 : slot + 1;
+                slot = slot == (RING - 1) * SLOT ? 0 : slot + SLOT;
                 batch += WK;
                 if (batch >= batches) {
                     // the warp's share of this tile is complete: its partial sums go to its own slot
-                    float *to = part + (size_t)wk * M * p.block_rows + tile * T::TILE + g;
-                    auto put = [&](int m, int row, float v) {
-                        if (m >= M || tile * T::TILE + g + row >= rows) return;
-                        v *= W4Type<E>::OUT;
-                        if (W4Type<E>::RESCALE) v *= xrows->down[m];
-                        float *q = to + m * p.block_rows + row;
-                        *q = u0 == 0 ? v : *q + v;
-                    };
 #pragma unroll
-                    for (int nb = 0; nb < NB; nb++) {
-                        put(nb * 8 + 2 * c, 0, total[nb][0]);
-                        put(nb * 8 + 2 * c + 1, 0, total[nb][1]);
-                        put(nb * 8 + 2 * c, 8, total[nb][2]);
-                        put(nb * 8 + 2 * c + 1, 8, total[nb][3]);
+                    for (int nb = 0; nb < NB; nb++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) total[nb][i] = 0.f;
-                    }
-                    do tile += WR;
-                    while (tile < tiles && (batch = first_batch(tile)) >= batches);
+                        for (int i = 0; i < 2; i++) {
+                            const int m = nb * 8 + 2 * c + i;
+                            if (m < M) {
+                                float *to = part + (wk * M + m) * p.block_rows + tile * T::TILE + g;
+                                float v0 = total[nb][i] * W4Type<E>::OUT, v1 = total[nb][2 + i] * W4Type<E>::OUT;
+                                if (W4Type<E>::RESCALE) {
+                                    v0 *= xrows->down[m];
+                                    v1 *= xrows->down[m];
+                                }
+                                to[0] = u0 == 0 ? v0 : to[0] + v0;
+                                to[8] = u0 == 0 ? v1 : to[8] + v1;
+                            }
+                            total[nb][i] = total[nb][2 + i] = 0.f;
+                        }
+                    batch = wk;
+                    tile += WR;
                 }
             }
             w4_copies_wait<0>();
@@ -535,7 +549,7 @@ __global__ void __launch_bounds__(32 * T::template WARPS<GPU>, 1) w4_matvec_kern
 
 template <class T>
 struct W4MatvecLauncher {
-    static bool can_run(int M, int N, int K) { return M >= 1 && M <= T::MPAD && N >= 1 && K >= 32 && K % 32 == 0 && K <= 1 << 28; }
+    static bool can_run(int M, int N, int K) { return M >= 1 && M <= T::MPAD && N >= 1 && K >= 32 && K % 32 == 0 && K <= 1 << 24; }
     // the family's figure, so that one workspace serves whichever W4A16 plugin is picked; nothing here touches it
     static size_t workspace_bytes(int, int, int) { return (size_t)2 * STREAMK_MAX_CTAS * 128 * 128 * sizeof(float); }
 
@@ -575,16 +589,13 @@ struct W4MatvecLauncher {
         // partial sums: rows of a CTA x M x WK floats; as many K slices as fit (a tile's bytes then arrive soonest), blocks of
         // rows when not even one slice of all rows does
         const int gpu = T::UNIT >> p.group_shift, rows = (a.N + grid - 1) / grid, units = (a.K + T::UNIT - 1) / T::UNIT;
-        const int most_units = T::x_bytes(gpu) / T::x_unit_bytes(a.M, gpu) / 2 * 2, passes = (units + most_units - 1) / most_units;
+        const int most_units = (T::x_bytes(gpu) - a.M * 64) / (a.M * T::UNIT * 2 + gpu * T::NB * 32) / 2 * 2, passes = (units + most_units - 1) / most_units;
         p.units_per_pass = ((units + passes - 1) / passes + 1) / 2 * 2;
-        const int slots = T::PART_BYTES / (int)sizeof(float) / a.M;
-        p.wk_shift = T::NB == 1 && gpu < 4 ? 4 : 3;
-        while (p.wk_shift > 0 && ((2 << p.wk_shift) > p.units_per_pass || (rows << p.wk_shift) > slots)) p.wk_shift--;
-        p.block_rows = rows;
-        if (rows > slots) {
-            const int blocks = (rows + slots / T::TILE * T::TILE - 1) / (slots / T::TILE * T::TILE);
-            p.block_rows = ((rows + blocks - 1) / blocks + T::TILE - 1) / T::TILE * T::TILE;
-        }
+        const int slots = T::PART_BYTES / (int)sizeof(float) / a.M, padded = (rows + T::TILE - 1) / T::TILE * T::TILE;
+        p.wk_shift = T::NB == 1 && gpu < 2 ? 4 : 3;
+        while (p.wk_shift > 0 && ((2 << p.wk_shift) > p.units_per_pass || (padded << p.wk_shift) > slots)) p.wk_shift--;
+        const int most_rows = (slots >> p.wk_shift) / T::TILE * T::TILE, blocks = (padded + most_rows - 1) / most_rows;
+        p.block_rows = ((padded + blocks - 1) / blocks + T::TILE - 1) / T::TILE * T::TILE;
         // how scales and zero points come: with whole batches, else in words around them (base 4-byte aligned), else one by one
         // when they are needed
         const bool whole = a.K % (2 * T::UNIT) == 0 && bits(a.w_scale) % (4 * gpu) == 0 && bits(a.w_zero) % 4 == 0;
@@ -593,7 +604,7 @@ struct W4MatvecLauncher {
         const size_t groups = (size_t)a.K / a.group_size;
         p.scales_end = static_cast<const uint8_t *>(a.w_scale) + (size_t)a.N * groups * 2;
         p.zeros_end = a.w_zero ? p.zeros + (size_t)a.N * ((groups + 1) / 2) : nullptr;
-        const int smem = T::PART_BYTES + T::ring_bytes(gpu) + T::ROW_BYTES + p.units_per_pass * T::x_unit_bytes(a.M, gpu);
+        const int smem = T::PART_BYTES + T::ring_bytes(gpu) + T::ROW_BYTES + T::staged_bytes(a.M, p.units_per_pass, gpu);
         if (a.x_dtype == GEMM_X_F16) return launch<__half>(p, whole, grid, smem, a.stream);
         return launch<__nv_bfloat16>(p, whole, grid, smem, a.stream);
     }

@@ -103,7 +103,7 @@ class GemmConfig:
         if M <= 0 or N <= 0 or K <= 0:
             return False
         if self.dt == "w4a16" and self.bk == 32:   # matrix-vector plugins (K must also be whole scale groups)
-            return M <= self.bn and K % 32 == 0 and K <= 1 << 28
+            return M <= self.bn and K % 32 == 0 and K <= 1 << 24
         if self.dt == "w4a16":   # decode kernel: M fits the padded UMMA N, whole 128-element scale groups
             return M <= self.bn and N % 8 == 0 and K % 128 == 0
         if (K * ELEM_BITS[self.dt]) % 128 != 0 or N % 8 != 0:
