@@ -64,6 +64,13 @@ template <>
 struct W4Type<__nv_bfloat16> {
     static constexpr bool RESCALE = true;
     static constexpr int K_USUAL = 100;          // X is staged as x * 2^K_USUAL
+    static constexpr uint32_t TWO_K_USUAL = 0x71807180u;
+    static __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b)
+    {
+        uint32_t r;
+        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
     static constexpr float OUT = 8589934592.f;   // 2^133 / 2^K_USUAL
     static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3)
     {
@@ -182,54 +189,80 @@ struct W4Rows {
     int top[16];         // largest finite exponent field
 };
 
-// Stages `nu` units of X from unit u0 on ([m][unit][32 k][c]: 8 values, 16 bytes), and their sums over the groups times
-// -8 d (signed) or -d ([unit][group][m]); x behind K is 0.  Returns whether this thread saw an |x| of 2^19 or more, or no
-// finite number (bf16).
-template <class E, int GPU, bool ZERO, class T>
-__device__ __forceinline__ bool w4_stage_x(const W4MatvecParams &p, uint4 *xs, float *sums, W4Rows *rows, int u0, int nu, bool usual)
+// Stages `nu` units of X from unit u0 on ([m][unit][32 k][c]: 8 values, 16 bytes); x behind K is 0.  Returns whether this
+// thread saw an |x| of 2^19 or more, or no finite number (bf16).
+template <class E, int WARPS, class T>
+__device__ __forceinline__ bool w4_stage_x(const W4MatvecParams &p, uint8_t *xs, W4Rows *rows, int u0, int nu, bool usual, int warp, int lane)
 {
-    const int M = p.M, K = p.K;
-    const E *X = static_cast<const E *>(p.X);
+    constexpr int AT_ONCE = 4;                                      // loads in flight per thread
+    const int M = p.M, K = p.K, row_bytes = T::x_row_bytes(p.units_per_pass);
+    const int at = lane & 15;                                       // 16 lanes to the 128 values of a unit
+    int u = 2 * warp + (lane >> 4), m = 0;
     bool far = false;
-    const int pieces = nu * M * 16;                                 // (unit, m, 32 k, c)
-    constexpr int THREADS = 32 * T::template WARPS<GPU>;
-    const int rounds = (pieces + THREADS - 1) / THREADS;
-    for (int it = 0; it < rounds; it++) {
-        const int i = it * THREADS + threadIdx.x;
-        const int at = i & 15, m = (i >> 4) % M, u = (i >> 4) / M;
-        const int k = (u0 + u) * T::UNIT + at * 8;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (i < pieces && k < K) v = __ldg(reinterpret_cast<const uint4 *>(X + (size_t)m * K + k));
-        float sum = 0.f;
-        const float up = usual ? 1.f : rows->up[m];
-        uint32_t most = 0;
-        uint32_t q[4] = {v.x, v.y, v.z, v.w};
+    if (u >= nu) return false;
+    const uint8_t *X = static_cast<const uint8_t *>(p.X) + (size_t)u0 * (2 * T::UNIT) + at * 16;
+    while (m < M) {
+        uint4 v[AT_ONCE];
+        int um[AT_ONCE], mm[AT_ONCE];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            float lo = W4Type<E>::to_f32(reinterpret_cast<const E *>(q + j)[0]), hi = W4Type<E>::to_f32(reinterpret_cast<const E *>(q + j)[1]);
-            if (W4Type<E>::RESCALE) {
-                most = max(most, max(q[j] & 0x7fff0000u, (q[j] << 16) & 0x7fff0000u));
-                lo *= up;
-                hi *= up;
-                const __nv_bfloat162 two = __floats2bfloat162_rn(lo * w4_power_of_two(W4Type<E>::K_USUAL), hi * w4_power_of_two(W4Type<E>::K_USUAL));
-                q[j] = *reinterpret_cast<const uint32_t *>(&two);
+        for (int j = 0; j < AT_ONCE; j++) {
+            um[j] = u;
+            mm[j] = m;
+            v[j] = make_uint4(0, 0, 0, 0);
+            if (m < M && (u0 + u) * T::UNIT + at * 8 < K) v[j] = __ldg(reinterpret_cast<const uint4 *>(X + (size_t)m * K * 2 + u * (2 * T::UNIT)));
+            u += 2 * WARPS;
+            if (u >= nu) {
+                u = 2 * warp + (lane >> 4);
+                m++;
             }
-            sum += lo;
-            sum += hi;
-        }
-        if (W4Type<E>::RESCALE && i < pieces) {
-            if (most >= 0x49000000u) far = true;                        // 2^19
-            if (most >= 0x2b800000u) rows->ordinary[m] = 1;             // 2^-40; every thread that gets here writes the same
         }
 #pragma unroll
-        for (int o = 1; o < 16 / GPU; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (i >= pieces) continue;
-        if (at % (16 / GPU) == 0) sums[(u * GPU + at * GPU / 16) * (T::NB * 8) + m] = sum * (ZERO ? -1.f : -8.f) / W4Type<E>::OUT;
-        // the pairs (0,4), (2,6), (1,5), (3,7) of the eight values: operands of the lo sums, then of the hi sums
-        xs[m * (T::x_row_bytes(p.units_per_pass) / 16) + u * 16 + at] =
-            make_uint4(__byte_perm(q[0], q[2], 0x5410), __byte_perm(q[1], q[3], 0x5410), __byte_perm(q[0], q[2], 0x7632), __byte_perm(q[1], q[3], 0x7632));
+        for (int j = 0; j < AT_ONCE; j++) {
+            if (mm[j] >= M) break;
+            uint32_t q[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+            if constexpr (W4Type<E>::RESCALE) {
+                uint32_t most = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) asm("max.u16x2 %0, %0, %1;" : "+r"(most) : "r"(q[i] & 0x7fff7fffu));      // |x| order like their bits
+                most = max(most >> 16, most & 0xffffu);
+                if (most >= 0x4900u) far = true;                        // 2^19
+                if (most >= 0x2b80u) rows->ordinary[mm[j]] = 1;         // 2^-40; every thread that gets here writes the same
+                if (!usual) {
+                    const uint32_t up = (__float_as_uint(rows->up[mm[j]]) >> 16) * 0x00010001u;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) q[i] = W4Type<E>::mul2(q[i], up);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) q[i] = W4Type<E>::mul2(q[i], W4Type<E>::TWO_K_USUAL);
+            }
+            // the pairs (0,4), (2,6), (1,5), (3,7) of the eight values: operands of the lo sums, then of the hi sums
+            *reinterpret_cast<uint4 *>(xs + mm[j] * row_bytes + um[j] * 256 + at * 16) =
+                make_uint4(__byte_perm(q[0], q[2], 0x5410), __byte_perm(q[1], q[3], 0x5410), __byte_perm(q[0], q[2], 0x7632), __byte_perm(q[1], q[3], 0x7632));
+        }
     }
     return far;
+}
+
+// The sums of the staged X over its groups times -8 d (signed weights) or -d, [unit][group][m]: products with a constant.
+template <class E, int WARPS, int GPU, bool ZERO, class T>
+__device__ __forceinline__ void w4_sum_x(const uint8_t *smem, const uint32_t (&xbase)[T::NB], float *sums, int nu, int warp, int lane)
+{
+    constexpr uint32_t A = ZERO ? 0x80018001u : 0x80088008u;
+    for (int u = warp; u < nu; u += WARPS)
+#pragma unroll
+        for (int nb = 0; nb < T::NB; nb++) {
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint4 x = *reinterpret_cast<const uint4 *>(smem + xbase[nb] + u * 256 + j * 64);
+                if (j % (4 / GPU) == 0) acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
+                W4Type<E>::mma(acc, A, A, A, A, x.x, x.y, acc[0], acc[1], acc[2], acc[3]);
+                W4Type<E>::mma(acc, A, A, A, A, x.z, x.w, acc[0], acc[1], acc[2], acc[3]);
+                // every row of the product is the same; lane c of the first quad holds columns 2c, 2c + 1
+                if ((j + 1) % (4 / GPU) == 0 && lane < 4)
+                    *reinterpret_cast<float2 *>(sums + (u * GPU + j / (4 / GPU)) * (T::NB * 8) + nb * 8 + 2 * lane) = make_float2(acc[0], acc[1]);
+            }
+        }
 }
 
 // The rows' scaling from their largest finite values in this pass (bf16 only; rare): brings them to 2^119 .. 2^120.
@@ -388,13 +421,15 @@ __global__ void __launch_bounds__(32 * T::template WARPS<GPU>, 1) w4_matvec_kern
                 __syncthreads();
 #pragma unroll 1
                 for (bool usual = true;; usual = false) {
-                    const bool far = w4_stage_x<E, GPU, ZERO, T>(p, reinterpret_cast<uint4 *>(smem + X_AT), reinterpret_cast<float *>(smem + sums_at), xrows, u0, 2 * batches, usual);
+                    const bool far = w4_stage_x<E, WARPS, T>(p, smem + X_AT, xrows, u0, 2 * batches, usual, warp, lane);
                     bool again = __syncthreads_or(far) && W4Type<E>::RESCALE;
                     if (W4Type<E>::RESCALE)
                         for (int m = 0; m < M; m++) again = again || !xrows->ordinary[m];
                     if (!again || !usual) break;
                     w4_rescale_rows<E, THREADS, T>(p, xrows, u0, nu);
                 }
+                w4_sum_x<E, WARPS, GPU, ZERO, T>(smem, xbase, reinterpret_cast<float *>(smem + sums_at), 2 * batches, warp, lane);
+                __syncthreads();
             }
             float total[NB][4];
 #pragma unroll
