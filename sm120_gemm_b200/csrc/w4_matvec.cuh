@@ -105,6 +105,7 @@ struct W4MatvecTraits {
     static constexpr int IN_FLIGHT = 48;             // batches of two units in flight, all warps together
     static constexpr int TILE = 16, UNIT = 128;
     static constexpr int UNIT_BYTES = TILE * UNIT / 2;
+    static constexpr int AHEAD_ROWS = 32;            // rows of W asked into L2 before the grid before has ended
     // a batch in the ring: two units, then per row the scales of its 2 GPU groups and a word in front of them, then per row
     // two words around its zero points
     static __host__ __device__ constexpr int scale_pitch(int gpu) { return 8 * gpu; }
@@ -153,6 +154,11 @@ template <int BYTES>
 __device__ __forceinline__ void w4_copy_small(uint32_t dst, const uint8_t *src)
 {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+// asks for [p, p + bytes) to be brought into L2; both multiples of 16
+__device__ __forceinline__ void w4_prefetch(const uint8_t *p, uint32_t bytes)
+{
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void w4_copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT>
@@ -329,6 +335,13 @@ __global__ void __launch_bounds__(32 * T::template WARPS<GPU>, 1) w4_matvec_kern
     uint32_t xbase[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) xbase[nb] = X_AT + min(nb * 8 + g, M - 1) * T::x_row_bytes(p.units_per_pass) + c * 16;
+
+    // Launched as a programmatic dependent: up to here, and for this hint, the grid before may still be running.  The first
+    // tiles are asked into L2 meanwhile (no data is read: what that grid still writes is seen all the same).
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (lane == 0)
+        for (int r = warp; r < T::AHEAD_ROWS && row_begin + r < row_end; r += WARPS) w4_prefetch(p.W + (size_t)(row_begin + r) * row_bytes, row_bytes);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 
     for (int row0 = row_begin; row0 < row_end; row0 += p.block_rows) {
         const int rows = min(p.block_rows, row_end - row0);
@@ -684,8 +697,9 @@ private:
             SM100_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM_ALLOC));
             attr_set[dev].store(true, std::memory_order_release);
         }
-        kernel<<<grid, 32 * T::template WARPS<GPU>, smem, stream>>>(p);
-        SM100_CUDA_TRY(cudaGetLastError());
+        cudaLaunchConfig_t cfg = dependent_launch_config(grid, 32 * T::template WARPS<GPU>, stream);
+        cfg.dynamicSmemBytes = smem;
+        SM100_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p));
         return GEMM_OK;
     }
 };
