@@ -100,8 +100,9 @@ struct W4MatvecTraits {
     static constexpr int STAGES = STAGES_;
     static constexpr int EPI = EPI_;
     static constexpr int NB = MPAD_ / 8;             // column blocks
-    template <int GPU>
-    static constexpr int WARPS = NB == 1 && GPU < 2 ? 16 : 8;      // as the registers allow
+    // 16 warps of 128 registers; 16 rows of X with cut batches need more: 8 warps
+    template <bool WHOLE>
+    static constexpr int WARPS = NB == 1 || WHOLE ? 16 : 8;
     static constexpr int IN_FLIGHT = 48;             // batches of two units in flight, all warps together
     static constexpr int TILE = 16, UNIT = 128;
     static constexpr int UNIT_BYTES = TILE * UNIT / 2;
@@ -300,10 +301,11 @@ __device__ __forceinline__ void w4_rescale_rows(const W4MatvecParams &p, W4Rows 
 // WHOLE: K is whole batches and the scales and zero points are aligned like them, so that nothing is cut and every row's
 // share of a batch is one aligned piece.
 template <class E, int GPU, bool ZERO, bool WHOLE, class T>
-__global__ void __launch_bounds__(32 * T::template WARPS<GPU>, 1) w4_matvec_kernel(const W4MatvecParams p)
+__global__ void __launch_bounds__(32 * T::template WARPS<WHOLE>, 1) w4_matvec_kernel(const W4MatvecParams p)
 {
-    constexpr int NB = T::NB, WARPS = T::template WARPS<GPU>, THREADS = 32 * WARPS, RING = T::IN_FLIGHT / WARPS;
+    constexpr int NB = T::NB, WARPS = T::template WARPS<WHOLE>, THREADS = 32 * WARPS, RING = T::IN_FLIGHT / WARPS;
     constexpr int GROUP_SUBS = 4 / GPU;                  // pieces of 32 k in a group
+    constexpr int STEPS = GPU == 1 ? 2 : 4, SUBS = 8 / STEPS, GROUPS = 2 * GPU / STEPS;      // steps of a batch, pieces and groups of a step
     constexpr int SLOT = T::slot_bytes(GPU), SCALES_AT = 2 * T::UNIT_BYTES, SCALE_PITCH = T::scale_pitch(GPU), ZEROS_AT = SCALES_AT + T::TILE * SCALE_PITCH;
     constexpr int X_AT = T::PART_BYTES + T::ring_bytes(GPU) + T::ROW_BYTES;
     extern __shared__ __align__(16) uint8_t smem[];
@@ -449,72 +451,59 @@ __global__ void __launch_bounds__(32 * T::template WARPS<GPU>, 1) w4_matvec_kern
             for (int nb = 0; nb < NB; nb++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) total[nb][i] = 0.f;
-            // scales of unit u (the i-th of its batch) for row `row` of the tile, row ra of W: GPU times 16 bits
-            auto scales_of = [&](uint32_t (&out)[(GPU + 1) / 2], const uint8_t *slot, int row, size_t ra, int u, int i) {
-                if (WHOLE) {
-                    const uint8_t *at = slot + SCALES_AT + row * SCALE_PITCH + i * GPU * 2;
-                    if constexpr (GPU == 1) out[0] = *reinterpret_cast<const uint16_t *>(at);
-                    else if constexpr (GPU == 2) out[0] = *reinterpret_cast<const uint32_t *>(at);
-                    else {
-                        const uint2 v = *reinterpret_cast<const uint2 *>(at);
-                        out[0] = v.x;
-                        out[(GPU + 1) / 2 - 1] = v.y;
-                    }
+            // A STEP is the part of a batch whose sums are kept apart: a unit (GPU = 1), else half a unit, GPU / 2 groups.
+            // scales of a step for row `row` of the tile, row ra of W: GROUPS times 16 bits
+            auto scales_of = [&](const uint8_t *slot, int row, size_t ra, int step) -> uint32_t {
+                const int first = (u0 + 2 * batch) * GPU + step * GROUPS;          // the step's first group
+                if constexpr (WHOLE) {
+                    const uint8_t *at = slot + SCALES_AT + row * SCALE_PITCH + step * (2 * GROUPS);
+                    return GROUPS == 1 ? *reinterpret_cast<const uint16_t *>(at) : *reinterpret_cast<const uint32_t *>(at);
                 } else {
-                    // (the window starts with the word that holds the first scale; its base is 4-byte aligned)
-                    const uint16_t *at = p.scale_window ? reinterpret_cast<const uint16_t *>(slot + SCALES_AT + row * SCALE_PITCH + (ra * groups & 1) * 2) + i * GPU
-                                                           : reinterpret_cast<const uint16_t *>(scales) + ra * groups + (size_t)u * GPU;
-                    uint32_t v[4] = {0, 0, 0, 0};
-#pragma unroll
-                    for (int j = 0; j < GPU; j++)
-                        if (u * GPU + j < groups) v[j] = at[j];
-#pragma unroll
-                    for (int w = 0; w < (GPU + 1) / 2; w++) out[w] = v[2 * w] | v[2 * w + 1] << 16;
+                    // (the window starts with the word that holds the batch's first scale; the array is 4-byte aligned)
+                    const uint16_t *at = p.scale_window ? reinterpret_cast<const uint16_t *>(slot + SCALES_AT + row * SCALE_PITCH + (ra * groups & 1) * 2) + step * GROUPS
+                                                        : reinterpret_cast<const uint16_t *>(scales) + ra * groups + first;
+                    uint32_t v = first < groups ? at[0] : 0u;
+                    if (GROUPS == 2 && first + 1 < groups) v |= (uint32_t)at[1] << 16;
+                    return v;
                 }
             };
-            // zero points of the unit: GPU nibbles
-            auto zeros_of = [&](const uint8_t *slot, int row, size_t ra, int u, int i) -> uint32_t {
+            // zero points of a step: GROUPS nibbles
+            auto zeros_of = [&](const uint8_t *slot, int row, size_t ra, int step) -> uint32_t {
                 if constexpr (WHOLE && GPU == 4) {
-                    return *reinterpret_cast<const uint16_t *>(slot + ZEROS_AT + row * 8 + 2 * i);
+                    return slot[ZEROS_AT + row * 8 + step];
                 } else {
                     // byte of the batch's first group; its low bits say where the window starts
-                    const size_t z = ra * zero_pitch + (size_t)(u - i) * GPU / 2;
-                    const bool window = WHOLE || p.zero_window;
-                    const uint8_t *at = window ? slot + ZEROS_AT + row * 8 + (z & 3) : p.zeros + z;
-                    if (!window && u * GPU >= groups) return 0;                   // (the ring has zeros there or bytes of the array)
-                    if constexpr (GPU == 1) return at[0] >> (4 * i);
-                    else if constexpr (GPU == 2) return at[i];
-                    else return at[2 * i] | (window || u * GPU + 2 < groups ? (uint32_t)at[2 * i + 1] << 8 : 0u);
+                    const size_t z = ra * zero_pitch + (size_t)(u0 + 2 * batch) * GPU / 2;
+                    const int first = (u0 + 2 * batch) * GPU + step * GROUPS;
+                    if (!WHOLE && !p.zero_window && first >= groups) return 0;     // (in the window are zeros or bytes of the array)
+                    const uint8_t *at = WHOLE || p.zero_window ? slot + ZEROS_AT + row * 8 + (z & 3) : p.zeros + z;
+                    return GROUPS == 2 ? at[step] : at[step >> 1] >> (4 * (step & 1));
                 }
             };
-            auto compute = [&](const uint8_t *slot, uint32_t from, int i) {
-                const int u = 2 * batch + i;
+            auto compute = [&](const uint8_t *slot, uint32_t from, int step) {
                 const size_t ra = row0 + min(tile * T::TILE + g, rows - 1), rb = row0 + min(tile * T::TILE + g + 8, rows - 1);
-                uint32_t sa[(GPU + 1) / 2], sb[(GPU + 1) / 2];
-                scales_of(sa, slot, g, ra, u0 + u, i);
-                scales_of(sb, slot, g + 8, rb, u0 + u, i);
+                const uint32_t sa = scales_of(slot, g, ra, step), sb = scales_of(slot, g + 8, rb, step);
                 uint32_t za = 0, zb = 0;
                 if (ZERO) {
-                    za = zeros_of(slot, g, ra, u0 + u, i);
-                    zb = zeros_of(slot, g + 8, rb, u0 + u, i);
+                    za = zeros_of(slot, g, ra, step);
+                    zb = zeros_of(slot, g + 8, rb, step);
                 }
-                uint32_t xu[NB];
-#pragma unroll
-                for (int nb = 0; nb < NB; nb++) xu[nb] = xbase[nb] + u * 256;
+                const uint32_t x_off = batch * 512 + step * (64 * SUBS), s_off = sums_at + (batch * (2 * GPU) + step * GROUPS) * (NB * 32) + c * 8;
                 float lo[NB][4], hi[NB][4];
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    uint32_t q[4];                       // rows g, g + 8 of piece 2 half, then of piece 2 half + 1
-                    w4_ldmatrix(q, half ? from ^ 32 : from);
+                for (int pair = 0; pair < SUBS / 2; pair++) {
+                    uint32_t q[4];                       // rows g, g + 8 of a piece, then of the next
+                    // piece 2 h of a unit lies where piece 0 does, bit 5 of the address flipped for h = 1
+                    w4_ldmatrix(q, GPU == 1 ? (from + step * T::UNIT_BYTES) ^ (pair * 32) : (from + (step >> 1) * T::UNIT_BYTES) ^ ((step & 1) * 32));
 #pragma unroll
                     for (int sub = 0; sub < 2; sub++) {
-                        const int j = 2 * half + sub;
+                        const int j = 2 * pair + sub;    // piece of the step
                         const uint32_t qa = q[2 * sub], qb = q[2 * sub + 1], va = qa >> 8, vb = qb >> 8;
                         const uint32_t la0 = w4_pick<0x000f000fu>(qa, flip_lo), lb0 = w4_pick<0x000f000fu>(qb, flip_lo);
                         const uint32_t la1 = w4_pick<0x000f000fu>(va, flip_lo), lb1 = w4_pick<0x000f000fu>(vb, flip_lo);
                         const uint32_t ha0 = w4_pick<0x00f000f0u>(qa, flip_hi), hb0 = w4_pick<0x00f000f0u>(qb, flip_hi);
                         const uint32_t ha1 = w4_pick<0x00f000f0u>(va, flip_hi), hb1 = w4_pick<0x00f000f0u>(vb, flip_hi);
-                        const int grp = j / GROUP_SUBS;
+                        const int grp = j / GROUP_SUBS;  // group of the step
                         float fa = 1.f, fb = 1.f;
                         if (ZERO && j % GROUP_SUBS == 0) {      // 2^23 + z is exact in FP32
                             fa = __uint_as_float((za >> (4 * grp) & 15u) | 0x4b000000u) - 8388608.f;
@@ -522,9 +511,9 @@ __global__ void __launch_bounds__(32 * T::template WARPS<GPU>, 1) w4_matvec_kern
                         }
 #pragma unroll
                         for (int nb = 0; nb < NB; nb++) {
-                            const uint4 x = *reinterpret_cast<const uint4 *>(smem + xu[nb] + j * 64);
+                            const uint4 x = *reinterpret_cast<const uint4 *>(smem + xbase[nb] + x_off + j * 64);
                             if (j % GROUP_SUBS == 0) {
-                                const float2 s = *reinterpret_cast<const float2 *>(smem + sums_at + (u * GPU + grp) * (NB * 32) + nb * 32 + c * 8);
+                                const float2 s = *reinterpret_cast<const float2 *>(smem + s_off + grp * (NB * 32) + nb * 32);
                                 W4Type<E>::mma(lo[nb], la0, lb0, la1, lb1, x.x, x.y, fa * s.x, fa * s.y, fb * s.x, fb * s.y);
                                 W4Type<E>::mma(hi[nb], ha0, hb0, ha1, hb1, x.z, x.w, 0.f, 0.f, 0.f, 0.f);
                             } else {
@@ -537,7 +526,7 @@ __global__ void __launch_bounds__(32 * T::template WARPS<GPU>, 1) w4_matvec_kern
                                 const uint16_t bits = (uint16_t)(which ? word >> 16 : word);
                                 return W4Type<E>::to_f32(*reinterpret_cast<const E *>(&bits));
                             };
-                            const float s_a = scale(sa[grp / 2], grp & 1), s_b = scale(sb[grp / 2], grp & 1);
+                            const float s_a = scale(sa, grp), s_b = scale(sb, grp);
 #pragma unroll
                             for (int nb = 0; nb < NB; nb++) {
                                 total[nb][0] = fmaf(s_a, fmaf(hi[nb][0], 0.0625f, lo[nb][0]), total[nb][0]);
@@ -553,8 +542,10 @@ __global__ void __launch_bounds__(32 * T::template WARPS<GPU>, 1) w4_matvec_kern
             while (tile < tiles) {
                 w4_copies_wait<RING - 1>();
                 __syncwarp();                            // the other lanes' copies too
-#pragma unroll
-                for (int i = 0; i < 2; i++) compute(smem + T::PART_BYTES + warp * (RING * SLOT) + slot, ring + slot + get_at + i * T::UNIT_BYTES, i);
+                // one step after the other where the registers are short
+                constexpr int UNROLL = GPU == 1 && NB == 1 ? 2 : 1;
+#pragma unroll UNROLL
+                for (int step = 0; step < STEPS; step++) compute(smem + T::PART_BYTES + warp * (RING * SLOT) + slot, ring + slot + get_at, step);
                 __syncwarp();                            // every lane has read the slot
                 load(slot);
                 slot = slot == (RING - 1) * SLOT ? 0 : slot + SLOT;
@@ -637,16 +628,16 @@ struct W4MatvecLauncher {
         // partial sums: rows of a CTA x M x WK floats; as many K slices as fit (a tile's bytes then arrive soonest), blocks of
         // rows when not even one slice of all rows does
         const int gpu = T::UNIT >> p.group_shift, rows = (a.N + grid - 1) / grid, units = (a.K + T::UNIT - 1) / T::UNIT;
-        const int most_units = (T::x_bytes(gpu) - a.M * 64) / (a.M * T::UNIT * 2 + gpu * T::NB * 32) / 2 * 2, passes = (units + most_units - 1) / most_units;
-        p.units_per_pass = ((units + passes - 1) / passes + 1) / 2 * 2;
-        const int slots = T::PART_BYTES / (int)sizeof(float) / a.M, padded = (rows + T::TILE - 1) / T::TILE * T::TILE;
-        p.wk_shift = T::NB == 1 && gpu < 2 ? 4 : 3;
-        while (p.wk_shift > 0 && ((2 << p.wk_shift) > p.units_per_pass || (padded << p.wk_shift) > slots)) p.wk_shift--;
-        const int most_rows = (slots >> p.wk_shift) / T::TILE * T::TILE, blocks = (padded + most_rows - 1) / most_rows;
-        p.block_rows = ((padded + blocks - 1) / blocks + T::TILE - 1) / T::TILE * T::TILE;
         // how scales and zero points come: with whole batches, else in words around them (base 4-byte aligned), else one by one
         // when they are needed
         const bool whole = a.K % (2 * T::UNIT) == 0 && bits(a.w_scale) % (4 * gpu) == 0 && bits(a.w_zero) % 4 == 0;
+        const int most_units = (T::x_bytes(gpu) - a.M * 64) / (a.M * T::UNIT * 2 + gpu * T::NB * 32) / 2 * 2, passes = (units + most_units - 1) / most_units;
+        p.units_per_pass = ((units + passes - 1) / passes + 1) / 2 * 2;
+        const int slots = T::PART_BYTES / (int)sizeof(float) / a.M, padded = (rows + T::TILE - 1) / T::TILE * T::TILE;
+        p.wk_shift = T::NB == 1 || whole ? 4 : 3;
+        while (p.wk_shift > 0 && ((2 << p.wk_shift) > p.units_per_pass || (padded << p.wk_shift) > slots)) p.wk_shift--;
+        const int most_rows = (slots >> p.wk_shift) / T::TILE * T::TILE, blocks = (padded + most_rows - 1) / most_rows;
+        p.block_rows = ((padded + blocks - 1) / blocks + T::TILE - 1) / T::TILE * T::TILE;
         p.scale_window = bits(a.w_scale) % 4 == 0;
         p.zero_window = bits(a.w_zero) % 4 == 0;
         const size_t groups = (size_t)a.K / a.group_size;
@@ -697,7 +688,7 @@ private:
             SM100_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM_ALLOC));
             attr_set[dev].store(true, std::memory_order_release);
         }
-        cudaLaunchConfig_t cfg = dependent_launch_config(grid, 32 * T::template WARPS<GPU>, stream);
+        cudaLaunchConfig_t cfg = dependent_launch_config(grid, 32 * T::template WARPS<WHOLE>, stream);
         cfg.dynamicSmemBytes = smem;
         SM100_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p));
         return GEMM_OK;
