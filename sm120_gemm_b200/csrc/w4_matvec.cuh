@@ -53,6 +53,7 @@ struct W4MatvecParams {
     int block_rows;              // rows of W whose partial sums shared memory holds
     int units_per_pass;          // units (128 K-elements) of X that shared memory holds
     int wk_shift;                // log2(WK)
+    int part_at;                 // partial sums: byte offset in shared memory
     int scale_window, zero_window;       // scales / zero points reach the ring in words around them, else they are read when needed
     const uint8_t *scales_end, *zeros_end;
 };
@@ -100,22 +101,20 @@ struct W4MatvecTraits {
     static constexpr int STAGES = STAGES_;
     static constexpr int EPI = EPI_;
     static constexpr int NB = MPAD_ / 8;             // column blocks
-    // 16 warps of 128 registers; 16 rows of X with cut batches need more: 8 warps
-    template <bool WHOLE>
-    static constexpr int WARPS = NB == 1 || WHOLE ? 16 : 8;
-    static constexpr int IN_FLIGHT = 48;             // batches of two units in flight, all warps together
-    static constexpr int TILE = 16, UNIT = 128;
+    // Every 16 rows of W need all of X from shared memory: 256 M bytes against 1 KB of weights per unit.  For 16 rows of X a
+    // tile is 32 rows of W, so that what is read of X is used twice; that takes the registers of 8 warps.
+    static constexpr int SUBTILES = NB, TILE = 16 * SUBTILES, UNIT = 128;
+    static constexpr int WARPS = NB == 1 ? 16 : 8, THREADS = 32 * WARPS;
+    static constexpr int RING = NB == 1 ? 3 : 2;     // batches of two units in flight per warp
     static constexpr int UNIT_BYTES = TILE * UNIT / 2;
     static constexpr int AHEAD_ROWS = 32;            // rows of W asked into L2 before the grid before has ended
     // a batch in the ring: two units, then per row the scales of its 2 GPU groups and a word in front of them, then per row
     // two words around its zero points
     static __host__ __device__ constexpr int scale_pitch(int gpu) { return 8 * gpu; }
     static __host__ __device__ constexpr int slot_bytes(int gpu) { return 2 * UNIT_BYTES + TILE * scale_pitch(gpu) + TILE * 8; }
-    static __host__ __device__ constexpr int ring_bytes(int gpu) { return IN_FLIGHT * slot_bytes(gpu); }
-    static constexpr int PART_BYTES = 26 * 1024;     // partial sums
+    static __host__ __device__ constexpr int ring_bytes(int gpu) { return WARPS * RING * slot_bytes(gpu); }
     static constexpr int ROW_BYTES = 256;            // per row of X: scaling, flags
-    static constexpr int SMEM_ALLOC = 227 * 1024;    // the rest: staged X and its sums
-    static __host__ __device__ constexpr int x_bytes(int gpu) { return SMEM_ALLOC - PART_BYTES - ROW_BYTES - ring_bytes(gpu); }
+    static constexpr int SMEM_ALLOC = 227 * 1024;    // ring, flags, staged X and its sums, partial sums
     // staged X: rows 64 bytes longer than their units, so that the eight lanes of a 16-byte access (two rows) reach all banks
     static __host__ __device__ constexpr int x_row_bytes(int units) { return units * UNIT * 2 + 64; }
     static __host__ __device__ constexpr int staged_bytes(int M, int units, int gpu) { return M * x_row_bytes(units) + units * gpu * NB * 32; }
@@ -196,57 +195,53 @@ struct W4Rows {
     int top[16];         // largest finite exponent field
 };
 
-// Stages `nu` units of X from unit u0 on ([m][unit][32 k][c]: 8 values, 16 bytes); x behind K is 0.  Returns whether this
-// thread saw an |x| of 2^19 or more, or no finite number (bf16).
-template <class E, int WARPS, class T>
-__device__ __forceinline__ bool w4_stage_x(const W4MatvecParams &p, uint8_t *xs, W4Rows *rows, int u0, int nu, bool usual, int warp, int lane)
+// Staging of `nu` units of X from unit u0 on ([m][unit][32 k][c]: 8 values, 16 bytes; x behind K is 0).  A thread copies its
+// pieces, all of them in flight at once, and then rewrites each in its place.
+template <int WARPS, class T, class F>
+__device__ __forceinline__ void w4_x_pieces(int M, int nu, int warp, int lane, F &&piece)
 {
-    constexpr int AT_ONCE = 4;                                      // loads in flight per thread
-    const int M = p.M, K = p.K, row_bytes = T::x_row_bytes(p.units_per_pass);
-    const int at = lane & 15;                                       // 16 lanes to the 128 values of a unit
-    int u = 2 * warp + (lane >> 4), m = 0;
+    for (int m = 0; m < M; m++)
+        for (int u = 2 * warp + (lane >> 4); u < nu; u += 2 * WARPS) piece(m, u);          // 16 lanes to the 128 values of a unit
+}
+template <int WARPS, class T>
+__device__ __forceinline__ void w4_copy_x(const W4MatvecParams &p, uint32_t xs, int u0, int nu, int warp, int lane)
+{
+    const int row_bytes = T::x_row_bytes(p.units_per_pass), at = lane & 15;
+    w4_x_pieces<WARPS, T>(p.M, nu, warp, lane, [&](int m, int u) {
+        const int k = (u0 + u) * T::UNIT + at * 8;
+        const uint8_t *X = static_cast<const uint8_t *>(p.X);
+        w4_copy16(xs + m * row_bytes + u * 256 + at * 16, k < p.K ? X + ((size_t)m * p.K + k) * 2 : X, k < p.K ? 16 : 0);
+    });
+    w4_copies_commit();
+}
+// Returns whether this thread saw an |x| of 2^19 or more, or no finite number (bf16).
+template <class E, int WARPS, class T>
+__device__ __forceinline__ bool w4_order_x(const W4MatvecParams &p, uint8_t *xs, W4Rows *rows, int nu, bool usual, int warp, int lane)
+{
+    const int row_bytes = T::x_row_bytes(p.units_per_pass), at = lane & 15;
     bool far = false;
-    if (u >= nu) return false;
-    const uint8_t *X = static_cast<const uint8_t *>(p.X) + (size_t)u0 * (2 * T::UNIT) + at * 16;
-    while (m < M) {
-        uint4 v[AT_ONCE];
-        int um[AT_ONCE], mm[AT_ONCE];
+    w4_x_pieces<WARPS, T>(p.M, nu, warp, lane, [&](int m, int u) {
+        uint4 *piece = reinterpret_cast<uint4 *>(xs + m * row_bytes + u * 256 + at * 16);
+        const uint4 v = *piece;
+        uint32_t q[4] = {v.x, v.y, v.z, v.w};
+        if constexpr (W4Type<E>::RESCALE) {
+            uint32_t most = 0;
 #pragma unroll
-        for (int j = 0; j < AT_ONCE; j++) {
-            um[j] = u;
-            mm[j] = m;
-            v[j] = make_uint4(0, 0, 0, 0);
-            if (m < M && (u0 + u) * T::UNIT + at * 8 < K) v[j] = __ldg(reinterpret_cast<const uint4 *>(X + (size_t)m * K * 2 + u * (2 * T::UNIT)));
-            u += 2 * WARPS;
-            if (u >= nu) {
-                u = 2 * warp + (lane >> 4);
-                m++;
+            for (int i = 0; i < 4; i++) asm("max.u16x2 %0, %0, %1;" : "+r"(most) : "r"(q[i] & 0x7fff7fffu));      // |x| order like their bits
+            most = max(most >> 16, most & 0xffffu);
+            if (most >= 0x4900u) far = true;                        // 2^19
+            if (most >= 0x2b80u) rows->ordinary[m] = 1;             // 2^-40; every thread that gets here writes the same
+            if (!usual) {
+                const uint32_t up = (__float_as_uint(rows->up[m]) >> 16) * 0x00010001u;
+#pragma unroll
+                for (int i = 0; i < 4; i++) q[i] = W4Type<E>::mul2(q[i], up);
             }
+#pragma unroll
+            for (int i = 0; i < 4; i++) q[i] = W4Type<E>::mul2(q[i], W4Type<E>::TWO_K_USUAL);
         }
-#pragma unroll
-        for (int j = 0; j < AT_ONCE; j++) {
-            if (mm[j] >= M) break;
-            uint32_t q[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-            if constexpr (W4Type<E>::RESCALE) {
-                uint32_t most = 0;
-#pragma unroll
-                for (int i = 0; i < 4; i++) asm("max.u16x2 %0, %0, %1;" : "+r"(most) : "r"(q[i] & 0x7fff7fffu));      // |x| order like their bits
-                most = max(most >> 16, most & 0xffffu);
-                if (most >= 0x4900u) far = true;                        // 2^19
-                if (most >= 0x2b80u) rows->ordinary[mm[j]] = 1;         // 2^-40; every thread that gets here writes the same
-                if (!usual) {
-                    const uint32_t up = (__float_as_uint(rows->up[mm[j]]) >> 16) * 0x00010001u;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) q[i] = W4Type<E>::mul2(q[i], up);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) q[i] = W4Type<E>::mul2(q[i], W4Type<E>::TWO_K_USUAL);
-            }
-            // the pairs (0,4), (2,6), (1,5), (3,7) of the eight values: operands of the lo sums, then of the hi sums
-            *reinterpret_cast<uint4 *>(xs + mm[j] * row_bytes + um[j] * 256 + at * 16) =
-                make_uint4(__byte_perm(q[0], q[2], 0x5410), __byte_perm(q[1], q[3], 0x5410), __byte_perm(q[0], q[2], 0x7632), __byte_perm(q[1], q[3], 0x7632));
-        }
-    }
+        // the pairs (0,4), (2,6), (1,5), (3,7) of the eight values: operands of the lo sums, then of the hi sums
+        *piece = make_uint4(__byte_perm(q[0], q[2], 0x5410), __byte_perm(q[1], q[3], 0x5410), __byte_perm(q[0], q[2], 0x7632), __byte_perm(q[1], q[3], 0x7632));
+    });
     return far;
 }
 
@@ -301,15 +296,16 @@ __device__ __forceinline__ void w4_rescale_rows(const W4MatvecParams &p, W4Rows 
 // WHOLE: K is whole batches and the scales and zero points are aligned like them, so that nothing is cut and every row's
 // share of a batch is one aligned piece.
 template <class E, int GPU, bool ZERO, bool WHOLE, class T>
-__global__ void __launch_bounds__(32 * T::template WARPS<WHOLE>, 1) w4_matvec_kernel(const W4MatvecParams p)
+__global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4MatvecParams p)
 {
-    constexpr int NB = T::NB, WARPS = T::template WARPS<WHOLE>, THREADS = 32 * WARPS, RING = T::IN_FLIGHT / WARPS;
+    constexpr int NB = T::NB, WARPS = T::WARPS, THREADS = T::THREADS, RING = T::RING, SUBTILES = T::SUBTILES, TILE = T::TILE;
+    constexpr int LANES_PER_ROW = 32 / TILE;             // that bring its scales and zero points
     constexpr int GROUP_SUBS = 4 / GPU;                  // pieces of 32 k in a group
     constexpr int STEPS = GPU == 1 ? 2 : 4, SUBS = 8 / STEPS, GROUPS = 2 * GPU / STEPS;      // steps of a batch, pieces and groups of a step
-    constexpr int SLOT = T::slot_bytes(GPU), SCALES_AT = 2 * T::UNIT_BYTES, SCALE_PITCH = T::scale_pitch(GPU), ZEROS_AT = SCALES_AT + T::TILE * SCALE_PITCH;
-    constexpr int X_AT = T::PART_BYTES + T::ring_bytes(GPU) + T::ROW_BYTES;
+    constexpr int SLOT = T::slot_bytes(GPU), SCALES_AT = 2 * T::UNIT_BYTES, SCALE_PITCH = T::scale_pitch(GPU), ZEROS_AT = SCALES_AT + TILE * SCALE_PITCH;
+    constexpr int X_AT = T::ring_bytes(GPU) + T::ROW_BYTES;
     extern __shared__ __align__(16) uint8_t smem[];
-    float *part = reinterpret_cast<float *>(smem);       // [WK][M][block_rows]
+    float *part = reinterpret_cast<float *>(smem + p.part_at);      // [WK][M][block_rows]
     W4Rows *xrows = reinterpret_cast<W4Rows *>(smem + X_AT - T::ROW_BYTES);
     const int lane = threadIdx.x & 31;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);                 // uniform over the warp, and known to be
@@ -324,12 +320,12 @@ __global__ void __launch_bounds__(32 * T::template WARPS<WHOLE>, 1) w4_matvec_ke
     const uint32_t sums_at = X_AT + M * T::x_row_bytes(p.units_per_pass);
     const int row_begin = (int)((long long)p.N * blockIdx.x / gridDim.x), row_end = (int)((long long)p.N * (blockIdx.x + 1) / gridDim.x);
     const uint8_t *scales = static_cast<const uint8_t *>(p.scales);
-    const uint32_t step_batch = WK * T::UNIT, step_w = WR * T::TILE * row_bytes, step_s = WR * T::TILE * groups * 2, step_z = WR * T::TILE * zero_pitch;      // K <= 2^24
+    const uint32_t step_batch = WK * T::UNIT, step_w = WR * TILE * row_bytes, step_s = WR * TILE * groups * 2, step_z = WR * TILE * zero_pitch;      // K <= 2^24
 
-    // The ring holds a unit as 16 rows of four 16-byte pieces; piece j of row r lies at (r, j ^ (r / 2 % 4)), so that the
-    // eight rows of a matrix reach all banks.  Copies: lane (g, c) brings piece c of rows g and g + 8.  ldmatrix: lane l names
-    // row l % 16 and piece l / 16 (then 2 more) of the four matrices (rows 0-7, 8-15) x (piece j, j + 1).
-    const uint32_t ring = smem_u32(smem) + T::PART_BYTES + warp * (RING * SLOT);
+    // The ring holds a unit as TILE rows of four 16-byte pieces; piece j of row r lies at (r, j ^ (r / 2 % 4)), so that the
+    // eight rows of a matrix reach all banks.  Copies: lane (g, c) brings piece c of rows g, g + 8, ...  ldmatrix: lane l
+    // names row l % 16 and piece l / 16 (then 2 more) of the four matrices (rows 0-7, 8-15) x (piece j, j + 1).
+    const uint32_t ring = smem_u32(smem) + warp * (RING * SLOT);
     const uint32_t put_at = g * 64 + ((c ^ (g >> 1 & 3)) << 4);
     const uint32_t get_at = (lane & 15) * 64 + (((lane >> 4) ^ (lane >> 1 & 3)) << 4);
     const uint32_t flip_lo = ZERO ? 0u : w4_keep(0x00080008u), flip_hi = ZERO ? 0u : w4_keep(0x00800080u);
@@ -347,7 +343,7 @@ __global__ void __launch_bounds__(32 * T::template WARPS<WHOLE>, 1) w4_matvec_ke
 
     for (int row0 = row_begin; row0 < row_end; row0 += p.block_rows) {
         const int rows = min(p.block_rows, row_end - row0);
-        const int tiles = (rows + T::TILE - 1) / T::TILE;
+        const int tiles = (rows + TILE - 1) / TILE;
         for (int u0 = 0; u0 < units; u0 += p.units_per_pass) {
             const int nu = min(p.units_per_pass, units - u0);       // units of this pass
             const int batches = (nu + 1) >> 1;
@@ -357,54 +353,58 @@ __global__ void __launch_bounds__(32 * T::template WARPS<WHOLE>, 1) w4_matvec_ke
             // loading side: place, and this lane's addresses; rows behind the block's last are read as the last.  Scales and
             // zero points are brought by lane l for row l % 16 (batches are whole bytes of zero points).
             int ld_tile = wr, ld_batch = wk;
-            const uint8_t *wa = p.W + (size_t)(row0 + wr * T::TILE + g) * row_bytes + (size_t)(u0 + 2 * wk) * (T::UNIT / 2) + c * 16;
-            const uint8_t *ls = scales + ((size_t)(row0 + wr * T::TILE + (lane & 15)) * groups + (size_t)(u0 + 2 * wk) * GPU) * 2;
-            const uint8_t *lz = ZERO ? p.zeros + (size_t)(row0 + wr * T::TILE + (lane & 15)) * zero_pitch + (size_t)(u0 + 2 * wk) * GPU / 2 : nullptr;
-            uint32_t eight_rows = 8 * row_bytes;
+            const uint8_t *wa = p.W + (size_t)(row0 + wr * TILE + g) * row_bytes + (size_t)(u0 + 2 * wk) * (T::UNIT / 2) + c * 16;
+            const uint8_t *ls = scales + ((size_t)(row0 + wr * TILE + lane % TILE) * groups + (size_t)(u0 + 2 * wk) * GPU) * 2;
+            const uint8_t *lz = ZERO ? p.zeros + (size_t)(row0 + wr * TILE + lane % TILE) * zero_pitch + (size_t)(u0 + 2 * wk) * GPU / 2 : nullptr;
+            uint32_t to_row[2 * SUBTILES];               // rows g + 8 k relative to row g
+#pragma unroll
+            for (int k = 0; k < 2 * SUBTILES; k++) to_row[k] = 8 * k * row_bytes;
             auto clamp_rows = [&]() {
-                const int last = rows - 1 - ld_tile * T::TILE;
-                if (last < T::TILE - 1 && last >= 0) {
-                    eight_rows = (min(g + 8, last) - min(g, last)) * row_bytes;
+                const int last = rows - 1 - ld_tile * TILE;
+                if (last < TILE - 1 && last >= 0) {
+#pragma unroll
+                    for (int k = 0; k < 2 * SUBTILES; k++) to_row[k] = (min(g + 8 * k, last) - min(g, last)) * row_bytes;
                     wa -= (size_t)max(g - last, 0) * row_bytes;
-                    ls -= (size_t)max((lane & 15) - last, 0) * groups * 2;
-                    if (ZERO) lz -= (size_t)max((lane & 15) - last, 0) * zero_pitch;
+                    ls -= (size_t)max(lane % TILE - last, 0) * groups * 2;
+                    if (ZERO) lz -= (size_t)max(lane % TILE - last, 0) * zero_pitch;
                 }
             };
             clamp_rows();
             auto load = [&](uint32_t slot) {               // slot: byte offset in the ring
                 if (ld_tile < tiles) {
                     const uint32_t dst = ring + slot;
-                    const uint8_t *wb = wa + eight_rows;
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
-                        if (WHOLE || ld_batch != cut) {
-                            w4_copy16(dst + put_at + i * T::UNIT_BYTES, wa + i * (T::UNIT / 2));
-                            w4_copy16(dst + put_at + i * T::UNIT_BYTES + 512, wb + i * (T::UNIT / 2));
-                        } else {
-                            const bool in_k = (u0 + 2 * ld_batch + i) * T::UNIT + c * 32 < K;
-                            w4_copy16(dst + put_at + i * T::UNIT_BYTES, in_k ? wa + i * (T::UNIT / 2) : p.W, in_k ? 16 : 0);
-                            w4_copy16(dst + put_at + i * T::UNIT_BYTES + 512, in_k ? wb + i * (T::UNIT / 2) : p.W, in_k ? 16 : 0);
+                        const bool in_k = WHOLE || ld_batch != cut || (u0 + 2 * ld_batch + i) * T::UNIT + c * 32 < K;
+#pragma unroll
+                        for (int k = 0; k < 2 * SUBTILES; k++) {
+                            const uint8_t *from = wa + to_row[k] + i * (T::UNIT / 2);
+                            if (WHOLE) w4_copy16(dst + put_at + i * T::UNIT_BYTES + k * 512, from);
+                            else w4_copy16(dst + put_at + i * T::UNIT_BYTES + k * 512, in_k ? from : p.W, in_k ? 16 : 0);
                         }
                     }
-                    const uint32_t dst_s = dst + SCALES_AT + (lane & 15) * SCALE_PITCH;
+                    const uint32_t dst_s = dst + SCALES_AT + lane % TILE * SCALE_PITCH, dst_z = dst + ZEROS_AT + lane % TILE * 8;
                     if (WHOLE) {
-                        if (lane < 16) w4_copy_small<4 * GPU>(dst_s, ls);
+                        if (lane < TILE) w4_copy_small<4 * GPU>(dst_s, ls);
                     } else if (p.scale_window) {
                         // words around them: from the word that holds the first, never behind the array's end
                         const uint8_t *from = reinterpret_cast<const uint8_t *>(reinterpret_cast<uintptr_t>(ls) & ~(uintptr_t)3);
 #pragma unroll
-                        for (int w = 0; w <= GPU / 2; w++) {
-                            const int word = 2 * w + (lane >> 4);
+                        for (int w = 0; w <= GPU / LANES_PER_ROW; w++) {
+                            const int word = w * LANES_PER_ROW + lane / TILE;
                             const long long left = p.scales_end - (from + 4 * word);
                             if (word <= GPU) w4_copy4(dst_s + 4 * word, left > 0 ? from + 4 * word : scales, left >= 4 ? 4 : left > 0 ? (int)left : 0);
                         }
                     }
                     if (ZERO && WHOLE && GPU == 4) {
-                        if (lane < 16) w4_copy_small<4>(dst + ZEROS_AT + lane * 8, lz);
+                        if (lane < TILE) w4_copy_small<4>(dst_z, lz);
                     } else if (ZERO && (WHOLE || p.zero_window)) {
-                        const uint8_t *from = reinterpret_cast<const uint8_t *>(reinterpret_cast<uintptr_t>(lz) & ~(uintptr_t)3) + 4 * (lane >> 4);
-                        const long long left = p.zeros_end - from;
-                        w4_copy4(dst + ZEROS_AT + (lane & 15) * 8 + 4 * (lane >> 4), left > 0 ? from : p.zeros, left >= 4 ? 4 : left > 0 ? (int)left : 0);
+#pragma unroll
+                        for (int w = lane / TILE; w < 2; w += LANES_PER_ROW) {
+                            const uint8_t *from = reinterpret_cast<const uint8_t *>(reinterpret_cast<uintptr_t>(lz) & ~(uintptr_t)3) + 4 * w;
+                            const long long left = p.zeros_end - from;
+                            w4_copy4(dst_z + 4 * w, left > 0 ? from : p.zeros, left >= 4 ? 4 : left > 0 ? (int)left : 0);
+                        }
                     }
                     ld_batch += WK;
                     wa += step_batch;
@@ -424,33 +424,42 @@ __global__ void __launch_bounds__(32 * T::template WARPS<WHOLE>, 1) w4_matvec_ke
             };
             if (wk >= batches) ld_tile = tiles;              // (a last pass of fewer batches than slices)
             int tile = ld_tile, batch = wk;                                 // computing side
-#pragma unroll
-            for (int d = 0; d < RING; d++) load(d * SLOT);
-            // stage X while the first weights are on their way; the pass before has to be through with its own
-            if (units > p.units_per_pass || row0 == row_begin) {
+            // X is staged while the first weights are on their way; the pass before has to be through with its own
+            const bool stage = units > p.units_per_pass || row0 == row_begin;
+            if (stage) {
                 if (u0 != 0 || row0 != row_begin) __syncthreads();
                 if (threadIdx.x < 16) {
                     xrows->ordinary[threadIdx.x] = 0;
                     xrows->down[threadIdx.x] = 1.f;
                 }
-                __syncthreads();
+                w4_copy_x<WARPS, T>(p, smem_u32(smem + X_AT), u0, 2 * batches, warp, lane);
+            }
+#pragma unroll
+            for (int d = 0; d < RING; d++) load(d * SLOT);
+            if (stage) {
+                w4_copies_wait<RING>();              // this thread's pieces of X
+                __syncthreads();                     // the flags
 #pragma unroll 1
                 for (bool usual = true;; usual = false) {
-                    const bool far = w4_stage_x<E, WARPS, T>(p, smem + X_AT, xrows, u0, 2 * batches, usual, warp, lane);
+                    const bool far = w4_order_x<E, WARPS, T>(p, smem + X_AT, xrows, 2 * batches, usual, warp, lane);
                     bool again = __syncthreads_or(far) && W4Type<E>::RESCALE;
                     if (W4Type<E>::RESCALE)
                         for (int m = 0; m < M; m++) again = again || !xrows->ordinary[m];
                     if (!again || !usual) break;
                     w4_rescale_rows<E, THREADS, T>(p, xrows, u0, nu);
+                    w4_copy_x<WARPS, T>(p, smem_u32(smem + X_AT), u0, 2 * batches, warp, lane);
+                    w4_copies_wait<0>();
                 }
                 w4_sum_x<E, WARPS, GPU, ZERO, T>(smem, xbase, reinterpret_cast<float *>(smem + sums_at), 2 * batches, warp, lane);
                 __syncthreads();
             }
-            float total[NB][4];
+            float total[SUBTILES][NB][4];
 #pragma unroll
-            for (int nb = 0; nb < NB; nb++)
+            for (int t = 0; t < SUBTILES; t++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) total[nb][i] = 0.f;
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) total[t][nb][i] = 0.f;
             // A STEP is the part of a batch whose sums are kept apart: a unit (GPU = 1), else half a unit, GPU / 2 groups.
             // scales of a step for row `row` of the tile, row ra of W: GROUPS times 16 bits
             auto scales_of = [&](const uint8_t *slot, int row, size_t ra, int step) -> uint32_t {
@@ -481,58 +490,74 @@ __global__ void __launch_bounds__(32 * T::template WARPS<WHOLE>, 1) w4_matvec_ke
                 }
             };
             auto compute = [&](const uint8_t *slot, uint32_t from, int step) {
-                const size_t ra = row0 + min(tile * T::TILE + g, rows - 1), rb = row0 + min(tile * T::TILE + g + 8, rows - 1);
-                const uint32_t sa = scales_of(slot, g, ra, step), sb = scales_of(slot, g + 8, rb, step);
-                uint32_t za = 0, zb = 0;
-                if (ZERO) {
-                    za = zeros_of(slot, g, ra, step);
-                    zb = zeros_of(slot, g + 8, rb, step);
+                uint32_t sa[SUBTILES], sb[SUBTILES], za[SUBTILES], zb[SUBTILES];       // of rows g and g + 8 of a subtile
+#pragma unroll
+                for (int t = 0; t < SUBTILES; t++) {
+                    const int r = t * 16 + g;
+                    const size_t ra = row0 + min(tile * TILE + r, rows - 1), rb = row0 + min(tile * TILE + r + 8, rows - 1);
+                    sa[t] = scales_of(slot, r, ra, step);
+                    sb[t] = scales_of(slot, r + 8, rb, step);
+                    za[t] = ZERO ? zeros_of(slot, r, ra, step) : 0;
+                    zb[t] = ZERO ? zeros_of(slot, r + 8, rb, step) : 0;
                 }
                 const uint32_t x_off = batch * 512 + step * (64 * SUBS), s_off = sums_at + (batch * (2 * GPU) + step * GROUPS) * (NB * 32) + c * 8;
-                float lo[NB][4], hi[NB][4];
+                float lo[SUBTILES][NB][4], hi[SUBTILES][NB][4];
 #pragma unroll
                 for (int pair = 0; pair < SUBS / 2; pair++) {
-                    uint32_t q[4];                       // rows g, g + 8 of a piece, then of the next
+                    uint32_t q[SUBTILES][4];             // rows g, g + 8 of a piece, then of the next
                     // piece 2 h of a unit lies where piece 0 does, bit 5 of the address flipped for h = 1
-                    w4_ldmatrix(q, GPU == 1 ? (from + step * T::UNIT_BYTES) ^ (pair * 32) : (from + (step >> 1) * T::UNIT_BYTES) ^ ((step & 1) * 32));
+#pragma unroll
+                    for (int t = 0; t < SUBTILES; t++)
+                        w4_ldmatrix(q[t], (GPU == 1 ? (from + step * T::UNIT_BYTES) ^ (pair * 32) : (from + (step >> 1) * T::UNIT_BYTES) ^ ((step & 1) * 32)) + t * 1024);
 #pragma unroll
                     for (int sub = 0; sub < 2; sub++) {
                         const int j = 2 * pair + sub;    // piece of the step
-                        const uint32_t qa = q[2 * sub], qb = q[2 * sub + 1], va = qa >> 8, vb = qb >> 8;
-                        const uint32_t la0 = w4_pick<0x000f000fu>(qa, flip_lo), lb0 = w4_pick<0x000f000fu>(qb, flip_lo);
-                        const uint32_t la1 = w4_pick<0x000f000fu>(va, flip_lo), lb1 = w4_pick<0x000f000fu>(vb, flip_lo);
-                        const uint32_t ha0 = w4_pick<0x00f000f0u>(qa, flip_hi), hb0 = w4_pick<0x00f000f0u>(qb, flip_hi);
-                        const uint32_t ha1 = w4_pick<0x00f000f0u>(va, flip_hi), hb1 = w4_pick<0x00f000f0u>(vb, flip_hi);
                         const int grp = j / GROUP_SUBS;  // group of the step
-                        float fa = 1.f, fb = 1.f;
-                        if (ZERO && j % GROUP_SUBS == 0) {      // 2^23 + z is exact in FP32
-                            fa = __uint_as_float((za >> (4 * grp) & 15u) | 0x4b000000u) - 8388608.f;
-                            fb = __uint_as_float((zb >> (4 * grp) & 15u) | 0x4b000000u) - 8388608.f;
-                        }
+                        uint4 x[NB];
+                        float2 s[NB];
 #pragma unroll
                         for (int nb = 0; nb < NB; nb++) {
-                            const uint4 x = *reinterpret_cast<const uint4 *>(smem + xbase[nb] + x_off + j * 64);
-                            if (j % GROUP_SUBS == 0) {
-                                const float2 s = *reinterpret_cast<const float2 *>(smem + s_off + grp * (NB * 32) + nb * 32);
-                                W4Type<E>::mma(lo[nb], la0, lb0, la1, lb1, x.x, x.y, fa * s.x, fa * s.y, fb * s.x, fb * s.y);
-                                W4Type<E>::mma(hi[nb], ha0, hb0, ha1, hb1, x.z, x.w, 0.f, 0.f, 0.f, 0.f);
-                            } else {
-                                W4Type<E>::mma(lo[nb], la0, lb0, la1, lb1, x.x, x.y, lo[nb][0], lo[nb][1], lo[nb][2], lo[nb][3]);
-                                W4Type<E>::mma(hi[nb], ha0, hb0, ha1, hb1, x.z, x.w, hi[nb][0], hi[nb][1], hi[nb][2], hi[nb][3]);
-                            }
+                            x[nb] = *reinterpret_cast<const uint4 *>(smem + xbase[nb] + x_off + j * 64);
+                            if (j % GROUP_SUBS == 0) s[nb] = *reinterpret_cast<const float2 *>(smem + s_off + grp * (NB * 32) + nb * 32);
                         }
-                        if ((j + 1) % GROUP_SUBS == 0) {
-                            auto scale = [](uint32_t word, int which) {
-                                const uint16_t bits = (uint16_t)(which ? word >> 16 : word);
-                                return W4Type<E>::to_f32(*reinterpret_cast<const E *>(&bits));
-                            };
-                            const float s_a = scale(sa, grp), s_b = scale(sb, grp);
+#pragma unroll
+                        for (int t = 0; t < SUBTILES; t++) {
+                            const uint32_t qa = q[t][2 * sub], qb = q[t][2 * sub + 1], va = qa >> 8, vb = qb >> 8;
+                            const uint32_t la0 = w4_pick<0x000f000fu>(qa, flip_lo), lb0 = w4_pick<0x000f000fu>(qb, flip_lo);
+                            const uint32_t la1 = w4_pick<0x000f000fu>(va, flip_lo), lb1 = w4_pick<0x000f000fu>(vb, flip_lo);
+                            const uint32_t ha0 = w4_pick<0x00f000f0u>(qa, flip_hi), hb0 = w4_pick<0x00f000f0u>(qb, flip_hi);
+                            const uint32_t ha1 = w4_pick<0x00f000f0u>(va, flip_hi), hb1 = w4_pick<0x00f000f0u>(vb, flip_hi);
+                            float fa = 1.f, fb = 1.f;
+                            if (ZERO && j % GROUP_SUBS == 0) {      // 2^23 + z is exact in FP32
+                                fa = __uint_as_float((za[t] >> (4 * grp) & 15u) | 0x4b000000u) - 8388608.f;
+                                fb = __uint_as_float((zb[t] >> (4 * grp) & 15u) | 0x4b000000u) - 8388608.f;
+                            }
 #pragma unroll
                             for (int nb = 0; nb < NB; nb++) {
-                                total[nb][0] = fmaf(s_a, fmaf(hi[nb][0], 0.0625f, lo[nb][0]), total[nb][0]);
-                                total[nb][1] = fmaf(s_a, fmaf(hi[nb][1], 0.0625f, lo[nb][1]), total[nb][1]);
-                                total[nb][2] = fmaf(s_b, fmaf(hi[nb][2], 0.0625f, lo[nb][2]), total[nb][2]);
-                                total[nb][3] = fmaf(s_b, fmaf(hi[nb][3], 0.0625f, lo[nb][3]), total[nb][3]);
+                                float (&l)[4] = lo[t][nb], (&h)[4] = hi[t][nb];
+                                if (j % GROUP_SUBS == 0) {
+                                    W4Type<E>::mma(l, la0, lb0, la1, lb1, x[nb].x, x[nb].y, fa * s[nb].x, fa * s[nb].y, fb * s[nb].x, fb * s[nb].y);
+                                    W4Type<E>::mma(h, ha0, hb0, ha1, hb1, x[nb].z, x[nb].w, 0.f, 0.f, 0.f, 0.f);
+                                } else {
+                                    W4Type<E>::mma(l, la0, lb0, la1, lb1, x[nb].x, x[nb].y, l[0], l[1], l[2], l[3]);
+                                    W4Type<E>::mma(h, ha0, hb0, ha1, hb1, x[nb].z, x[nb].w, h[0], h[1], h[2], h[3]);
+                                }
+                            }
+                            if ((j + 1) % GROUP_SUBS == 0) {
+                                auto scale = [](uint32_t word, int which) {
+                                    const uint16_t bits = (uint16_t)(which ? word >> 16 : word);
+                                    return W4Type<E>::to_f32(*reinterpret_cast<const E *>(&bits));
+                                };
+                                const float s_a = scale(sa[t], grp), s_b = scale(sb[t], grp);
+#pragma unroll
+                                for (int nb = 0; nb < NB; nb++) {
+                                    float (&sum)[4] = total[t][nb];
+                                    const float (&l)[4] = lo[t][nb], (&h)[4] = hi[t][nb];
+                                    sum[0] = fmaf(s_a, fmaf(h[0], 0.0625f, l[0]), sum[0]);
+                                    sum[1] = fmaf(s_a, fmaf(h[1], 0.0625f, l[1]), sum[1]);
+                                    sum[2] = fmaf(s_b, fmaf(h[2], 0.0625f, l[2]), sum[2]);
+                                    sum[3] = fmaf(s_b, fmaf(h[3], 0.0625f, l[3]), sum[3]);
+                                }
                             }
                         }
                     }
@@ -545,7 +570,7 @@ __global__ void __launch_bounds__(32 * T::template WARPS<WHOLE>, 1) w4_matvec_ke
                 // one step after the other where the registers are short
                 constexpr int UNROLL = GPU == 1 && NB == 1 ? 2 : 1;
 #pragma unroll UNROLL
-                for (int step = 0; step < STEPS; step++) compute(smem + T::PART_BYTES + warp * (RING * SLOT) + slot, ring + slot + get_at, step);
+                for (int step = 0; step < STEPS; step++) compute(smem + warp * (RING * SLOT) + slot, ring + slot + get_at, step);
                 __syncwarp();                            // every lane has read the slot
                 load(slot);
                 slot = slot == (RING - 1) * SLOT ? 0 : slot + SLOT;
@@ -558,16 +583,16 @@ __global__ void __launch_bounds__(32 * T::template WARPS<WHOLE>, 1) w4_matvec_ke
                         for (int i = 0; i < 2; i++) {
                             const int m = nb * 8 + 2 * c + i;
                             if (m < M) {
-                                float *to = part + (wk * M + m) * p.block_rows + tile * T::TILE + g;
-                                float v0 = total[nb][i] * W4Type<E>::OUT, v1 = total[nb][2 + i] * W4Type<E>::OUT;
-                                if (W4Type<E>::RESCALE) {
-                                    v0 *= xrows->down[m];
-                                    v1 *= xrows->down[m];
+                                float *to = part + (wk * M + m) * p.block_rows + tile * TILE + g;
+                                const float out = W4Type<E>::RESCALE ? xrows->down[m] : 1.f;
+#pragma unroll
+                                for (int k = 0; k < 2 * SUBTILES; k++) {
+                                    const float v = total[k / 2][nb][2 * (k % 2) + i] * W4Type<E>::OUT * out;
+                                    to[8 * k] = u0 == 0 ? v : to[8 * k] + v;
                                 }
-                                to[0] = u0 == 0 ? v0 : to[0] + v0;
-                                to[8] = u0 == 0 ? v1 : to[8] + v1;
                             }
-                            total[nb][i] = total[nb][2 + i] = 0.f;
+#pragma unroll
+                            for (int k = 0; k < 2 * SUBTILES; k++) total[k / 2][nb][2 * (k % 2) + i] = 0.f;
                         }
                     batch = wk;
                     tile += WR;
@@ -625,25 +650,39 @@ struct W4MatvecLauncher {
         if (rc != GEMM_OK) return rc;
         int grid = a.sm_limit > 0 && a.sm_limit < sms ? a.sm_limit : sms;
         if (grid > a.N) grid = a.N;
-        // partial sums: rows of a CTA x M x WK floats; as many K slices as fit (a tile's bytes then arrive soonest), blocks of
-        // rows when not even one slice of all rows does
         const int gpu = T::UNIT >> p.group_shift, rows = (a.N + grid - 1) / grid, units = (a.K + T::UNIT - 1) / T::UNIT;
         // how scales and zero points come: with whole batches, else in words around them (base 4-byte aligned), else one by one
         // when they are needed
         const bool whole = a.K % (2 * T::UNIT) == 0 && bits(a.w_scale) % (4 * gpu) == 0 && bits(a.w_zero) % 4 == 0;
-        const int most_units = (T::x_bytes(gpu) - a.M * 64) / (a.M * T::UNIT * 2 + gpu * T::NB * 32) / 2 * 2, passes = (units + most_units - 1) / most_units;
-        p.units_per_pass = ((units + passes - 1) / passes + 1) / 2 * 2;
-        const int slots = T::PART_BYTES / (int)sizeof(float) / a.M, padded = (rows + T::TILE - 1) / T::TILE * T::TILE;
-        p.wk_shift = T::NB == 1 || whole ? 4 : 3;
-        while (p.wk_shift > 0 && ((2 << p.wk_shift) > p.units_per_pass || (padded << p.wk_shift) > slots)) p.wk_shift--;
-        const int most_rows = (slots >> p.wk_shift) / T::TILE * T::TILE, blocks = (padded + most_rows - 1) / most_rows;
-        p.block_rows = ((padded + blocks - 1) / blocks + T::TILE - 1) / T::TILE * T::TILE;
         p.scale_window = bits(a.w_scale) % 4 == 0;
         p.zero_window = bits(a.w_zero) % 4 == 0;
+        // The plan: WK slices of K leave WARPS / WK groups for the tiles, and WK partial sums of every result in shared memory,
+        // which X shares (what does not fit goes in passes).  The WK with the fewest rounds of batches is taken, counting a pass
+        // as 4 of them (its staging), the largest of equals (a tile's bytes then arrive soonest).
+        const int fixed = T::ring_bytes(gpu) + T::ROW_BYTES, padded = (rows + T::TILE - 1) / T::TILE * T::TILE;
+        long long best = -1;
+        for (int shift = T::WARPS == 16 ? 4 : 3; shift >= 0; shift--) {
+            const int wk = 1 << shift, per_tile = wk * a.M * T::TILE * (int)sizeof(float);
+            const int most_rows = (T::SMEM_ALLOC - fixed) / 2 / per_tile * T::TILE;       // at most half of the rest
+            if (most_rows == 0) continue;
+            const int blocks = (padded + most_rows - 1) / most_rows, block_rows = ((padded + blocks - 1) / blocks + T::TILE - 1) / T::TILE * T::TILE;
+            const int part_bytes = block_rows / T::TILE * per_tile;
+            const int most_units = (T::SMEM_ALLOC - fixed - part_bytes - a.M * 64) / (a.M * T::UNIT * 2 + gpu * T::NB * 32) / 2 * 2;
+            const int passes = (units + most_units - 1) / most_units, per_pass = ((units + passes - 1) / passes + 1) / 2 * 2;
+            if (per_pass < 2 * wk && wk > 1) continue;
+            const int groups_of_tiles = T::WARPS / wk, tiles = block_rows / T::TILE;
+            const long long cost = (long long)blocks * passes * ((long long)((tiles + groups_of_tiles - 1) / groups_of_tiles) * ((per_pass / 2 + wk - 1) / wk) + 4);
+            if (best >= 0 && cost >= best) continue;
+            best = cost;
+            p.wk_shift = shift;
+            p.block_rows = block_rows;
+            p.units_per_pass = per_pass;
+            p.part_at = fixed + T::staged_bytes(a.M, per_pass, gpu);
+        }
+        const int smem = p.part_at + p.block_rows * a.M * (int)sizeof(float) * (1 << p.wk_shift);
         const size_t groups = (size_t)a.K / a.group_size;
         p.scales_end = static_cast<const uint8_t *>(a.w_scale) + (size_t)a.N * groups * 2;
         p.zeros_end = a.w_zero ? p.zeros + (size_t)a.N * ((groups + 1) / 2) : nullptr;
-        const int smem = T::PART_BYTES + T::ring_bytes(gpu) + T::ROW_BYTES + T::staged_bytes(a.M, p.units_per_pass, gpu);
         if (a.x_dtype == GEMM_X_F16) return launch<__half>(p, whole, grid, smem, a.stream);
         return launch<__nv_bfloat16>(p, whole, grid, smem, a.stream);
     }
@@ -688,7 +727,7 @@ private:
             SM100_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM_ALLOC));
             attr_set[dev].store(true, std::memory_order_release);
         }
-        cudaLaunchConfig_t cfg = dependent_launch_config(grid, 32 * T::template WARPS<WHOLE>, stream);
+        cudaLaunchConfig_t cfg = dependent_launch_config(grid, T::THREADS, stream);
         cfg.dynamicSmemBytes = smem;
         SM100_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p));
         return GEMM_OK;
