@@ -53,6 +53,7 @@ struct W4MatvecParams {
     int block_rows;              // rows of W whose partial sums shared memory holds
     int units_per_pass;          // units (128 K-elements) of X that shared memory holds
     int wk_shift;                // log2(WK)
+    int ring;                    // batches in flight per warp
     int part_at;                 // partial sums: byte offset in shared memory
     int scale_window, zero_window;       // scales / zero points reach the ring in words around them, else they are read when needed
     const uint8_t *scales_end, *zeros_end;
@@ -66,6 +67,13 @@ struct W4Type<__nv_bfloat16> {
     static constexpr bool RESCALE = true;
     static constexpr int K_USUAL = 100;          // X is staged as x * 2^K_USUAL
     static constexpr uint32_t TWO_K_USUAL = 0x71807180u;
+    // the larger magnitude of each half (its sign may be either's; a NaN gives way)
+    static __device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b)
+    {
+        uint32_t r;
+        asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
     static __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b)
     {
         uint32_t r;
@@ -105,14 +113,14 @@ struct W4MatvecTraits {
     // tile is 32 rows of W, so that what is read of X is used twice; that takes the registers of 8 warps.
     static constexpr int SUBTILES = NB, TILE = 16 * SUBTILES, UNIT = 128;
     static constexpr int WARPS = NB == 1 ? 16 : 8, THREADS = 32 * WARPS;
-    static constexpr int RING = NB == 1 ? 3 : 2;     // batches of two units in flight per warp
+    static constexpr int MOST_RING = 3;              // batches of two units in flight per warp: 3, or 2 where X needs the room
     static constexpr int UNIT_BYTES = TILE * UNIT / 2;
     static constexpr int AHEAD_ROWS = 32;            // rows of W asked into L2 before the grid before has ended
     // a batch in the ring: two units, then per row the scales of its 2 GPU groups and a word in front of them, then per row
     // two words around its zero points
     static __host__ __device__ constexpr int scale_pitch(int gpu) { return 8 * gpu; }
     static __host__ __device__ constexpr int slot_bytes(int gpu) { return 2 * UNIT_BYTES + TILE * scale_pitch(gpu) + TILE * 8; }
-    static __host__ __device__ constexpr int ring_bytes(int gpu) { return WARPS * RING * slot_bytes(gpu); }
+    static __host__ __device__ constexpr int ring_bytes(int gpu, int ring) { return WARPS * ring * slot_bytes(gpu); }
     static constexpr int ROW_BYTES = 256;            // per row of X: scaling, flags
     static constexpr int SMEM_ALLOC = 227 * 1024;    // ring, flags, staged X and its sums, partial sums
     // staged X: rows 64 bytes longer than their units, so that the eight lanes of a 16-byte access (two rows) reach all banks
@@ -196,52 +204,74 @@ struct W4Rows {
 };
 
 // Staging of `nu` units of X from unit u0 on ([m][unit][32 k][c]: 8 values, 16 bytes; x behind K is 0).  A thread copies its
-// pieces, all of them in flight at once, and then rewrites each in its place.
-template <int WARPS, class T, class F>
-__device__ __forceinline__ void w4_x_pieces(int M, int nu, int warp, int lane, F &&piece)
-{
-    for (int m = 0; m < M; m++)
-        for (int u = 2 * warp + (lane >> 4); u < nu; u += 2 * WARPS) piece(m, u);          // 16 lanes to the 128 values of a unit
-}
+// pieces, all of them in flight at once, and then rewrites each in its place; 16 lanes to the 128 values of a unit.
 template <int WARPS, class T>
 __device__ __forceinline__ void w4_copy_x(const W4MatvecParams &p, uint32_t xs, int u0, int nu, int warp, int lane)
 {
-    const int row_bytes = T::x_row_bytes(p.units_per_pass), at = lane & 15;
-    w4_x_pieces<WARPS, T>(p.M, nu, warp, lane, [&](int m, int u) {
-        const int k = (u0 + u) * T::UNIT + at * 8;
-        const uint8_t *X = static_cast<const uint8_t *>(p.X);
-        w4_copy16(xs + m * row_bytes + u * 256 + at * 16, k < p.K ? X + ((size_t)m * p.K + k) * 2 : X, k < p.K ? 16 : 0);
-    });
+    const int first = 2 * warp + (lane >> 4), at = lane & 15;
+    const uint8_t *X = static_cast<const uint8_t *>(p.X) + ((size_t)(u0 + first) * T::UNIT + at * 8) * 2;
+    uint32_t row = xs + first * 256 + at * 16;
+    for (int m = 0; m < p.M; m++) {
+        int k = (u0 + first) * T::UNIT + at * 8;
+        const uint8_t *from = X;
+        uint32_t to = row;
+        for (int u = first; u < nu; u += 2 * WARPS) {
+            w4_copy16(to, k < p.K ? from : static_cast<const uint8_t *>(p.X), k < p.K ? 16 : 0);
+            k += 2 * WARPS * T::UNIT;
+            from += 2 * WARPS * T::UNIT * 2;
+            to += 2 * WARPS * 256;
+        }
+        X += (size_t)p.K * 2;
+        row += T::x_row_bytes(p.units_per_pass);
+    }
     w4_copies_commit();
 }
-// Returns whether this thread saw an |x| of 2^19 or more, or no finite number (bf16).
+// Returns whether this thread saw an |x| of 2^19 or more (bf16).
 template <class E, int WARPS, class T>
 __device__ __forceinline__ bool w4_order_x(const W4MatvecParams &p, uint8_t *xs, W4Rows *rows, int nu, bool usual, int warp, int lane)
 {
-    const int row_bytes = T::x_row_bytes(p.units_per_pass), at = lane & 15;
+    constexpr int AT_ONCE = 4;                       // rows side by side: each piece is a round trip to shared memory
+    const int first = 2 * warp + (lane >> 4), at = lane & 15, row_bytes = T::x_row_bytes(p.units_per_pass);
     bool far = false;
-    w4_x_pieces<WARPS, T>(p.M, nu, warp, lane, [&](int m, int u) {
-        uint4 *piece = reinterpret_cast<uint4 *>(xs + m * row_bytes + u * 256 + at * 16);
-        const uint4 v = *piece;
-        uint32_t q[4] = {v.x, v.y, v.z, v.w};
+    for (int m0 = 0; m0 < p.M; m0 += AT_ONCE) {
+        uint32_t most[AT_ONCE] = {}, up[AT_ONCE];
         if constexpr (W4Type<E>::RESCALE) {
-            uint32_t most = 0;
 #pragma unroll
-            for (int i = 0; i < 4; i++) asm("max.u16x2 %0, %0, %1;" : "+r"(most) : "r"(q[i] & 0x7fff7fffu));      // |x| order like their bits
-            most = max(most >> 16, most & 0xffffu);
-            if (most >= 0x4900u) far = true;                        // 2^19
-            if (most >= 0x2b80u) rows->ordinary[m] = 1;             // 2^-40; every thread that gets here writes the same
-            if (!usual) {
-                const uint32_t up = (__float_as_uint(rows->up[m]) >> 16) * 0x00010001u;
-#pragma unroll
-                for (int i = 0; i < 4; i++) q[i] = W4Type<E>::mul2(q[i], up);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++) q[i] = W4Type<E>::mul2(q[i], W4Type<E>::TWO_K_USUAL);
+            for (int j = 0; j < AT_ONCE; j++) up[j] = usual || m0 + j >= p.M ? 0x3f803f80u : (__float_as_uint(rows->up[m0 + j]) >> 16) * 0x00010001u;
         }
-        // the pairs (0,4), (2,6), (1,5), (3,7) of the eight values: operands of the lo sums, then of the hi sums
-        *piece = make_uint4(__byte_perm(q[0], q[2], 0x5410), __byte_perm(q[1], q[3], 0x5410), __byte_perm(q[0], q[2], 0x7632), __byte_perm(q[1], q[3], 0x7632));
-    });
+        uint8_t *row = xs + m0 * row_bytes + first * 256 + at * 16;
+        for (int u = first; u < nu; u += 2 * WARPS) {
+            uint4 v[AT_ONCE];
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; j++)
+                if (m0 + j < p.M) v[j] = *reinterpret_cast<const uint4 *>(row + j * row_bytes);
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; j++) {
+                if (m0 + j >= p.M) break;
+                uint32_t q[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+                if constexpr (W4Type<E>::RESCALE) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        most[j] = W4Type<E>::max_abs2(most[j], q[i]);
+                        if (!usual) q[i] = W4Type<E>::mul2(q[i], up[j]);
+                        q[i] = W4Type<E>::mul2(q[i], W4Type<E>::TWO_K_USUAL);
+                    }
+                }
+                // the pairs (0,4), (2,6), (1,5), (3,7) of the eight values: operands of the lo sums, then of the hi sums
+                *reinterpret_cast<uint4 *>(row + j * row_bytes) = make_uint4(__byte_perm(q[0], q[2], 0x5410), __byte_perm(q[1], q[3], 0x5410),
+                                                                             __byte_perm(q[0], q[2], 0x7632), __byte_perm(q[1], q[3], 0x7632));
+            }
+            row += 2 * WARPS * 256;
+        }
+        if constexpr (W4Type<E>::RESCALE) {
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; j++) {
+                const uint32_t top = max(most[j] & 0x7fffu, most[j] >> 16 & 0x7fffu);
+                if (top >= 0x4900u) far = true;                                     // 2^19
+                if (top >= 0x2b80u && m0 + j < p.M) rows->ordinary[m0 + j] = 1;     // 2^-40; every thread that gets here writes the same
+            }
+        }
+    }
     return far;
 }
 
@@ -253,16 +283,16 @@ __device__ __forceinline__ void w4_sum_x(const uint8_t *smem, const uint32_t (&x
     for (int u = warp; u < nu; u += WARPS)
 #pragma unroll
         for (int nb = 0; nb < T::NB; nb++) {
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            float even[4], odd[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const uint4 x = *reinterpret_cast<const uint4 *>(smem + xbase[nb] + u * 256 + j * 64);
-                if (j % (4 / GPU) == 0) acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
-                W4Type<E>::mma(acc, A, A, A, A, x.x, x.y, acc[0], acc[1], acc[2], acc[3]);
-                W4Type<E>::mma(acc, A, A, A, A, x.z, x.w, acc[0], acc[1], acc[2], acc[3]);
+                if (j % (4 / GPU) == 0) even[0] = even[1] = even[2] = even[3] = odd[0] = odd[1] = odd[2] = odd[3] = 0.f;
+                W4Type<E>::mma(even, A, A, A, A, x.x, x.y, even[0], even[1], even[2], even[3]);
+                W4Type<E>::mma(odd, A, A, A, A, x.z, x.w, odd[0], odd[1], odd[2], odd[3]);
                 // every row of the product is the same; lane c of the first quad holds columns 2c, 2c + 1
                 if ((j + 1) % (4 / GPU) == 0 && lane < 4)
-                    *reinterpret_cast<float2 *>(sums + (u * GPU + j / (4 / GPU)) * (T::NB * 8) + nb * 8 + 2 * lane) = make_float2(acc[0], acc[1]);
+                    *reinterpret_cast<float2 *>(sums + (u * GPU + j / (4 / GPU)) * (T::NB * 8) + nb * 8 + 2 * lane) = make_float2(even[0] + odd[0], even[1] + odd[1]);
             }
         }
 }
@@ -298,12 +328,13 @@ __device__ __forceinline__ void w4_rescale_rows(const W4MatvecParams &p, W4Rows 
 template <class E, int GPU, bool ZERO, bool WHOLE, class T>
 __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4MatvecParams p)
 {
-    constexpr int NB = T::NB, WARPS = T::WARPS, THREADS = T::THREADS, RING = T::RING, SUBTILES = T::SUBTILES, TILE = T::TILE;
+    constexpr int NB = T::NB, WARPS = T::WARPS, THREADS = T::THREADS, SUBTILES = T::SUBTILES, TILE = T::TILE;
     constexpr int LANES_PER_ROW = 32 / TILE;             // that bring its scales and zero points
     constexpr int GROUP_SUBS = 4 / GPU;                  // pieces of 32 k in a group
     constexpr int STEPS = GPU == 1 ? 2 : 4, SUBS = 8 / STEPS, GROUPS = 2 * GPU / STEPS;      // steps of a batch, pieces and groups of a step
     constexpr int SLOT = T::slot_bytes(GPU), SCALES_AT = 2 * T::UNIT_BYTES, SCALE_PITCH = T::scale_pitch(GPU), ZEROS_AT = SCALES_AT + TILE * SCALE_PITCH;
-    constexpr int X_AT = T::ring_bytes(GPU) + T::ROW_BYTES;
+    const int ring_slots = p.ring;
+    const uint32_t X_AT = T::ring_bytes(GPU, ring_slots) + T::ROW_BYTES;
     extern __shared__ __align__(16) uint8_t smem[];
     float *part = reinterpret_cast<float *>(smem + p.part_at);      // [WK][M][block_rows]
     W4Rows *xrows = reinterpret_cast<W4Rows *>(smem + X_AT - T::ROW_BYTES);
@@ -325,7 +356,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
     // The ring holds a unit as TILE rows of four 16-byte pieces; piece j of row r lies at (r, j ^ (r / 2 % 4)), so that the
     // eight rows of a matrix reach all banks.  Copies: lane (g, c) brings piece c of rows g, g + 8, ...  ldmatrix: lane l
     // names row l % 16 and piece l / 16 (then 2 more) of the four matrices (rows 0-7, 8-15) x (piece j, j + 1).
-    const uint32_t ring = smem_u32(smem) + warp * (RING * SLOT);
+    const uint32_t ring = smem_u32(smem) + warp * (ring_slots * SLOT);
     const uint32_t put_at = g * 64 + ((c ^ (g >> 1 & 3)) << 4);
     const uint32_t get_at = (lane & 15) * 64 + (((lane >> 4) ^ (lane >> 1 & 3)) << 4);
     const uint32_t flip_lo = ZERO ? 0u : w4_keep(0x00080008u), flip_hi = ZERO ? 0u : w4_keep(0x00800080u);
@@ -434,10 +465,10 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
                 }
                 w4_copy_x<WARPS, T>(p, smem_u32(smem + X_AT), u0, 2 * batches, warp, lane);
             }
-#pragma unroll
-            for (int d = 0; d < RING; d++) load(d * SLOT);
+            for (int d = 0; d < ring_slots; d++) load(d * SLOT);
             if (stage) {
-                w4_copies_wait<RING>();              // this thread's pieces of X
+                if (ring_slots == 3) w4_copies_wait<3>();    // this thread's pieces of X
+                else w4_copies_wait<2>();
                 __syncthreads();                     // the flags
 #pragma unroll 1
                 for (bool usual = true;; usual = false) {
@@ -565,15 +596,16 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
             };
             uint32_t slot = 0;
             while (tile < tiles) {
-                w4_copies_wait<RING - 1>();
+                if (ring_slots == 3) w4_copies_wait<2>();
+                else w4_copies_wait<1>();
                 __syncwarp();                            // the other lanes' copies too
                 // one step after the other where the registers are short
                 constexpr int UNROLL = GPU == 1 && NB == 1 ? 2 : 1;
 #pragma unroll UNROLL
-                for (int step = 0; step < STEPS; step++) compute(smem + warp * (RING * SLOT) + slot, ring + slot + get_at, step);
+                for (int step = 0; step < STEPS; step++) compute(smem + warp * (ring_slots * SLOT) + slot, ring + slot + get_at, step);
                 __syncwarp();                            // every lane has read the slot
                 load(slot);
-                slot = slot == (RING - 1) * SLOT ? 0 : slot + SLOT;
+                slot = slot == (ring_slots - 1) * SLOT ? 0 : slot + SLOT;
                 batch += WK;
                 if (batch >= batches) {
                     // the warp's share of this tile is complete: its partial sums go to its own slot
@@ -657,27 +689,33 @@ struct W4MatvecLauncher {
         p.scale_window = bits(a.w_scale) % 4 == 0;
         p.zero_window = bits(a.w_zero) % 4 == 0;
         // The plan: WK slices of K leave WARPS / WK groups for the tiles, and WK partial sums of every result in shared memory,
-        // which X shares (what does not fit goes in passes).  The WK with the fewest rounds of batches is taken, counting a pass
-        // as 4 of them (its staging), the largest of equals (a tile's bytes then arrive soonest).
-        const int fixed = T::ring_bytes(gpu) + T::ROW_BYTES, padded = (rows + T::TILE - 1) / T::TILE * T::TILE;
+        // which the ring and X share (what does not fit of X goes in passes).  The one with the fewest rounds of batches is
+        // taken, counting a pass as 8 of them (its staging) and a ring of 2 batches instead of 3 as an eighth more; of equals
+        // the longest ring and the largest WK (a tile's bytes then arrive soonest).
+        const int padded = (rows + T::TILE - 1) / T::TILE * T::TILE;
         long long best = -1;
-        for (int shift = T::WARPS == 16 ? 4 : 3; shift >= 0; shift--) {
-            const int wk = 1 << shift, per_tile = wk * a.M * T::TILE * (int)sizeof(float);
-            const int most_rows = (T::SMEM_ALLOC - fixed) / 2 / per_tile * T::TILE;       // at most half of the rest
-            if (most_rows == 0) continue;
-            const int blocks = (padded + most_rows - 1) / most_rows, block_rows = ((padded + blocks - 1) / blocks + T::TILE - 1) / T::TILE * T::TILE;
-            const int part_bytes = block_rows / T::TILE * per_tile;
-            const int most_units = (T::SMEM_ALLOC - fixed - part_bytes - a.M * 64) / (a.M * T::UNIT * 2 + gpu * T::NB * 32) / 2 * 2;
-            const int passes = (units + most_units - 1) / most_units, per_pass = ((units + passes - 1) / passes + 1) / 2 * 2;
-            if (per_pass < 2 * wk && wk > 1) continue;
-            const int groups_of_tiles = T::WARPS / wk, tiles = block_rows / T::TILE;
-            const long long cost = (long long)blocks * passes * ((long long)((tiles + groups_of_tiles - 1) / groups_of_tiles) * ((per_pass / 2 + wk - 1) / wk) + 4);
-            if (best >= 0 && cost >= best) continue;
-            best = cost;
-            p.wk_shift = shift;
-            p.block_rows = block_rows;
-            p.units_per_pass = per_pass;
-            p.part_at = fixed + T::staged_bytes(a.M, per_pass, gpu);
+        for (int ring = T::MOST_RING; ring >= 2; ring--) {
+            const int fixed = T::ring_bytes(gpu, ring) + T::ROW_BYTES;
+            for (int shift = T::WARPS == 16 ? 4 : 3; shift >= 0; shift--) {
+                const int wk = 1 << shift, per_tile = wk * a.M * T::TILE * (int)sizeof(float);
+                const int most_rows = (T::SMEM_ALLOC - fixed) / 2 / per_tile * T::TILE;       // at most half of the rest
+                if (most_rows == 0) continue;
+                const int blocks = (padded + most_rows - 1) / most_rows, block_rows = ((padded + blocks - 1) / blocks + T::TILE - 1) / T::TILE * T::TILE;
+                const int part_bytes = block_rows / T::TILE * per_tile;
+                const int most_units = (T::SMEM_ALLOC - fixed - part_bytes - a.M * 64) / (a.M * T::UNIT * 2 + gpu * T::NB * 32) / 2 * 2;
+                const int passes = (units + most_units - 1) / most_units, per_pass = ((units + passes - 1) / passes + 1) / 2 * 2;
+                if (per_pass < 2 * wk && wk > 1) continue;
+                const int groups_of_tiles = T::WARPS / wk, tiles = block_rows / T::TILE;
+                const long long rounds = (long long)((tiles + groups_of_tiles - 1) / groups_of_tiles) * ((per_pass / 2 + wk - 1) / wk);
+                const long long cost = (long long)blocks * passes * (rounds * (11 - ring) + 8 * 8);
+                if (best >= 0 && cost >= best) continue;
+                best = cost;
+                p.ring = ring;
+                p.wk_shift = shift;
+                p.block_rows = block_rows;
+                p.units_per_pass = per_pass;
+                p.part_at = fixed + T::staged_bytes(a.M, per_pass, gpu);
+            }
         }
         const int smem = p.part_at + p.block_rows * a.M * (int)sizeof(float) * (1 << p.wk_shift);
         const size_t groups = (size_t)a.K / a.group_size;
