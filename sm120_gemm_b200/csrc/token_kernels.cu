@@ -58,55 +58,134 @@ struct RotaryParams {
     const void *x;
     void *y;
     const long long *positions;
-    long long tokens, x_token, x_head, y_token, y_head;
-    int heads, dim, rot, layout, backward;
+    long long tokens, x_token, x_head, y_token, y_head;      // strides in elements
+    int heads, dim, rot, backward;
     float scale;
+    int turned, units;           // units of a head: the first `turned` hold pairs, the others elements behind them
+    int slots;                   // head slots of a token: a thread takes the heads slot, slot + slots, ...
+    unsigned per_slice;          // tokens of one grid.y
 };
 
-// cos and sin (times scale) of `phase` / 2^64 turns: the nearest quarter turn is taken off exactly, the rest (at most an
-// eighth of a turn) is converted to FP32 with full relative accuracy
+// cos and sin (times scale) of `phase` / 2^64 turns.  16-bit data: the hardware's sine of the nearest half turn either way,
+// off by at most 2^-21.4, and 2^-22.3 from the angle's conversion.
+template <class T>
 __device__ __forceinline__ float2 cos_sin(unsigned long long phase, float scale)
 {
-    const unsigned quarter = (unsigned)((phase + (1ull << 61)) >> 62);
-    const long long rest = (long long)(phase - ((unsigned long long)quarter << 62));
-    float s, c;
-    sincospif((float)rest * 1.0842021724855044e-19f /* 2^-63: half turns */, &s, &c);
-    float cq = (quarter & 1) ? s : c, sq = (quarter & 1) ? c : s;
-    if (quarter == 1 || quarter == 2) cq = -cq;
-    if (quarter & 2) sq = -sq;
-    return make_float2(cq * scale, sq * scale);
+    if constexpr (sizeof(T) == 2) {
+        const float angle = (float)(int)(phase >> 32) * 1.4629180792671596e-9f /* 2 pi / 2^32 */;
+        return make_float2(__cosf(angle) * scale, __sinf(angle) * scale);
+    } else {
+        // the nearest quarter turn is taken off exactly, the rest (at most an eighth of a turn) is converted to FP32 with full
+        // relative accuracy
+        const unsigned quarter = (unsigned)((phase + (1ull << 61)) >> 62);
+        const long long rest = (long long)(phase - ((unsigned long long)quarter << 62));
+        float s, c;
+        sincospif((float)rest * 1.0842021724855044e-19f /* 2^-63: half turns */, &s, &c);
+        float cq = (quarter & 1) ? s : c, sq = (quarter & 1) ? c : s;
+        if (quarter == 1 || quarter == 2) cq = -cq;
+        if (quarter & 2) sq = -sq;
+        return make_float2(cq * scale, sq * scale);
+    }
 }
 
-template <class T>
+template <class T, int N>
+struct alignas(N * sizeof(T)) Pack {
+    T v[N];
+};
+
+// A unit is P pairs of one head (two pieces of P elements) or, behind the pairs, 2 P elements that are copied; a thread has
+// one unit of a token in every `slots`-th head, so that the sines, which cost more than the turning, are taken once for
+// several heads.  HBM-bound: 2 * heads * dim elements per token.
+template <class T, int P, bool INTERLEAVED>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p, const __grid_constant__ RotaryTable table)
 {
-    const int half = p.rot / 2, units = half + (p.dim - p.rot);
-    const long long total = p.tokens * p.heads * units;
-    const T *x = static_cast<const T *>(p.x);
-    T *y = static_cast<T *>(p.y);
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
-        const int u = (int)(i % units);
-        const long long t = (i / units) / p.heads;
-        const int h = (int)((i / units) % p.heads);
-        const T *xr = x + t * p.x_token + h * p.x_head;
-        T *yr = y + t * p.y_token + h * p.y_head;
-        if (u >= half) {
-            yr[u + half] = xr[u + half];
-            continue;
-        }
-        const int ia = p.layout ? 2 * u : u, ib = p.layout ? 2 * u + 1 : u + half;
-        const long long pos = p.positions[t];
-        const float a = load_f32(xr + ia), b = load_f32(xr + ib);
-        if (pos < 0) {
-            yr[ia] = xr[ia];
-            yr[ib] = xr[ib];
-            continue;
-        }
-        float2 cs = cos_sin((unsigned long long)pos * table.freq[u], p.scale);
-        if (p.backward) cs.y = -cs.y;
-        store_f32(yr + ia, a * cs.x - b * cs.y);
-        store_f32(yr + ib, a * cs.y + b * cs.x);
+    using Piece = Pack<T, P>;
+    const unsigned i = blockIdx.x * 256u + threadIdx.x;
+    const unsigned u = i % (unsigned)p.units, j = i / (unsigned)p.units;
+    const unsigned slot = j % (unsigned)p.slots, local = j / (unsigned)p.slots;
+    const long long t = (long long)blockIdx.y * p.per_slice + local;
+    if (local >= p.per_slice || t >= p.tokens) return;
+    const long long pos = p.positions[t];
+    const bool pairs = (int)u < p.turned;
+    // elements of the unit's two pieces
+    int first, second;
+    if (pairs) {
+        first = INTERLEAVED ? 2 * P * (int)u : P * (int)u;
+        second = INTERLEAVED ? first + P : first + p.rot / 2;
+    } else {
+        first = p.rot + 2 * P * ((int)u - p.turned);
+        second = first + P;
     }
+    const T *x = static_cast<const T *>(p.x) + t * p.x_token;
+    T *y = static_cast<T *>(p.y) + t * p.y_token;
+    if (!pairs || pos < 0) {
+        if (static_cast<const void *>(x) == static_cast<const void *>(y)) return;
+        for (int h = slot; h < p.heads; h += p.slots) {
+            const T *from = x + h * p.x_head;
+            T *to = y + h * p.y_head;
+            *reinterpret_cast<Piece *>(to + first) = *reinterpret_cast<const Piece *>(from + first);
+            if (pairs || second < p.dim) *reinterpret_cast<Piece *>(to + second) = *reinterpret_cast<const Piece *>(from + second);
+        }
+        return;
+    }
+    float2 cs[P];
+#pragma unroll
+    for (int k = 0; k < P; k++) {
+        cs[k] = cos_sin<T>((unsigned long long)pos * table.freq[u * P + k], p.scale);
+        if (p.backward) cs[k].y = -cs[k].y;
+    }
+#pragma unroll 2
+    for (int h = slot; h < p.heads; h += p.slots) {
+        const T *from = x + h * p.x_head;
+        T *to = y + h * p.y_head;
+        Piece one = *reinterpret_cast<const Piece *>(from + first), two = *reinterpret_cast<const Piece *>(from + second);
+#pragma unroll
+        for (int k = 0; k < P; k++) {
+            // pair k: (one[k], two[k]), or neighbours
+            T &ra = INTERLEAVED ? (2 * k < P ? one.v[(2 * k) % P] : two.v[(2 * k) % P]) : one.v[k];
+            T &rb = INTERLEAVED ? (2 * k + 1 < P ? one.v[(2 * k + 1) % P] : two.v[(2 * k + 1) % P]) : two.v[k];
+            const float a = load_f32(&ra), b = load_f32(&rb);
+            store_f32(&ra, a * cs[k].x - b * cs[k].y);
+            store_f32(&rb, a * cs[k].y + b * cs[k].x);
+        }
+        *reinterpret_cast<Piece *>(to + first) = one;
+        *reinterpret_cast<Piece *>(to + second) = two;
+    }
+}
+
+template <class T, int P>
+void launch_rotary(RotaryParams p, int layout, const RotaryTable &table, cudaStream_t st)
+{
+    p.turned = p.rot / 2 / P;
+    p.units = p.turned + (p.x == p.y ? 0 : (p.dim - p.rot + 2 * P - 1) / (2 * P));
+    if (p.units == 0) return;
+    // heads per thread: as many as still leave 1024 threads for each SM, at most 8
+    const double threads = (double)p.tokens * p.heads * p.units;
+    int each = (int)fmin(fmax(threads / (148.0 * 1024), 1.0), 8.0);
+    p.slots = (p.heads + each - 1) / each;
+    const unsigned long long row = (unsigned long long)p.slots * p.units;
+    unsigned long long slice = (1ull << 31) / row;
+    if (slice < 1) slice = 1;
+    if (slice > (unsigned long long)p.tokens) slice = (unsigned long long)p.tokens;
+    p.per_slice = (unsigned)slice;
+    const dim3 grid((unsigned)((slice * row + 255) / 256), (unsigned)((p.tokens + slice - 1) / slice));
+    if (layout == GEMM_ROTARY_INTERLEAVED) rotary_kernel<T, P, true><<<grid, 256, 0, st>>>(p, table);
+    else rotary_kernel<T, P, false><<<grid, 256, 0, st>>>(p, table);
+}
+
+// the widest pieces that every row, every head and both halves of the pairs are aligned to
+template <class T>
+void launch_rotary_wide(const RotaryParams &p, int layout, const RotaryTable &table, cudaStream_t st)
+{
+    const size_t bits = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.y) |
+                        (size_t)(p.x_token | p.x_head | p.y_token | p.y_head) * sizeof(T);
+    const int each = p.rot / 2 | (p.dim - p.rot);        // pairs, and elements behind them
+    auto fits = [&](int n) { return bits % (n * sizeof(T)) == 0 && each % n == 0; };
+    if constexpr (sizeof(T) == 2)
+        if (fits(8)) return launch_rotary<T, 8>(p, layout, table, st);
+    if (fits(4)) launch_rotary<T, 4>(p, layout, table, st);
+    else if (fits(2)) launch_rotary<T, 2>(p, layout, table, st);
+    else launch_rotary<T, 1>(p, layout, table, st);
 }
 
 // The frequency table of a set of parameters, kept per thread (the last few sets): a value of its key alone.
@@ -298,15 +377,13 @@ int gemm_rotary(const GemmRotaryArgs *a)
     p.positions = reinterpret_cast<const long long *>(a->positions);
     p.tokens = a->tokens;
     p.x_token = a->x_token_stride; p.x_head = a->x_head_stride; p.y_token = a->y_token_stride; p.y_head = a->y_head_stride;
-    p.heads = a->heads; p.dim = a->head_dim; p.rot = a->rot_dim; p.layout = a->layout; p.backward = a->backward != 0;
+    p.heads = a->heads; p.dim = a->head_dim; p.rot = a->rot_dim; p.backward = a->backward != 0;
     p.scale = a->scale;
-    const RotaryTable *table = rotary_table(key);
-    long long blocks = (a->tokens * a->heads * (a->rot_dim / 2 + a->head_dim - a->rot_dim) + 255) / 256;
-    if (blocks > 148 * 32) blocks = 148 * 32;
+    const RotaryTable &table = *rotary_table(key);
     cudaStream_t st = static_cast<cudaStream_t>(a->stream);
-    if (a->dtype == GEMM_X_BF16) rotary_kernel<__nv_bfloat16><<<(unsigned)blocks, 256, 0, st>>>(p, *table);
-    else if (a->dtype == GEMM_X_F16) rotary_kernel<__half><<<(unsigned)blocks, 256, 0, st>>>(p, *table);
-    else rotary_kernel<float><<<(unsigned)blocks, 256, 0, st>>>(p, *table);
+    if (a->dtype == GEMM_X_BF16) launch_rotary_wide<__nv_bfloat16>(p, a->layout, table, st);
+    else if (a->dtype == GEMM_X_F16) launch_rotary_wide<__half>(p, a->layout, table, st);
+    else launch_rotary_wide<float>(p, a->layout, table, st);
     return launched();
 }
 
