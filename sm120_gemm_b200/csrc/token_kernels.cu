@@ -34,6 +34,30 @@ int launched()
     return (int)e;
 }
 
+// The kernels here are launched as programmatic dependents: set up while the grid before is still running, and held here
+// until its results are there.
+__device__ __forceinline__ void after_the_grid_before()
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+template <class... P, class... A>
+void launch_dependent(void (*kernel)(P...), dim3 grid, unsigned threads, unsigned smem, cudaStream_t st, const A &...args)
+{
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kernel, args...);       // its error, if any, is cudaGetLastError's: launched() reports it
+}
+
 __device__ __forceinline__ float load_f32(const float *p) { return *p; }
 __device__ __forceinline__ float load_f32(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
 __device__ __forceinline__ float load_f32(const __half *p) { return __half2float(*p); }
@@ -100,6 +124,7 @@ template <class T, int P, bool INTERLEAVED>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p, const __grid_constant__ RotaryTable table)
 {
     using Piece = Pack<T, P>;
+    after_the_grid_before();
     const unsigned i = blockIdx.x * 256u + threadIdx.x;
     const unsigned u = i % (unsigned)p.units, j = i / (unsigned)p.units;
     const unsigned slot = j % (unsigned)p.slots, local = j / (unsigned)p.slots;
@@ -128,28 +153,44 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p, const
         }
         return;
     }
+    // the first heads are on their way while the sines are taken
+    constexpr int AT_ONCE = 2;
+    Piece one[AT_ONCE], two[AT_ONCE];
+    auto load = [&](int h) {
+#pragma unroll
+        for (int n = 0; n < AT_ONCE; n++)
+            if (h + n * p.slots < p.heads) {
+                const T *from = x + (h + n * p.slots) * p.x_head;
+                one[n] = *reinterpret_cast<const Piece *>(from + first);
+                two[n] = *reinterpret_cast<const Piece *>(from + second);
+            }
+    };
+    load(slot);
     float2 cs[P];
 #pragma unroll
     for (int k = 0; k < P; k++) {
         cs[k] = cos_sin<T>((unsigned long long)pos * table.freq[u * P + k], p.scale);
         if (p.backward) cs[k].y = -cs[k].y;
     }
-#pragma unroll 2
-    for (int h = slot; h < p.heads; h += p.slots) {
-        const T *from = x + h * p.x_head;
-        T *to = y + h * p.y_head;
-        Piece one = *reinterpret_cast<const Piece *>(from + first), two = *reinterpret_cast<const Piece *>(from + second);
+    for (int h = slot; h < p.heads;) {
 #pragma unroll
-        for (int k = 0; k < P; k++) {
-            // pair k: (one[k], two[k]), or neighbours
-            T &ra = INTERLEAVED ? (2 * k < P ? one.v[(2 * k) % P] : two.v[(2 * k) % P]) : one.v[k];
-            T &rb = INTERLEAVED ? (2 * k + 1 < P ? one.v[(2 * k + 1) % P] : two.v[(2 * k + 1) % P]) : two.v[k];
-            const float a = load_f32(&ra), b = load_f32(&rb);
-            store_f32(&ra, a * cs[k].x - b * cs[k].y);
-            store_f32(&rb, a * cs[k].y + b * cs[k].x);
-        }
-        *reinterpret_cast<Piece *>(to + first) = one;
-        *reinterpret_cast<Piece *>(to + second) = two;
+        for (int n = 0; n < AT_ONCE; n++)
+            if (h + n * p.slots < p.heads) {
+#pragma unroll
+                for (int k = 0; k < P; k++) {
+                    // pair k: (one[k], two[k]), or neighbours
+                    T &ra = INTERLEAVED ? (2 * k < P ? one[n].v[(2 * k) % P] : two[n].v[(2 * k) % P]) : one[n].v[k];
+                    T &rb = INTERLEAVED ? (2 * k + 1 < P ? one[n].v[(2 * k + 1) % P] : two[n].v[(2 * k + 1) % P]) : two[n].v[k];
+                    const float a = load_f32(&ra), b = load_f32(&rb);
+                    store_f32(&ra, a * cs[k].x - b * cs[k].y);
+                    store_f32(&rb, a * cs[k].y + b * cs[k].x);
+                }
+                T *to = y + (h + n * p.slots) * p.y_head;
+                *reinterpret_cast<Piece *>(to + first) = one[n];
+                *reinterpret_cast<Piece *>(to + second) = two[n];
+            }
+        h += AT_ONCE * p.slots;
+        load(h);
     }
 }
 
@@ -159,9 +200,9 @@ void launch_rotary(RotaryParams p, int layout, const RotaryTable &table, cudaStr
     p.turned = p.rot / 2 / P;
     p.units = p.turned + (p.x == p.y ? 0 : (p.dim - p.rot + 2 * P - 1) / (2 * P));
     if (p.units == 0) return;
-    // heads per thread: as many as still leave 1024 threads for each SM, at most 8
+    // heads per thread: as many as still leave 2048 threads for each SM, at most 10
     const double threads = (double)p.tokens * p.heads * p.units;
-    int each = (int)fmin(fmax(threads / (148.0 * 1024), 1.0), 8.0);
+    int each = (int)fmin(fmax(threads / (148.0 * 2048), 1.0), 10.0);
     p.slots = (p.heads + each - 1) / each;
     const unsigned long long row = (unsigned long long)p.slots * p.units;
     unsigned long long slice = (1ull << 31) / row;
@@ -169,8 +210,8 @@ void launch_rotary(RotaryParams p, int layout, const RotaryTable &table, cudaStr
     if (slice > (unsigned long long)p.tokens) slice = (unsigned long long)p.tokens;
     p.per_slice = (unsigned)slice;
     const dim3 grid((unsigned)((slice * row + 255) / 256), (unsigned)((p.tokens + slice - 1) / slice));
-    if (layout == GEMM_ROTARY_INTERLEAVED) rotary_kernel<T, P, true><<<grid, 256, 0, st>>>(p, table);
-    else rotary_kernel<T, P, false><<<grid, 256, 0, st>>>(p, table);
+    if (layout == GEMM_ROTARY_INTERLEAVED) launch_dependent(rotary_kernel<T, P, true>, grid, 256, 0, st, p, table);
+    else launch_dependent(rotary_kernel<T, P, false>, grid, 256, 0, st, p, table);
 }
 
 // the widest pieces that every row, every head and both halves of the pairs are aligned to
