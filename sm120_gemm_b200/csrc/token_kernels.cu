@@ -286,94 +286,224 @@ struct LogitsParams {
     const int *bias_begin;
     const unsigned *mask;
     int rows, vocab;
+    int slices;                  // of a row
 };
 
-constexpr int LOGITS_SLICE = 4096;
+// A row is cut into groups of 8 values and slices of SLICE = 256 * 8 * G of them; a CTA takes a slice, a cluster of C CTAs
+// neighbouring ones.  The tokens of the history are counted in shared memory (integer atomics: the order does not matter):
+// with C = 1 every CTA goes through the whole history and keeps what is in its slice, with C = 8 every CTA goes through an
+// eighth and counts in the shared memory of the CTA that has the token.  HBM-bound on long rows: x once, y once.
 constexpr unsigned NO_BIAS = 0xffffffffu;
+constexpr unsigned SEEN = 0x80000000u;           // in the prompt; below it: how often generated
 
-template <class TX, class TY>
-__global__ void __launch_bounds__(256) logits_kernel(const LogitsParams p)
+template <class T>
+struct Eight {                                   // 8 values as they lie in memory, 16-byte accesses
+    uint4 raw[sizeof(T) / 2];
+};
+template <class T>
+__device__ __forceinline__ void load_eight(Eight<T> &e, const T *p, bool whole, int first, int last)
 {
-    __shared__ unsigned count[LOGITS_SLICE];     // generated occurrences; top bit: occurs at all
-    __shared__ unsigned bias[LOGITS_SLICE];      // float bits, NO_BIAS = none listed
-    __shared__ int doubled;
-    for (int row = blockIdx.y; row < p.rows; row += gridDim.y) {
-        const int v0 = blockIdx.x * LOGITS_SLICE;
-        const int n = min(LOGITS_SLICE, p.vocab - v0);
-        for (int i = threadIdx.x; i < n; i += blockDim.x) { count[i] = 0; bias[i] = NO_BIAS; }
-        if (threadIdx.x == 0) doubled = 0;
-        __syncthreads();
-        if (p.history) {
-            const int len = (int)min((long long)max(p.history_len[row], 0), p.history_ld);
-            const int prompt = p.prompt_len ? p.prompt_len[row] : 0;
-            const int *h = p.history + row * p.history_ld;
-            for (int i = threadIdx.x; i < len; i += blockDim.x) {
-                const unsigned at = (unsigned)h[i] - (unsigned)v0;
-                if (h[i] < 0 || at >= (unsigned)n) continue;
-                if (i < prompt) atomicOr(&count[at], 0x80000000u);
-                else { atomicOr(&count[at], 0x80000000u); atomicAdd(&count[at], 1u); }
-            }
-        }
-        int b0 = 0, b1 = 0;
-        if (p.bias_begin) {
-            b0 = max(p.bias_begin[row], 0);
-            b1 = p.bias_begin[row + 1];
-            for (int e = b0 + threadIdx.x; e < b1; e += blockDim.x) {
-                const int id = p.bias_ids[e];
-                const unsigned at = (unsigned)id - (unsigned)v0;
-                if (id < 0 || at >= (unsigned)n) continue;
-                if (atomicExch(&bias[at], __float_as_uint(p.bias_values[e])) != NO_BIAS) doubled = 1;
-            }
-        }
-        __syncthreads();
-        if (doubled) {
-            // an id listed more than once: its values are added in the order of the list, by the first entry's thread
-            for (int e = b0 + threadIdx.x; e < b1; e += blockDim.x) {
-                const int id = p.bias_ids[e];
-                const unsigned at = (unsigned)id - (unsigned)v0;
-                if (id < 0 || at >= (unsigned)n) continue;
-                bool first = true;
-                for (int d = b0; d < e && first; d++) first = p.bias_ids[d] != id;
-                if (!first) continue;
-                float sum = p.bias_values[e];
-                for (int d = e + 1; d < b1; d++)
-                    if (p.bias_ids[d] == id) sum += p.bias_values[d];
-                bias[at] = __float_as_uint(sum);
-            }
-            __syncthreads();
-        }
-        const float rep = p.repetition ? p.repetition[row] : 1.f, pres = p.presence ? p.presence[row] : 0.f, freq = p.frequency ? p.frequency[row] : 0.f;
-        const TX *x = static_cast<const TX *>(p.x) + row * p.x_ld + v0;
-        TY *y = static_cast<TY *>(p.y) + row * p.y_ld + v0;
-        for (int i = threadIdx.x; i < n; i += blockDim.x) {
-            float v = load_f32(x + i);
-            const unsigned c = count[i];
-            if (c) {
-                v = v > 0.f ? v / rep : v * rep;
-                const unsigned k = c & 0x7fffffffu;
-                if (k) v -= freq * (float)k + pres;
-            }
-            if (bias[i] != NO_BIAS) v += __uint_as_float(bias[i]);
-            if (p.mask && !((p.mask[row * p.mask_ld + (v0 + i) / 32] >> ((v0 + i) % 32)) & 1u)) v = -INFINITY;
-            store_f32(y + i, v);
-        }
-        __syncthreads();
+    if (whole) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) e.raw[i] = reinterpret_cast<const uint4 *>(p)[i];
+    } else {
+        T *v = reinterpret_cast<T *>(e.raw);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i >= first && i < last) v[i] = p[i];
     }
 }
 
-template <class TX, class TY>
-void launch_logits(const LogitsParams &p, cudaStream_t st)
+template <class TX, class TY, int G, int C>
+__global__ void __launch_bounds__(256) logits_kernel(const LogitsParams p)
 {
-    const dim3 grid((p.vocab + LOGITS_SLICE - 1) / LOGITS_SLICE, p.rows < 65535 ? p.rows : 65535);
-    logits_kernel<TX, TY><<<grid, 256, 0, st>>>(p);
+    constexpr int SLICE = 256 * 8 * G;
+    extern __shared__ __align__(16) unsigned count[];      // [SLICE], then, with biases, [SLICE] of their bits
+    unsigned *bias = count + SLICE;
+    __shared__ int doubled;
+    after_the_grid_before();
+    const int row = blockIdx.x / p.slices, slice = blockIdx.x % p.slices;
+    const TX *x = static_cast<const TX *>(p.x) + (long long)row * p.x_ld;
+    TY *y = static_cast<TY *>(p.y) + (long long)row * p.y_ld;
+    // groups start where x and, if there is such a place, y too are 16-byte aligned: at v = shift - 8, shift, ...
+    constexpr int NX = 16 / sizeof(TX), NY = 16 / sizeof(TY);
+    const int ox = (int)(reinterpret_cast<uintptr_t>(x) / sizeof(TX)), oy = (int)(reinterpret_cast<uintptr_t>(y) / sizeof(TY));
+    int shift = (8 - (ox & (NX - 1))) & (NX - 1);
+    if (NX == 4 && ((oy + shift) & (NY - 1)) != 0 && ((oy + shift + 4) & (NY - 1)) == 0) shift += 4;
+    const bool wide_y = ((oy + shift) & (NY - 1)) == 0;
+    const int first = shift - 8 + slice * SLICE;           // token of count[0]; below 0 in the first slice of a row
+    Eight<TX> in[G];
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        const int v = first + (g * 256 + (int)threadIdx.x) * 8;
+        if (v < p.vocab && v + 8 > 0) load_eight(in[g], x + v, v >= 0 && v + 8 <= p.vocab, -v, p.vocab - v);
+    }
+    const bool biased = p.bias_begin != nullptr;
+    for (int i = threadIdx.x; i < SLICE / 4; i += 256) {
+        reinterpret_cast<uint4 *>(count)[i] = make_uint4(0, 0, 0, 0);
+        if (biased) reinterpret_cast<uint4 *>(bias)[i] = make_uint4(NO_BIAS, NO_BIAS, NO_BIAS, NO_BIAS);
+    }
+    if (threadIdx.x == 0) doubled = 0;
+    auto all_here = [] {
+        if (C == 1) __syncthreads();
+        else asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+    };
+    if (p.history) all_here();
+    else __syncthreads();
+    if (p.history) {
+        const unsigned rank = C == 1 ? 0 : slice % C;
+        const int window = first - (int)rank * SLICE;      // token of the cluster's first count
+        const int len = (int)min((long long)max(p.history_len[row], 0), p.history_ld), prompt = p.prompt_len ? p.prompt_len[row] : 0;
+        const int *h = p.history + (long long)row * p.history_ld;
+        auto tally = [&](int id, int i) {
+            const unsigned at = (unsigned)(id - window);
+            if (id < 0 || id >= p.vocab || at >= (unsigned)(C * SLICE)) return;
+            if constexpr (C == 1) {
+                if (i < prompt) atomicOr(&count[at], SEEN);
+                else atomicAdd(&count[at], 1u);
+            } else {
+                unsigned to;
+                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"((unsigned)__cvta_generic_to_shared(&count[at % SLICE])), "r"(at / SLICE));
+                if (i < prompt) asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(to), "r"(SEEN) : "memory");
+                else asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(to), "r"(1u) : "memory");
+            }
+        };
+        const int lone = min(len, (int)((16 - (reinterpret_cast<uintptr_t>(h) & 15)) & 15) / 4), fours = (len - lone) / 4;       // 16-byte pieces
+        const int me = rank * 256 + threadIdx.x;
+        if (me < lone) tally(h[me], me);
+        for (int q = me; q < fours; q += C * 256) {
+            const int4 id = __ldg(reinterpret_cast<const int4 *>(h + lone) + q);
+            const int i = lone + 4 * q;
+            tally(id.x, i);
+            tally(id.y, i + 1);
+            tally(id.z, i + 2);
+            tally(id.w, i + 3);
+        }
+        const int rest = lone + 4 * fours + me;
+        if (rest < len) tally(h[rest], rest);
+    }
+    int b0 = 0, b1 = 0;
+    if (biased) {
+        b0 = max(p.bias_begin[row], 0);
+        b1 = p.bias_begin[row + 1];
+        for (int e = b0 + threadIdx.x; e < b1; e += 256) {
+            const int id = p.bias_ids[e];
+            const unsigned at = (unsigned)(id - first);
+            if (id < 0 || id >= p.vocab || at >= (unsigned)SLICE) continue;
+            if (atomicExch(&bias[at], __float_as_uint(p.bias_values[e])) != NO_BIAS) doubled = 1;
+        }
+    }
+    if (p.history) all_here();
+    else __syncthreads();
+    if (biased && doubled) {
+        // an id listed more than once: its values are added in the order of the list, by the first entry's thread
+        for (int e = b0 + threadIdx.x; e < b1; e += 256) {
+            const int id = p.bias_ids[e];
+            const unsigned at = (unsigned)(id - first);
+            if (id < 0 || id >= p.vocab || at >= (unsigned)SLICE) continue;
+            bool again = false;
+            for (int d = b0; d < e && !again; d++) again = p.bias_ids[d] == id;
+            if (again) continue;
+            float sum = p.bias_values[e];
+            for (int d = e + 1; d < b1; d++)
+                if (p.bias_ids[d] == id) sum += p.bias_values[d];
+            bias[at] = __float_as_uint(sum);
+        }
+        __syncthreads();
+    }
+    const float rep = p.repetition ? p.repetition[row] : 1.f, pres = p.presence ? p.presence[row] : 0.f, freq = p.frequency ? p.frequency[row] : 0.f;
+    const unsigned *mask = p.mask ? p.mask + (long long)row * p.mask_ld : nullptr;
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        const int at = (g * 256 + (int)threadIdx.x) * 8, v = first + at;
+        if (v >= p.vocab || v + 8 <= 0) continue;
+        const int from = max(-v, 0), to = min(p.vocab - v, 8);
+        unsigned allowed = 0xffu;
+        if (mask) {
+            // bits v .. v + 7, of at most two words; those in front of the row and behind it do not matter
+            const int w0 = max(v, 0) >> 5, w1 = (v + to - 1) >> 5;
+            const unsigned long long bits = (unsigned long long)__ldg(mask + w1) << 32 | __ldg(mask + w0);
+            allowed = v < 0 ? (unsigned)bits << -v : (unsigned)((w1 == w0 ? bits & 0xffffffffull : bits) >> (v & 31));
+        }
+        Eight<TY> out;
+        TY *o = reinterpret_cast<TY *>(out.raw);
+        const TX *i = reinterpret_cast<const TX *>(in[g].raw);
+#pragma unroll
+        for (int k = 0; k < 8; k += 4) {
+            const uint4 c4 = *reinterpret_cast<const uint4 *>(count + at + k);
+            uint4 b4 = make_uint4(NO_BIAS, NO_BIAS, NO_BIAS, NO_BIAS);
+            if (biased) b4 = *reinterpret_cast<const uint4 *>(bias + at + k);
+            const unsigned c[4] = {c4.x, c4.y, c4.z, c4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                float l = load_f32(i + k + j);
+                if (c[j]) {
+                    l = l > 0.f ? l / rep : l * rep;
+                    const unsigned n = c[j] & ~SEEN;
+                    if (n) l -= freq * (float)n + pres;
+                }
+                if (b[j] != NO_BIAS) l += __uint_as_float(b[j]);
+                if (!(allowed >> (k + j) & 1u)) l = -INFINITY;
+                store_f32(o + k + j, l);
+            }
+        }
+        if (wide_y && from == 0 && to == 8) {
+#pragma unroll
+            for (int q = 0; q < (int)sizeof(TY) / 2; q++) reinterpret_cast<uint4 *>(y + v)[q] = out.raw[q];
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (k >= from && k < to) y[v + k] = o[k];
+        }
+    }
+}
+
+template <class TX, class TY, int G, int C>
+int launch_logits(LogitsParams p, cudaStream_t st)
+{
+    constexpr int SLICE = 256 * 8 * G;
+    p.slices = ((p.vocab + 8 + SLICE - 1) / SLICE + C - 1) / C * C;        // (the groups may start up to 8 in front of the row)
+    const long long ctas = (long long)p.slices * p.rows;
+    if (ctas > 0x7fffffffll) return refuse("%d rows of %d are too many for one call", p.rows, p.vocab);
+    auto *kernel = logits_kernel<TX, TY, G, C>;
+    const unsigned smem = SLICE * 4 * (p.bias_begin ? 2 : 1);
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return refuse("cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    }
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = C;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = C == 1 ? 1 : 2;
+    cudaLaunchKernelEx(&cfg, kernel, p);
+    return launched();
+}
+
+template <class TX, class TY>
+int launch_logits_sized(const LogitsParams &p, cudaStream_t st)
+{
+    // Slices of 8192 where that still gives every SM several, of 2048 for few rows; clusters where the history, read by every
+    // slice of a row, would be more than a slice's own values.
+    const bool large = (long long)p.rows * p.vocab >= 148ll * 3 * 8192;
+    if (p.history && p.history_ld > 8192) return large ? launch_logits<TX, TY, 4, 8>(p, st) : launch_logits<TX, TY, 1, 8>(p, st);
+    return large ? launch_logits<TX, TY, 4, 1>(p, st) : launch_logits<TX, TY, 1, 1>(p, st);
 }
 
 template <class TX>
-void launch_logits_to(const LogitsParams &p, int y_dtype, cudaStream_t st)
+int launch_logits_to(const LogitsParams &p, int y_dtype, cudaStream_t st)
 {
-    if (y_dtype == GEMM_X_BF16) launch_logits<TX, __nv_bfloat16>(p, st);
-    else if (y_dtype == GEMM_X_F16) launch_logits<TX, __half>(p, st);
-    else launch_logits<TX, float>(p, st);
+    if (y_dtype == GEMM_X_BF16) return launch_logits_sized<TX, __nv_bfloat16>(p, st);
+    if (y_dtype == GEMM_X_F16) return launch_logits_sized<TX, __half>(p, st);
+    return launch_logits_sized<TX, float>(p, st);
 }
 
 bool aligned(const void *p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
@@ -453,9 +583,8 @@ int gemm_logits(const GemmLogitsArgs *a)
     p.mask = a->mask; p.mask_ld = a->mask_ld;
     p.rows = a->rows; p.vocab = a->vocab;
     cudaStream_t st = static_cast<cudaStream_t>(a->stream);
-    if (a->x_dtype == GEMM_X_BF16) launch_logits_to<__nv_bfloat16>(p, a->y_dtype, st);
-    else if (a->x_dtype == GEMM_X_F16) launch_logits_to<__half>(p, a->y_dtype, st);
-    else launch_logits_to<float>(p, a->y_dtype, st);
-    return launched();
+    if (a->x_dtype == GEMM_X_BF16) return launch_logits_to<__nv_bfloat16>(p, a->y_dtype, st);
+    if (a->x_dtype == GEMM_X_F16) return launch_logits_to<__half>(p, a->y_dtype, st);
+    return launch_logits_to<float>(p, a->y_dtype, st);
 }
 }
