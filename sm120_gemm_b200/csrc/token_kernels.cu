@@ -11,6 +11,8 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <atomic>
+
 #include "../../include/sm100_gemm.h"
 #include "../../include/sm100_gemm_util.h"
 
@@ -26,6 +28,8 @@ int refuse(const char *fmt, ...)
     va_end(ap);
     return (int)cudaErrorInvalidValue;
 }
+
+bool aligned(const void *p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
 int launched()
 {
@@ -56,6 +60,31 @@ void launch_dependent(void (*kernel)(P...), dim3 grid, unsigned threads, unsigne
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     cudaLaunchKernelEx(&cfg, kernel, args...);       // its error, if any, is cudaGetLastError's: launched() reports it
+}
+
+// more shared memory than a kernel gets unasked (48 KB), once per kernel and device
+template <class... P>
+int ask_for_shared(void (*kernel)(P...), int bytes)
+{
+    static std::atomic<const void *> asked[32][64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev < 0 || dev >= 32)) return refuse("device ordinal %d out of range", dev);
+    const void *me = reinterpret_cast<const void *>(kernel);
+    if (e == cudaSuccess) {
+        for (auto &a : asked[dev])
+            if (a.load(std::memory_order_acquire) == me) return 0;
+        if (bytes > 0) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        if (e == cudaSuccess)
+            for (auto &a : asked[dev]) {
+                const void *none = nullptr;
+                if (a.compare_exchange_strong(none, me, std::memory_order_acq_rel) || none == me) return 0;
+            }
+        if (e == cudaSuccess) return 0;      // (no place left to remember it)
+    }
+    snprintf(g_message, sizeof(g_message), "cudaFuncSetAttribute failed: %s", cudaGetErrorString(e));
+    return (int)e;
 }
 
 __device__ __forceinline__ float load_f32(const float *p) { return *p; }
@@ -289,12 +318,21 @@ struct LogitsParams {
     int slices;                  // of a row
 };
 
-// A row is cut into groups of 8 values and slices of SLICE = 256 * 8 * G of them; a CTA takes a slice, a cluster of C CTAs
-// neighbouring ones.  The tokens of the history are counted in shared memory (integer atomics: the order does not matter):
-// with C = 1 every CTA goes through the whole history and keeps what is in its slice, with C = 8 every CTA goes through an
-// eighth and counts in the shared memory of the CTA that has the token.  HBM-bound on long rows: x once, y once.
+// Two ways, by size:
+//   one kernel   few values and a short history: a CTA takes a slice of a row (SLICE values), goes through the row's whole
+//                history, counts what is in its slice in shared memory and writes the slice once.  One launch, 3.9 us at
+//                1 x 32001.
+//   two kernels  else: the first streams x to y under the mask at the memory's rate; the second, a programmatic dependent that
+//                counts beside it and then waits for it, rewrites the few tokens that were said or have a bias.  Counting in
+//                the streaming kernel held every slice up for the history's round trips: 64 x 131072 with 4096 said took
+//                29 us whatever the slices' size.
+// The tokens that need arithmetic (a division among it) are listed, so that whole warps do it, not every warp for the one lane
+// in thirty that has such a token.  Counting is by integer atomics in shared memory: the order does not matter.
 constexpr unsigned NO_BIAS = 0xffffffffu;
-constexpr unsigned SEEN = 0x80000000u;           // in the prompt; below it: how often generated
+// a token's count word: in the prompt; has a bias, several (second kernel); below them how often it was generated
+constexpr unsigned SEEN = 0x80000000u, BIASED = 0x40000000u, BIASED_AGAIN = 0x20000000u, GENERATED = 0x1fffffffu;
+constexpr unsigned SEVERAL = 0xfffffffeu;        // first kernel: in the place of bias bits
+__device__ __forceinline__ unsigned bias_bits(float v) { return v == v ? __float_as_uint(v) : 0x7fc00000u; }      // never one of the marks
 
 template <class T>
 struct Eight {                                   // 8 values as they lie in memory, 16-byte accesses
@@ -314,188 +352,433 @@ __device__ __forceinline__ void load_eight(Eight<T> &e, const T *p, bool whole, 
     }
 }
 
-template <class TX, class TY, int G, int C>
-__global__ void __launch_bounds__(256) logits_kernel(const LogitsParams p)
+template <class T>
+__device__ __forceinline__ void store_eight(const Eight<T> &e, T *p, bool wide, int from, int to)
 {
-    constexpr int SLICE = 256 * 8 * G;
-    extern __shared__ __align__(16) unsigned count[];      // [SLICE], then, with biases, [SLICE] of their bits
-    unsigned *bias = count + SLICE;
-    __shared__ int doubled;
+    if (wide && from == 0 && to == 8) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) reinterpret_cast<uint4 *>(p)[i] = e.raw[i];
+    } else {
+        const T *v = reinterpret_cast<const T *>(e.raw);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i >= from && i < to) p[i] = v[i];
+    }
+}
+// Where the groups of 8 of a row start: where x and, if there is such a place, y too are 16-byte aligned.
+template <class TX, class TY>
+struct RowGroups {
+    int first;          // token of the first group's first value; below 0 where a part of a group is in front of the boundary
+    bool wide_y;        // y is aligned there
+    __device__ __forceinline__ RowGroups(const TX *x, const TY *y)
+    {
+        constexpr int NX = 16 / sizeof(TX), NY = 16 / sizeof(TY);
+        const int ox = (int)(reinterpret_cast<uintptr_t>(x) / sizeof(TX)), oy = (int)(reinterpret_cast<uintptr_t>(y) / sizeof(TY));
+        int shift = (8 - (ox & (NX - 1))) & (NX - 1);
+        if (NX == 4 && ((oy + shift) & (NY - 1)) != 0 && ((oy + shift + 4) & (NY - 1)) == 0) shift += 4;
+        wide_y = ((oy + shift) & (NY - 1)) == 0;
+        first = shift ? shift - 8 : 0;
+    }
+};
+
+// a token that was said (c: count word) or has a bias (its bits)
+__device__ __forceinline__ float adjust(float l, unsigned c, unsigned b, float rep, float pres, float freq)
+{
+    if (c & (SEEN | GENERATED)) {
+        l = l > 0.f ? l / rep : l * rep;
+        const unsigned n = c & GENERATED;
+        if (n) l -= freq * (float)n + pres;
+    }
+    return b != NO_BIAS ? l + __uint_as_float(b) : l;
+}
+
+// An id that is listed more than once: its values are added in the order of the list, by the thread of the first entry (true).
+__device__ __forceinline__ bool sum_of_biases(const LogitsParams &p, int b0, int b1, int e, int id, float &sum)
+{
+    bool first = true;
+    sum = 0.f;
+#pragma unroll 8
+    for (int d = b0; d < b1; d++) {
+        const bool same = p.bias_ids[d] == id;
+        first = first && !(same && d < e);
+        if (same) sum = d == e ? p.bias_values[d] : sum + p.bias_values[d];
+    }
+    return first;
+}
+
+template <class TX, class TY, int THREADS, int G>
+__global__ void __launch_bounds__(THREADS, 1536 / THREADS) logits_kernel(const LogitsParams p)
+{
+    constexpr int SLICE = THREADS * 8 * G;
+    extern __shared__ __align__(16) unsigned count[];      // [SLICE]; [SLICE] 16-bit places of the list; with biases [SLICE] of their bits
+    uint16_t *list = reinterpret_cast<uint16_t *>(count + SLICE);
+    unsigned *bias = count + SLICE + SLICE / 2;
+    __shared__ int doubled, listed;
     after_the_grid_before();
     const int row = blockIdx.x / p.slices, slice = blockIdx.x % p.slices;
+    // what the row's parts start with is asked for first: each is the address of the next load
+    const int said = p.history ? p.history_len[row] : 0, prompt = p.history && p.prompt_len ? p.prompt_len[row] : 0;
+    const bool biased = p.bias_begin != nullptr;
+    const int bias_from = biased ? p.bias_begin[row] : 0, b1 = biased ? p.bias_begin[row + 1] : 0;
+    const float rep = p.repetition ? p.repetition[row] : 1.f, pres = p.presence ? p.presence[row] : 0.f, freq = p.frequency ? p.frequency[row] : 0.f;
     const TX *x = static_cast<const TX *>(p.x) + (long long)row * p.x_ld;
     TY *y = static_cast<TY *>(p.y) + (long long)row * p.y_ld;
-    // groups start where x and, if there is such a place, y too are 16-byte aligned: at v = shift - 8, shift, ...
-    constexpr int NX = 16 / sizeof(TX), NY = 16 / sizeof(TY);
-    const int ox = (int)(reinterpret_cast<uintptr_t>(x) / sizeof(TX)), oy = (int)(reinterpret_cast<uintptr_t>(y) / sizeof(TY));
-    int shift = (8 - (ox & (NX - 1))) & (NX - 1);
-    if (NX == 4 && ((oy + shift) & (NY - 1)) != 0 && ((oy + shift + 4) & (NY - 1)) == 0) shift += 4;
-    const bool wide_y = ((oy + shift) & (NY - 1)) == 0;
-    const int first = shift - 8 + slice * SLICE;           // token of count[0]; below 0 in the first slice of a row
+    const RowGroups<TX, TY> groups(x, y);
+    const bool wide_y = groups.wide_y;
+    const int first = groups.first + slice * SLICE;        // token of count[0]; below 0 in the first slice of some rows
+    if (first >= p.vocab) return;
     Eight<TX> in[G];
 #pragma unroll
     for (int g = 0; g < G; g++) {
-        const int v = first + (g * 256 + (int)threadIdx.x) * 8;
+        const int v = first + (g * THREADS + (int)threadIdx.x) * 8;
         if (v < p.vocab && v + 8 > 0) load_eight(in[g], x + v, v >= 0 && v + 8 <= p.vocab, -v, p.vocab - v);
     }
-    const bool biased = p.bias_begin != nullptr;
-    for (int i = threadIdx.x; i < SLICE / 4; i += 256) {
+    // mask words of the groups, and the first ids of the history (those behind its end do not count later)
+    const unsigned *mask = p.mask ? p.mask + (long long)row * p.mask_ld : nullptr;
+    unsigned words[G][2];
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        const int v = first + (g * THREADS + (int)threadIdx.x) * 8, end = min(v + 8, p.vocab);
+        words[g][0] = words[g][1] = 0xffffffffu;
+        if (mask && v < p.vocab && v + 8 > 0) {          // bits v .. v + 7 are in at most two words
+            words[g][0] = __ldg(mask + (max(v, 0) >> 5));
+            words[g][1] = __ldg(mask + ((end - 1) >> 5));
+        }
+    }
+    const int *h = p.history + (long long)row * p.history_ld;
+    const int lone = (int)min(p.history_ld, (long long)(((16 - (reinterpret_cast<uintptr_t>(h) & 15)) & 15) / 4));        // in front of the 16-byte pieces
+    constexpr int AT_ONCE = 2;
+    int4 ids[AT_ONCE];
+    auto load_ids = [&](int q, long long pieces) {
+#pragma unroll
+        for (int n = 0; n < AT_ONCE; n++)
+            if (q + n * THREADS < pieces) ids[n] = __ldg(reinterpret_cast<const int4 *>(h + lone) + q + n * THREADS);
+    };
+    if (p.history) load_ids(threadIdx.x, (p.history_ld - lone) / 4);
+    for (int i = threadIdx.x; i < SLICE / 4; i += THREADS) {
         reinterpret_cast<uint4 *>(count)[i] = make_uint4(0, 0, 0, 0);
         if (biased) reinterpret_cast<uint4 *>(bias)[i] = make_uint4(NO_BIAS, NO_BIAS, NO_BIAS, NO_BIAS);
     }
-    if (threadIdx.x == 0) doubled = 0;
-    auto all_here = [] {
-        if (C == 1) __syncthreads();
-        else asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-    };
-    if (p.history) all_here();
-    else __syncthreads();
+    if (threadIdx.x == 0) doubled = listed = 0;
+    __syncthreads();
+    // the slice's tokens are start .. start + tokens - 1, the first of them at count[lead]
+    const int start = max(first, 0), lead = start - first;
+    const unsigned tokens = min((long long)first + SLICE, (long long)p.vocab) - start;
+    const int b0 = max(bias_from, 0);
+    int bias_id = -1;
+    float bias_value = 0.f;
+    if (b0 + (int)threadIdx.x < b1) {
+        bias_id = p.bias_ids[b0 + threadIdx.x];
+        bias_value = p.bias_values[b0 + threadIdx.x];
+    }
     if (p.history) {
-        const unsigned rank = C == 1 ? 0 : slice % C;
-        const int window = first - (int)rank * SLICE;      // token of the cluster's first count
-        const int len = (int)min((long long)max(p.history_len[row], 0), p.history_ld), prompt = p.prompt_len ? p.prompt_len[row] : 0;
-        const int *h = p.history + (long long)row * p.history_ld;
-        auto tally = [&](int id, int i) {
-            const unsigned at = (unsigned)(id - window);
-            if (id < 0 || id >= p.vocab || at >= (unsigned)(C * SLICE)) return;
-            if constexpr (C == 1) {
-                if (i < prompt) atomicOr(&count[at], SEEN);
-                else atomicAdd(&count[at], 1u);
-            } else {
-                unsigned to;
-                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"((unsigned)__cvta_generic_to_shared(&count[at % SLICE])), "r"(at / SLICE));
-                if (i < prompt) asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(to), "r"(SEEN) : "memory");
-                else asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(to), "r"(1u) : "memory");
-            }
+        const int len = (int)min((long long)max(said, 0), p.history_ld), me = threadIdx.x;
+        auto seen = [&](int id) {
+            const unsigned at = (unsigned)id - (unsigned)start;
+            if (at < tokens) atomicOr(&count[lead + at], SEEN);
         };
-        const int lone = min(len, (int)((16 - (reinterpret_cast<uintptr_t>(h) & 15)) & 15) / 4), fours = (len - lone) / 4;       // 16-byte pieces
-        const int me = rank * 256 + threadIdx.x;
+        auto generated = [&](int id) {
+            const unsigned at = (unsigned)id - (unsigned)start;
+            if (at < tokens) atomicAdd(&count[lead + at], 1u);
+        };
+        auto tally = [&](int id, int i) {
+            if (i < min(prompt, len)) seen(id);
+            else if (i < len) generated(id);
+        };
         if (me < lone) tally(h[me], me);
-        for (int q = me; q < fours; q += C * 256) {
-            const int4 id = __ldg(reinterpret_cast<const int4 *>(h + lone) + q);
-            const int i = lone + 4 * q;
-            tally(id.x, i);
-            tally(id.y, i + 1);
-            tally(id.z, i + 2);
-            tally(id.w, i + 3);
+        const int pieces = (int)((p.history_ld - lone) / 4);
+        for (int q = me; lone + 4 * q < len; q += AT_ONCE * THREADS) {
+            if (q != me) load_ids(q, pieces);
+#pragma unroll
+            for (int n = 0; n < AT_ONCE; n++) {
+                const int i = lone + 4 * (q + n * THREADS);
+                if (q + n * THREADS >= pieces || i >= len) break;
+                if (i >= prompt && i + 3 < len) {
+                    generated(ids[n].x);
+                    generated(ids[n].y);
+                    generated(ids[n].z);
+                    generated(ids[n].w);
+                } else if (i + 3 < prompt && i + 3 < len) {
+                    seen(ids[n].x);
+                    seen(ids[n].y);
+                    seen(ids[n].z);
+                    seen(ids[n].w);
+                } else {
+                    tally(ids[n].x, i);
+                    tally(ids[n].y, i + 1);
+                    tally(ids[n].z, i + 2);
+                    tally(ids[n].w, i + 3);
+                }
+            }
         }
-        const int rest = lone + 4 * fours + me;
+        const int rest = lone + 4 * pieces + me;         // the row's last ids behind the pieces
         if (rest < len) tally(h[rest], rest);
     }
-    int b0 = 0, b1 = 0;
-    if (biased) {
-        b0 = max(p.bias_begin[row], 0);
-        b1 = p.bias_begin[row + 1];
-        for (int e = b0 + threadIdx.x; e < b1; e += 256) {
-            const int id = p.bias_ids[e];
-            const unsigned at = (unsigned)(id - first);
-            if (id < 0 || id >= p.vocab || at >= (unsigned)SLICE) continue;
-            if (atomicExch(&bias[at], __float_as_uint(p.bias_values[e])) != NO_BIAS) doubled = 1;
+    auto biased_here = [&](int id, unsigned &at) {
+        at = (unsigned)id - (unsigned)start;
+        const bool here = at < tokens;
+        at += lead;
+        return here;
+    };
+    unsigned at_bias;
+    for (int e = b0 + threadIdx.x; e < b1; e += THREADS) {
+        if (e != b0 + (int)threadIdx.x) {
+            bias_id = p.bias_ids[e];
+            bias_value = p.bias_values[e];
+        }
+        if (biased_here(bias_id, at_bias) && atomicExch(&bias[at_bias], bias_bits(bias_value)) != NO_BIAS) {
+            atomicExch(&bias[at_bias], SEVERAL);          // after the last of them, whichever it is
+            doubled = 1;
         }
     }
-    if (p.history) all_here();
-    else __syncthreads();
+    __syncthreads();
     if (biased && doubled) {
-        // an id listed more than once: its values are added in the order of the list, by the first entry's thread
-        for (int e = b0 + threadIdx.x; e < b1; e += 256) {
+        for (int e = b0 + threadIdx.x; e < b1; e += THREADS) {
             const int id = p.bias_ids[e];
-            const unsigned at = (unsigned)(id - first);
-            if (id < 0 || id >= p.vocab || at >= (unsigned)SLICE) continue;
-            bool again = false;
-            for (int d = b0; d < e && !again; d++) again = p.bias_ids[d] == id;
-            if (again) continue;
-            float sum = p.bias_values[e];
-            for (int d = e + 1; d < b1; d++)
-                if (p.bias_ids[d] == id) sum += p.bias_values[d];
-            bias[at] = __float_as_uint(sum);
+            float sum;
+            if (biased_here(id, at_bias) && bias[at_bias] == SEVERAL && sum_of_biases(p, b0, b1, e, id, sum)) bias[at_bias] = bias_bits(sum);
         }
         __syncthreads();
     }
-    const float rep = p.repetition ? p.repetition[row] : 1.f, pres = p.presence ? p.presence[row] : 0.f, freq = p.frequency ? p.frequency[row] : 0.f;
-    const unsigned *mask = p.mask ? p.mask + (long long)row * p.mask_ld : nullptr;
+    // the tokens of this thread's groups that have something to be done
+    unsigned marked[G];
 #pragma unroll
     for (int g = 0; g < G; g++) {
-        const int at = (g * 256 + (int)threadIdx.x) * 8, v = first + at;
-        if (v >= p.vocab || v + 8 <= 0) continue;
-        const int from = max(-v, 0), to = min(p.vocab - v, 8);
-        unsigned allowed = 0xffu;
-        if (mask) {
-            // bits v .. v + 7, of at most two words; those in front of the row and behind it do not matter
-            const int w0 = max(v, 0) >> 5, w1 = (v + to - 1) >> 5;
-            const unsigned long long bits = (unsigned long long)__ldg(mask + w1) << 32 | __ldg(mask + w0);
-            allowed = v < 0 ? (unsigned)bits << -v : (unsigned)((w1 == w0 ? bits & 0xffffffffull : bits) >> (v & 31));
-        }
-        Eight<TY> out;
-        TY *o = reinterpret_cast<TY *>(out.raw);
-        const TX *i = reinterpret_cast<const TX *>(in[g].raw);
+        const int at = (g * THREADS + (int)threadIdx.x) * 8;
+        marked[g] = 0;
 #pragma unroll
         for (int k = 0; k < 8; k += 4) {
             const uint4 c4 = *reinterpret_cast<const uint4 *>(count + at + k);
-            uint4 b4 = make_uint4(NO_BIAS, NO_BIAS, NO_BIAS, NO_BIAS);
-            if (biased) b4 = *reinterpret_cast<const uint4 *>(bias + at + k);
-            const unsigned c[4] = {c4.x, c4.y, c4.z, c4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                float l = load_f32(i + k + j);
-                if (c[j]) {
-                    l = l > 0.f ? l / rep : l * rep;
-                    const unsigned n = c[j] & ~SEEN;
-                    if (n) l -= freq * (float)n + pres;
-                }
-                if (b[j] != NO_BIAS) l += __uint_as_float(b[j]);
-                if (!(allowed >> (k + j) & 1u)) l = -INFINITY;
-                store_f32(o + k + j, l);
+            marked[g] |= (c4.x ? 1u : 0u) << k | (c4.y ? 2u : 0u) << k | (c4.z ? 4u : 0u) << k | (c4.w ? 8u : 0u) << k;
+            if (biased) {
+                const uint4 b4 = *reinterpret_cast<const uint4 *>(bias + at + k);
+                marked[g] |= (b4.x != NO_BIAS ? 1u : 0u) << k | (b4.y != NO_BIAS ? 2u : 0u) << k | (b4.z != NO_BIAS ? 4u : 0u) << k | (b4.w != NO_BIAS ? 8u : 0u) << k;
             }
         }
-        if (wide_y && from == 0 && to == 8) {
+        if (marked[g]) {
+            int to = atomicAdd(&listed, __popc(marked[g]));
+            for (unsigned left = marked[g]; left; left &= left - 1) list[to++] = (uint16_t)(at + __ffs(left) - 1);
+        }
+    }
+    __syncthreads();
+    // what they become takes the place of their counts
+    for (int n = threadIdx.x; n < listed; n += THREADS) {
+        const int at = list[n];
+        count[at] = __float_as_uint(adjust(load_f32(x + first + at), count[at], biased ? bias[at] : NO_BIAS, rep, pres, freq));
+    }
+    __syncthreads();
 #pragma unroll
-            for (int q = 0; q < (int)sizeof(TY) / 2; q++) reinterpret_cast<uint4 *>(y + v)[q] = out.raw[q];
-        } else {
+    for (int g = 0; g < G; g++) {
+        const int at = (g * THREADS + (int)threadIdx.x) * 8, v = first + at;
+        if (v >= p.vocab || v + 8 <= 0) continue;
+        const int from = max(-v, 0), to = min(p.vocab - v, 8);
+        // bits v .. v + 7; those in front of the row and behind it do not matter
+        const unsigned allowed = v < 0 ? words[g][0] << -v : __funnelshift_r(words[g][0], words[g][1], v & 31);
+        Eight<TY> out;
+        TY *o = reinterpret_cast<TY *>(out.raw);
+        const TX *i = reinterpret_cast<const TX *>(in[g].raw);
+        float l[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) l[k] = load_f32(i + k);
+        if (marked[g]) {
 #pragma unroll
             for (int k = 0; k < 8; k++)
-                if (k >= from && k < to) y[v + k] = o[k];
+                if (marked[g] >> k & 1u) l[k] = __uint_as_float(count[at + k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++) store_f32(o + k, allowed >> k & 1u ? l[k] : -INFINITY);
+        store_eight(out, y + v, wide_y, from, to);
+    }
+}
+
+template <class TX, class TY>
+int launch_logits(LogitsParams p, cudaStream_t st)
+{
+    constexpr int THREADS = 256, G = 1, SLICE = THREADS * 8 * G;
+    // a row that does not start on a 16-byte boundary of x (or whose y does not) has a part of a group in front
+    const bool even = aligned(p.x, 16) && aligned(p.y, 16) && p.x_ld % 8 == 0 && p.y_ld % 8 == 0;
+    p.slices = (int)(((long long)p.vocab + (even ? 0 : 8) + SLICE - 1) / SLICE);
+    launch_dependent(logits_kernel<TX, TY, THREADS, G>, dim3((unsigned)(p.slices * p.rows)), THREADS, SLICE * (4 + 2 + (p.bias_begin ? 4 : 0)), st, p);
+    return launched();
+}
+
+// First of the two kernels: y = x under the mask.  As many CTAs as are resident at a time (with the second kernel's beside
+// them), so that the second may start at once; each takes pieces in turn.
+template <class TX>
+constexpr int MASK_GROUPS = sizeof(TX) == 4 ? 1 : 2;     // 32 bytes of x per thread and piece
+template <class TX, class TY>
+__global__ void __launch_bounds__(512, 4) logits_mask_kernel(const LogitsParams p)
+{
+    constexpr int G = MASK_GROUPS<TX>, SLICE = 512 * 8 * G;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");       // not before: the dependent reads what the grid before wrote
+    const long long pieces = (long long)p.slices * p.rows;
+    for (long long piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
+        const int row = (int)(piece / p.slices), slice = (int)(piece % p.slices);
+        const TX *x = static_cast<const TX *>(p.x) + (long long)row * p.x_ld;
+        TY *y = static_cast<TY *>(p.y) + (long long)row * p.y_ld;
+        const RowGroups<TX, TY> at(x, y);
+        const unsigned *mask = p.mask ? p.mask + (long long)row * p.mask_ld : nullptr;
+        Eight<TX> in[G];
+        unsigned words[G][2];
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            const int v = at.first + slice * SLICE + (g * 512 + (int)threadIdx.x) * 8;
+            if (v >= p.vocab || v + 8 <= 0) continue;
+            load_eight(in[g], x + v, v >= 0 && v + 8 <= p.vocab, -v, p.vocab - v);
+            words[g][0] = words[g][1] = 0xffffffffu;
+            if (mask) {                                      // bits v .. v + 7 are in at most two words
+                words[g][0] = __ldg(mask + (max(v, 0) >> 5));
+                words[g][1] = __ldg(mask + ((min(v + 8, p.vocab) - 1) >> 5));
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            const int v = at.first + slice * SLICE + (g * 512 + (int)threadIdx.x) * 8;
+            if (v >= p.vocab || v + 8 <= 0) continue;
+            Eight<TY> out;
+            TY *o = reinterpret_cast<TY *>(out.raw);
+            const TX *i = reinterpret_cast<const TX *>(in[g].raw);
+            const unsigned allowed = v < 0 ? words[g][0] << -v : __funnelshift_r(words[g][0], words[g][1], v & 31);
+#pragma unroll
+            for (int k = 0; k < 8; k++) store_f32(o + k, allowed >> k & 1u ? load_f32(i + k) : -INFINITY);
+            store_eight(out, y + v, at.wide_y, max(-v, 0), min(p.vocab - v, 8));
         }
     }
 }
 
-template <class TX, class TY, int G, int C>
-int launch_logits(LogitsParams p, cudaStream_t st)
+// Second: counts the tokens of a window of the vocabulary in a row's history, waits for the first, and rewrites what was said or
+// has a bias.  In place, y still has x where the mask allows.
+constexpr int LOGITS_WINDOW = 16384;
+
+template <class TX, class TY>
+__global__ void __launch_bounds__(1024, 2) logits_said_kernel(const LogitsParams p)
 {
-    constexpr int SLICE = 256 * 8 * G;
-    p.slices = ((p.vocab + 8 + SLICE - 1) / SLICE + C - 1) / C * C;        // (the groups may start up to 8 in front of the row)
-    const long long ctas = (long long)p.slices * p.rows;
-    if (ctas > 0x7fffffffll) return refuse("%d rows of %d are too many for one call", p.rows, p.vocab);
-    auto *kernel = logits_kernel<TX, TY, G, C>;
-    const unsigned smem = SLICE * 4 * (p.bias_begin ? 2 : 1);
-    if (smem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return refuse("cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    constexpr int THREADS = 1024, AT_ONCE = 2;
+    extern __shared__ __align__(16) unsigned count[];      // [LOGITS_WINDOW], then the list's 16-bit places
+    uint16_t *list = reinterpret_cast<uint16_t *>(count + LOGITS_WINDOW);
+    __shared__ int listed;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int windows = (p.vocab + LOGITS_WINDOW - 1) / LOGITS_WINDOW;
+    const int row = blockIdx.x / windows, start = blockIdx.x % windows * LOGITS_WINDOW;
+    const unsigned tokens = min(p.vocab - start, LOGITS_WINDOW);
+    const int said = p.history ? p.history_len[row] : 0, prompt = p.history && p.prompt_len ? p.prompt_len[row] : 0;
+    const bool biased = p.bias_begin != nullptr;
+    const int b0 = biased ? max(p.bias_begin[row], 0) : 0, b1 = biased ? p.bias_begin[row + 1] : 0;
+    for (int i = threadIdx.x; i < LOGITS_WINDOW / 4 && 4 * i < (int)tokens; i += THREADS) reinterpret_cast<uint4 *>(count)[i] = make_uint4(0, 0, 0, 0);
+    if (threadIdx.x == 0) listed = 0;
+    __syncthreads();
+    if (p.history) {
+        const int *h = p.history + (long long)row * p.history_ld;
+        const int len = (int)min((long long)max(said, 0), p.history_ld), me = threadIdx.x;
+        auto seen = [&](int id) {
+            const unsigned at = (unsigned)id - (unsigned)start;
+            if (at < tokens) atomicOr(&count[at], SEEN);
+        };
+        auto generated = [&](int id) {
+            const unsigned at = (unsigned)id - (unsigned)start;
+            if (at < tokens) atomicAdd(&count[at], 1u);
+        };
+        auto tally = [&](int id, int i) {
+            if (i < min(prompt, len)) seen(id);
+            else if (i < len) generated(id);
+        };
+        const int lone = min(len, (int)(((16 - (reinterpret_cast<uintptr_t>(h) & 15)) & 15) / 4)), pieces = (len - lone) / 4;      // 16-byte pieces
+        if (me < lone) tally(h[me], me);
+        for (int q = me; q < pieces; q += AT_ONCE * THREADS) {
+            int4 ids[AT_ONCE];
+#pragma unroll
+            for (int n = 0; n < AT_ONCE; n++)
+                if (q + n * THREADS < pieces) ids[n] = __ldg(reinterpret_cast<const int4 *>(h + lone) + q + n * THREADS);
+#pragma unroll
+            for (int n = 0; n < AT_ONCE; n++) {
+                if (q + n * THREADS >= pieces) break;
+                const int i = lone + 4 * (q + n * THREADS);
+                if (i >= prompt) {
+                    generated(ids[n].x);
+                    generated(ids[n].y);
+                    generated(ids[n].z);
+                    generated(ids[n].w);
+                } else if (i + 3 < prompt) {
+                    seen(ids[n].x);
+                    seen(ids[n].y);
+                    seen(ids[n].z);
+                    seen(ids[n].w);
+                } else {
+                    tally(ids[n].x, i);
+                    tally(ids[n].y, i + 1);
+                    tally(ids[n].z, i + 2);
+                    tally(ids[n].w, i + 3);
+                }
+            }
+        }
+        const int rest = lone + 4 * pieces + me;
+        if (rest < len) tally(h[rest], rest);
     }
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = C;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cfg.attrs = attr;
-    cfg.numAttrs = C == 1 ? 1 : 2;
-    cudaLaunchKernelEx(&cfg, kernel, p);
+    for (int e = b0 + threadIdx.x; e < b1; e += THREADS) {
+        const unsigned at = (unsigned)p.bias_ids[e] - (unsigned)start;
+        if (at < tokens && (atomicOr(&count[at], BIASED) & BIASED)) atomicOr(&count[at], BIASED_AGAIN);
+    }
+    const float rep = p.repetition ? p.repetition[row] : 1.f, pres = p.presence ? p.presence[row] : 0.f, freq = p.frequency ? p.frequency[row] : 0.f;
+    const TX *x = static_cast<const TX *>(p.x) + (long long)row * p.x_ld + start;
+    TY *y = static_cast<TY *>(p.y) + (long long)row * p.y_ld + start;
+    const unsigned *mask = p.mask ? p.mask + (long long)row * p.mask_ld : nullptr;
+    auto allowed = [&](unsigned at) { return !mask || __ldg(mask + ((start + at) >> 5)) >> ((start + at) & 31) & 1u; };
+    __syncthreads();
+    if (p.history) {
+        for (int i = threadIdx.x; i < LOGITS_WINDOW / 4 && 4 * i < (int)tokens; i += THREADS) {
+            const uint4 c4 = reinterpret_cast<const uint4 *>(count)[i];
+            const unsigned c[4] = {c4.x, c4.y, c4.z, c4.w};
+            if ((c4.x | c4.y | c4.z | c4.w) == 0) continue;
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (c[k] && !(c[k] & BIASED)) list[atomicAdd(&listed, 1)] = (uint16_t)(4 * i + k);
+        }
+        __syncthreads();
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int n = threadIdx.x; n < listed; n += THREADS) {
+        const unsigned at = list[n], c = count[at];
+        if (allowed(at)) store_f32(y + at, adjust(load_f32(x + at), c, NO_BIAS, rep, pres, freq));
+    }
+    for (int e = b0 + threadIdx.x; e < b1; e += THREADS) {
+        const int id = p.bias_ids[e];
+        const unsigned at = (unsigned)id - (unsigned)start;
+        if (at >= tokens || !allowed(at)) continue;
+        float bias = p.bias_values[e];
+        if ((count[at] & BIASED_AGAIN) && !sum_of_biases(p, b0, b1, e, id, bias)) continue;
+        store_f32(y + at, adjust(load_f32(x + at), count[at], bias_bits(bias), rep, pres, freq));
+    }
+}
+
+template <class TX, class TY>
+int launch_logits_two(LogitsParams p, cudaStream_t st)
+{
+    constexpr int SLICE = 512 * 8 * MASK_GROUPS<TX>;
+    const bool even = aligned(p.x, 16) && aligned(p.y, 16) && p.x_ld % 8 == 0 && p.y_ld % 8 == 0;
+    p.slices = (int)(((long long)p.vocab + (even ? 0 : 8) + SLICE - 1) / SLICE);
+    const long long pieces = (long long)p.slices * p.rows, windows = ((long long)p.vocab + LOGITS_WINDOW - 1) / LOGITS_WINDOW * p.rows;
+    if (windows > 0x7fffffffll) return refuse("%d rows of %d are too many for one call", p.rows, p.vocab);
+    constexpr int SMEM = LOGITS_WINDOW * 6;
+    const bool rewrite = p.history || p.bias_begin;
+    if (rewrite) {
+        int rc = ask_for_shared(logits_said_kernel<TX, TY>, SMEM);
+        if (rc == 0) rc = ask_for_shared(logits_mask_kernel<TX, TY>, 0);
+        if (rc != 0) return rc;
+    }
+    launch_dependent(logits_mask_kernel<TX, TY>, dim3((unsigned)(pieces < 148 * 2 ? pieces : 148 * 2)), 512, 0, st, p);
+    const int rc = launched();
+    if (rc != 0 || !rewrite) return rc;
+    launch_dependent(logits_said_kernel<TX, TY>, dim3((unsigned)windows), 1024, SMEM, st, p);
     return launched();
 }
 
 template <class TX, class TY>
 int launch_logits_sized(const LogitsParams &p, cudaStream_t st)
 {
-    // Slices of 8192 where that still gives every SM several, of 2048 for few rows; clusters where the history, read by every
-    // slice of a row, would be more than a slice's own values.
-    const bool large = (long long)p.rows * p.vocab >= 148ll * 3 * 8192;
-    if (p.history && p.history_ld > 8192) return large ? launch_logits<TX, TY, 4, 8>(p, st) : launch_logits<TX, TY, 1, 8>(p, st);
-    return large ? launch_logits<TX, TY, 4, 1>(p, st) : launch_logits<TX, TY, 1, 1>(p, st);
+    // slices of 2048 that do not give every SM more than four, and a history that each of them can go through
+    if ((long long)p.rows * p.vocab <= 148ll * 4 * 2048 && (!p.history || p.history_ld <= 8192)) return launch_logits<TX, TY>(p, st);
+    return launch_logits_two<TX, TY>(p, st);
 }
 
 template <class TX>
@@ -506,7 +789,6 @@ int launch_logits_to(const LogitsParams &p, int y_dtype, cudaStream_t st)
     return launch_logits_sized<TX, float>(p, st);
 }
 
-bool aligned(const void *p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 bool is_type(int t) { return t == GEMM_X_BF16 || t == GEMM_X_F16 || t == GEMM_X_F32; }
 
 }  // namespace
@@ -571,6 +853,7 @@ int gemm_logits(const GemmLogitsArgs *a)
     if (a->x == a->y && (a->x_dtype != a->y_dtype || a->x_ld != a->y_ld)) return refuse("in place, x and y have the same type and row pitch");
     if (a->history && (!a->history_len || a->history_ld < 0)) return refuse("history needs history_len and history_ld >= 0");
     if ((a->bias_begin || a->bias_ids || a->bias_values) && !(a->bias_begin && a->bias_ids && a->bias_values)) return refuse("biases need ids, values and row borders");
+    if (a->history_ld >= 1ll << 29) return refuse("history_ld %lld: fewer than 2^29 are wanted", (long long)a->history_ld);
     if (a->mask && a->mask_ld < ((long long)a->vocab + 31) / 32) return refuse("mask_ld %lld is below %lld words", (long long)a->mask_ld, ((long long)a->vocab + 31) / 32);
     const void *words[] = {a->history, a->history_len, a->prompt_len, a->repetition, a->presence, a->frequency, a->bias_ids, a->bias_values, a->bias_begin, a->mask};
     for (const void *w : words)
