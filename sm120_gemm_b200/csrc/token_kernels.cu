@@ -315,24 +315,56 @@ struct LogitsParams {
     const int *bias_begin;
     const unsigned *mask;
     int rows, vocab;
-    int slices;                  // of a row
+    int windows, window;         // windows of a row, tokens of a window
+    int counting_warps;
 };
 
-// Two ways, by size:
-//   one kernel   few values and a short history: a CTA takes a slice of a row (SLICE values), goes through the row's whole
-//                history, counts what is in its slice in shared memory and writes the slice once.  One launch, 3.9 us at
-//                1 x 32001.
-//   two kernels  else: the first streams x to y under the mask at the memory's rate; the second, a programmatic dependent that
-//                counts beside it and then waits for it, rewrites the few tokens that were said or have a bias.  Counting in
-//                the streaming kernel held every slice up for the history's round trips: 64 x 131072 with 4096 said took
-//                29 us whatever the slices' size.
-// The tokens that need arithmetic (a division among it) are listed, so that whole warps do it, not every warp for the one lane
-// in thirty that has such a token.  Counting is by integer atomics in shared memory: the order does not matter.
-constexpr unsigned NO_BIAS = 0xffffffffu;
-// a token's count word: in the prompt; has a bias, several (second kernel); below them how often it was generated
+// A CTA has a window of a row's vocabulary.  Some of its warps count the row's history into shared memory, what is in the
+// window (integer atomics: the order does not matter); meanwhile the others write y = x under the mask for the window, chunk
+// by chunk, and the counting warps join them.  Then the few tokens that were said or have a bias are listed and rewritten:
+// whole warps do their arithmetic (a division among it), not every warp for the one lane in thirty that needs it.  HBM-bound on long rows: x once, y once.  What it must not do is wait: with the counting in front of the
+// writing a CTA held its window up for four round trips to memory, 29 us at 64 x 131072 with 4096 said whatever the size of
+// the windows; writing and rewriting in two kernels took 28.
+// a token's count: in the prompt; has a bias, several; how often it was generated.  16 bits hold it (the flags in the upper
+// three) as long as the history has fewer than 2^13 ids, which lets the windows be twice as large.
 constexpr unsigned SEEN = 0x80000000u, BIASED = 0x40000000u, BIASED_AGAIN = 0x20000000u, GENERATED = 0x1fffffffu;
-constexpr unsigned SEVERAL = 0xfffffffeu;        // first kernel: in the place of bias bits
-__device__ __forceinline__ unsigned bias_bits(float v) { return v == v ? __float_as_uint(v) : 0x7fc00000u; }      // never one of the marks
+template <bool NARROW>
+struct Counts {
+    unsigned *words;
+    static constexpr int BITS = NARROW ? 16 : 32, PER_WORD = 32 / BITS;
+    __device__ __forceinline__ void add(unsigned at) { atomicAdd(words + at / PER_WORD, 1u << at % PER_WORD * BITS % 32); }
+    // sets flag bits (of the 32-bit form); returns what was there
+    __device__ __forceinline__ unsigned set(unsigned at, unsigned flag)
+    {
+        if constexpr (NARROW) return wide(atomicOr(words + at / 2, (flag >> 16) << at % 2 * 16) >> at % 2 * 16 & 0xffffu);
+        else return atomicOr(words + at, flag);
+    }
+    static __device__ __forceinline__ unsigned wide(unsigned half) { return (half & 0xe000u) << 16 | (half & 0x1fffu); }
+    // which of the 8 tokens from `at` on (a multiple of 8) were said and have no bias
+    __device__ __forceinline__ unsigned said(unsigned at) const
+    {
+        unsigned w[8 / PER_WORD], bits = 0;
+#pragma unroll
+        for (int i = 0; i < 8 / PER_WORD; i += 4) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(words + at / PER_WORD + i);
+            w[i] = v.x;
+            w[i + 1] = v.y;
+            w[i + 2] = v.z;
+            w[i + 3] = v.w;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const unsigned c = w[k / PER_WORD] >> k % PER_WORD * BITS % 32 & (NARROW ? 0xffffu : 0xffffffffu);
+            bits |= c != 0 && !(c & (BIASED >> (32 - BITS))) ? 1u << k : 0u;
+        }
+        return bits;
+    }
+    __device__ __forceinline__ unsigned get(unsigned at) const
+    {
+        if constexpr (NARROW) return wide(reinterpret_cast<const uint16_t *>(words)[at]);
+        else return words[at];
+    }
+};
 
 template <class T>
 struct Eight {                                   // 8 values as they lie in memory, 16-byte accesses
@@ -381,15 +413,15 @@ struct RowGroups {
     }
 };
 
-// a token that was said (c: count word) or has a bias (its bits)
-__device__ __forceinline__ float adjust(float l, unsigned c, unsigned b, float rep, float pres, float freq)
+// a token's logit under its count and its biases' sum
+__device__ __forceinline__ float adjust(float l, unsigned c, float bias, float rep, float pres, float freq)
 {
     if (c & (SEEN | GENERATED)) {
         l = l > 0.f ? l / rep : l * rep;
         const unsigned n = c & GENERATED;
         if (n) l -= freq * (float)n + pres;
     }
-    return b != NO_BIAS ? l + __uint_as_float(b) : l;
+    return c & BIASED ? l + bias : l;
 }
 
 // An id that is listed more than once: its values are added in the order of the list, by the thread of the first entry (true).
@@ -406,225 +438,97 @@ __device__ __forceinline__ bool sum_of_biases(const LogitsParams &p, int b0, int
     return first;
 }
 
-template <class TX, class TY, int THREADS, int G>
-__global__ void __launch_bounds__(THREADS, 1536 / THREADS) logits_kernel(const LogitsParams p)
+template <class TX, class TY, bool NARROW, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 3 : 1) logits_kernel(const LogitsParams p)
 {
-    constexpr int SLICE = THREADS * 8 * G;
-    extern __shared__ __align__(16) unsigned count[];      // [SLICE]; [SLICE] 16-bit places of the list; with biases [SLICE] of their bits
-    uint16_t *list = reinterpret_cast<uint16_t *>(count + SLICE);
-    unsigned *bias = count + SLICE + SLICE / 2;
-    __shared__ int doubled, listed;
+    constexpr int G = sizeof(TX) == 4 ? 1 : 2, CHUNK = 32 * 8 * G;
+    extern __shared__ __align__(16) unsigned shared[];     // the window's counts, then the list (16-bit places in the window)
+    __shared__ int next_chunk, listed;
     after_the_grid_before();
-    const int row = blockIdx.x / p.slices, slice = blockIdx.x % p.slices;
-    // what the row's parts start with is asked for first: each is the address of the next load
-    const int said = p.history ? p.history_len[row] : 0, prompt = p.history && p.prompt_len ? p.prompt_len[row] : 0;
-    const bool biased = p.bias_begin != nullptr;
-    const int bias_from = biased ? p.bias_begin[row] : 0, b1 = biased ? p.bias_begin[row + 1] : 0;
-    const float rep = p.repetition ? p.repetition[row] : 1.f, pres = p.presence ? p.presence[row] : 0.f, freq = p.frequency ? p.frequency[row] : 0.f;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Counts<NARROW> count = {shared};
+    uint16_t *list = reinterpret_cast<uint16_t *>(shared + p.window / count.PER_WORD);
+    const int row = blockIdx.x / p.windows;
     const TX *x = static_cast<const TX *>(p.x) + (long long)row * p.x_ld;
     TY *y = static_cast<TY *>(p.y) + (long long)row * p.y_ld;
     const RowGroups<TX, TY> groups(x, y);
-    const bool wide_y = groups.wide_y;
-    const int first = groups.first + slice * SLICE;        // token of count[0]; below 0 in the first slice of some rows
-    if (first >= p.vocab) return;
-    Eight<TX> in[G];
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-        const int v = first + (g * THREADS + (int)threadIdx.x) * 8;
-        if (v < p.vocab && v + 8 > 0) load_eight(in[g], x + v, v >= 0 && v + 8 <= p.vocab, -v, p.vocab - v);
-    }
-    // mask words of the groups, and the first ids of the history (those behind its end do not count later)
+    // the window's tokens are start .. start + tokens - 1; counts and chunks begin at lo, up to 8 in front of the row
+    const int lo = groups.first + blockIdx.x % p.windows * p.window, start = max(lo, 0), lead = start - lo;
+    const int tokens = (int)(min((long long)lo + p.window, (long long)p.vocab) - start);
+    if (tokens <= 0) return;
+    const int said = p.history ? p.history_len[row] : 0, prompt = p.history && p.prompt_len ? p.prompt_len[row] : 0;
+    const bool biased = p.bias_begin != nullptr;
+    const int b0 = biased ? max(p.bias_begin[row], 0) : 0, b1 = biased ? p.bias_begin[row + 1] : 0;
+    const float rep = p.repetition ? p.repetition[row] : 1.f, pres = p.presence ? p.presence[row] : 0.f, freq = p.frequency ? p.frequency[row] : 0.f;
     const unsigned *mask = p.mask ? p.mask + (long long)row * p.mask_ld : nullptr;
-    unsigned words[G][2];
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-        const int v = first + (g * THREADS + (int)threadIdx.x) * 8, end = min(v + 8, p.vocab);
-        words[g][0] = words[g][1] = 0xffffffffu;
-        if (mask && v < p.vocab && v + 8 > 0) {          // bits v .. v + 7 are in at most two words
-            words[g][0] = __ldg(mask + (max(v, 0) >> 5));
-            words[g][1] = __ldg(mask + ((end - 1) >> 5));
-        }
-    }
-    const int *h = p.history + (long long)row * p.history_ld;
-    const int lone = (int)min(p.history_ld, (long long)(((16 - (reinterpret_cast<uintptr_t>(h) & 15)) & 15) / 4));        // in front of the 16-byte pieces
-    constexpr int AT_ONCE = 2;
-    int4 ids[AT_ONCE];
-    auto load_ids = [&](int q, long long pieces) {
-#pragma unroll
-        for (int n = 0; n < AT_ONCE; n++)
-            if (q + n * THREADS < pieces) ids[n] = __ldg(reinterpret_cast<const int4 *>(h + lone) + q + n * THREADS);
-    };
-    if (p.history) load_ids(threadIdx.x, (p.history_ld - lone) / 4);
-    for (int i = threadIdx.x; i < SLICE / 4; i += THREADS) {
-        reinterpret_cast<uint4 *>(count)[i] = make_uint4(0, 0, 0, 0);
-        if (biased) reinterpret_cast<uint4 *>(bias)[i] = make_uint4(NO_BIAS, NO_BIAS, NO_BIAS, NO_BIAS);
-    }
-    if (threadIdx.x == 0) doubled = listed = 0;
+    const bool rewrite = p.history || biased;
+    if (rewrite)
+        for (int i = threadIdx.x; i * 4 * count.PER_WORD < p.window; i += THREADS) reinterpret_cast<uint4 *>(count.words)[i] = make_uint4(0, 0, 0, 0);
+    if (threadIdx.x == 0) next_chunk = listed = 0;
     __syncthreads();
-    // the slice's tokens are start .. start + tokens - 1, the first of them at count[lead]
-    const int start = max(first, 0), lead = start - first;
-    const unsigned tokens = min((long long)first + SLICE, (long long)p.vocab) - start;
-    const int b0 = max(bias_from, 0);
-    int bias_id = -1;
-    float bias_value = 0.f;
-    if (b0 + (int)threadIdx.x < b1) {
-        bias_id = p.bias_ids[b0 + threadIdx.x];
-        bias_value = p.bias_values[b0 + threadIdx.x];
-    }
-    if (p.history) {
-        const int len = (int)min((long long)max(said, 0), p.history_ld), me = threadIdx.x;
-        auto seen = [&](int id) {
-            const unsigned at = (unsigned)id - (unsigned)start;
-            if (at < tokens) atomicOr(&count[lead + at], SEEN);
-        };
-        auto generated = [&](int id) {
-            const unsigned at = (unsigned)id - (unsigned)start;
-            if (at < tokens) atomicAdd(&count[lead + at], 1u);
-        };
-        auto tally = [&](int id, int i) {
-            if (i < min(prompt, len)) seen(id);
-            else if (i < len) generated(id);
-        };
-        if (me < lone) tally(h[me], me);
-        const int pieces = (int)((p.history_ld - lone) / 4);
-        for (int q = me; lone + 4 * q < len; q += AT_ONCE * THREADS) {
-            if (q != me) load_ids(q, pieces);
+    if (warp < p.counting_warps) {
+        const int counting = p.counting_warps * 32, me = threadIdx.x;
+        if (p.history) {
+            const int len = (int)min((long long)max(said, 0), p.history_ld);
+            const int *h = p.history + (long long)row * p.history_ld;
+            auto seen = [&](int id) {
+                const unsigned at = (unsigned)id - (unsigned)start;
+                if (at < (unsigned)tokens) count.set(lead + at, SEEN);
+            };
+            auto generated = [&](int id) {
+                const unsigned at = (unsigned)id - (unsigned)start;
+                if (at < (unsigned)tokens) count.add(lead + at);
+            };
+            auto either = [&](int id, int i) {
+                if (i < prompt) seen(id);
+                else generated(id);
+            };
+            const int lone = min(len, (int)(((16 - (reinterpret_cast<uintptr_t>(h) & 15)) & 15) / 4)), pieces = (len - lone) / 4;      // 16-byte pieces
+            if (me < lone) either(h[me], me);
+            constexpr int AT_ONCE = 4;
+            for (int q = me; q < pieces; q += AT_ONCE * counting) {
+                int4 ids[AT_ONCE];
 #pragma unroll
-            for (int n = 0; n < AT_ONCE; n++) {
-                const int i = lone + 4 * (q + n * THREADS);
-                if (q + n * THREADS >= pieces || i >= len) break;
-                if (i >= prompt && i + 3 < len) {
-                    generated(ids[n].x);
-                    generated(ids[n].y);
-                    generated(ids[n].z);
-                    generated(ids[n].w);
-                } else if (i + 3 < prompt && i + 3 < len) {
-                    seen(ids[n].x);
-                    seen(ids[n].y);
-                    seen(ids[n].z);
-                    seen(ids[n].w);
-                } else {
-                    tally(ids[n].x, i);
-                    tally(ids[n].y, i + 1);
-                    tally(ids[n].z, i + 2);
-                    tally(ids[n].w, i + 3);
+                for (int n = 0; n < AT_ONCE; n++)
+                    if (q + n * counting < pieces) ids[n] = __ldg(reinterpret_cast<const int4 *>(h + lone) + q + n * counting);
+#pragma unroll
+                for (int n = 0; n < AT_ONCE; n++) {
+                    if (q + n * counting >= pieces) break;
+                    const int i = lone + 4 * (q + n * counting);
+                    if (i >= prompt) {
+                        generated(ids[n].x);
+                        generated(ids[n].y);
+                        generated(ids[n].z);
+                        generated(ids[n].w);
+                    } else {
+                        either(ids[n].x, i);
+                        either(ids[n].y, i + 1);
+                        either(ids[n].z, i + 2);
+                        either(ids[n].w, i + 3);
+                    }
                 }
             }
+            const int rest = lone + 4 * pieces + me;
+            if (rest < len) either(h[rest], rest);
         }
-        const int rest = lone + 4 * pieces + me;         // the row's last ids behind the pieces
-        if (rest < len) tally(h[rest], rest);
-    }
-    auto biased_here = [&](int id, unsigned &at) {
-        at = (unsigned)id - (unsigned)start;
-        const bool here = at < tokens;
-        at += lead;
-        return here;
-    };
-    unsigned at_bias;
-    for (int e = b0 + threadIdx.x; e < b1; e += THREADS) {
-        if (e != b0 + (int)threadIdx.x) {
-            bias_id = p.bias_ids[e];
-            bias_value = p.bias_values[e];
-        }
-        if (biased_here(bias_id, at_bias) && atomicExch(&bias[at_bias], bias_bits(bias_value)) != NO_BIAS) {
-            atomicExch(&bias[at_bias], SEVERAL);          // after the last of them, whichever it is
-            doubled = 1;
+        for (int e = b0 + me; e < b1; e += counting) {
+            const unsigned at = (unsigned)p.bias_ids[e] - (unsigned)start;
+            if (at < (unsigned)tokens && (count.set(lead + at, BIASED) & BIASED)) count.set(lead + at, BIASED_AGAIN);
         }
     }
-    __syncthreads();
-    if (biased && doubled) {
-        for (int e = b0 + threadIdx.x; e < b1; e += THREADS) {
-            const int id = p.bias_ids[e];
-            float sum;
-            if (biased_here(id, at_bias) && bias[at_bias] == SEVERAL && sum_of_biases(p, b0, b1, e, id, sum)) bias[at_bias] = bias_bits(sum);
-        }
-        __syncthreads();
-    }
-    // the tokens of this thread's groups that have something to be done
-    unsigned marked[G];
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-        const int at = (g * THREADS + (int)threadIdx.x) * 8;
-        marked[g] = 0;
-#pragma unroll
-        for (int k = 0; k < 8; k += 4) {
-            const uint4 c4 = *reinterpret_cast<const uint4 *>(count + at + k);
-            marked[g] |= (c4.x ? 1u : 0u) << k | (c4.y ? 2u : 0u) << k | (c4.z ? 4u : 0u) << k | (c4.w ? 8u : 0u) << k;
-            if (biased) {
-                const uint4 b4 = *reinterpret_cast<const uint4 *>(bias + at + k);
-                marked[g] |= (b4.x != NO_BIAS ? 1u : 0u) << k | (b4.y != NO_BIAS ? 2u : 0u) << k | (b4.z != NO_BIAS ? 4u : 0u) << k | (b4.w != NO_BIAS ? 8u : 0u) << k;
-            }
-        }
-        if (marked[g]) {
-            int to = atomicAdd(&listed, __popc(marked[g]));
-            for (unsigned left = marked[g]; left; left &= left - 1) list[to++] = (uint16_t)(at + __ffs(left) - 1);
-        }
-    }
-    __syncthreads();
-    // what they become takes the place of their counts
-    for (int n = threadIdx.x; n < listed; n += THREADS) {
-        const int at = list[n];
-        count[at] = __float_as_uint(adjust(load_f32(x + first + at), count[at], biased ? bias[at] : NO_BIAS, rep, pres, freq));
-    }
-    __syncthreads();
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-        const int at = (g * THREADS + (int)threadIdx.x) * 8, v = first + at;
-        if (v >= p.vocab || v + 8 <= 0) continue;
-        const int from = max(-v, 0), to = min(p.vocab - v, 8);
-        // bits v .. v + 7; those in front of the row and behind it do not matter
-        const unsigned allowed = v < 0 ? words[g][0] << -v : __funnelshift_r(words[g][0], words[g][1], v & 31);
-        Eight<TY> out;
-        TY *o = reinterpret_cast<TY *>(out.raw);
-        const TX *i = reinterpret_cast<const TX *>(in[g].raw);
-        float l[8];
-#pragma unroll
-        for (int k = 0; k < 8; k++) l[k] = load_f32(i + k);
-        if (marked[g]) {
-#pragma unroll
-            for (int k = 0; k < 8; k++)
-                if (marked[g] >> k & 1u) l[k] = __uint_as_float(count[at + k]);
-        }
-#pragma unroll
-        for (int k = 0; k < 8; k++) store_f32(o + k, allowed >> k & 1u ? l[k] : -INFINITY);
-        store_eight(out, y + v, wide_y, from, to);
-    }
-}
-
-template <class TX, class TY>
-int launch_logits(LogitsParams p, cudaStream_t st)
-{
-    constexpr int THREADS = 256, G = 1, SLICE = THREADS * 8 * G;
-    // a row that does not start on a 16-byte boundary of x (or whose y does not) has a part of a group in front
-    const bool even = aligned(p.x, 16) && aligned(p.y, 16) && p.x_ld % 8 == 0 && p.y_ld % 8 == 0;
-    p.slices = (int)(((long long)p.vocab + (even ? 0 : 8) + SLICE - 1) / SLICE);
-    launch_dependent(logits_kernel<TX, TY, THREADS, G>, dim3((unsigned)(p.slices * p.rows)), THREADS, SLICE * (4 + 2 + (p.bias_begin ? 4 : 0)), st, p);
-    return launched();
-}
-
-// First of the two kernels: y = x under the mask.  As many CTAs as are resident at a time (with the second kernel's beside
-// them), so that the second may start at once; each takes pieces in turn.
-template <class TX>
-constexpr int MASK_GROUPS = sizeof(TX) == 4 ? 1 : 2;     // 32 bytes of x per thread and piece
-template <class TX, class TY>
-__global__ void __launch_bounds__(512, 4) logits_mask_kernel(const LogitsParams p)
-{
-    constexpr int G = MASK_GROUPS<TX>, SLICE = 512 * 8 * G;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");       // not before: the dependent reads what the grid before wrote
-    const long long pieces = (long long)p.slices * p.rows;
-    for (long long piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
-        const int row = (int)(piece / p.slices), slice = (int)(piece % p.slices);
-        const TX *x = static_cast<const TX *>(p.x) + (long long)row * p.x_ld;
-        TY *y = static_cast<TY *>(p.y) + (long long)row * p.y_ld;
-        const RowGroups<TX, TY> at(x, y);
-        const unsigned *mask = p.mask ? p.mask + (long long)row * p.mask_ld : nullptr;
+    // y = x under the mask
+    const int chunks = (lead + tokens + CHUNK - 1) / CHUNK;
+    for (;;) {
+        int c = 0;
+        if (lane == 0) c = atomicAdd(&next_chunk, 1);
+        c = __shfl_sync(0xffffffffu, c, 0);
+        if (c >= chunks) break;
         Eight<TX> in[G];
         unsigned words[G][2];
 #pragma unroll
         for (int g = 0; g < G; g++) {
-            const int v = at.first + slice * SLICE + (g * 512 + (int)threadIdx.x) * 8;
-            if (v >= p.vocab || v + 8 <= 0) continue;
+            const int at = c * CHUNK + (g * 32 + lane) * 8, v = lo + at;
+            if (at >= lead + tokens || v + 8 <= 0) continue;
             load_eight(in[g], x + v, v >= 0 && v + 8 <= p.vocab, -v, p.vocab - v);
             words[g][0] = words[g][1] = 0xffffffffu;
             if (mask) {                                      // bits v .. v + 7 are in at most two words
@@ -634,151 +538,83 @@ __global__ void __launch_bounds__(512, 4) logits_mask_kernel(const LogitsParams 
         }
 #pragma unroll
         for (int g = 0; g < G; g++) {
-            const int v = at.first + slice * SLICE + (g * 512 + (int)threadIdx.x) * 8;
-            if (v >= p.vocab || v + 8 <= 0) continue;
+            const int at = c * CHUNK + (g * 32 + lane) * 8, v = lo + at;
+            if (at >= lead + tokens || v + 8 <= 0) continue;
             Eight<TY> out;
             TY *o = reinterpret_cast<TY *>(out.raw);
             const TX *i = reinterpret_cast<const TX *>(in[g].raw);
             const unsigned allowed = v < 0 ? words[g][0] << -v : __funnelshift_r(words[g][0], words[g][1], v & 31);
 #pragma unroll
             for (int k = 0; k < 8; k++) store_f32(o + k, allowed >> k & 1u ? load_f32(i + k) : -INFINITY);
-            store_eight(out, y + v, at.wide_y, max(-v, 0), min(p.vocab - v, 8));
+            store_eight(out, y + v, groups.wide_y, max(-v, 0), min(p.vocab - v, 8));
         }
     }
-}
-
-// Second: counts the tokens of a window of the vocabulary in a row's history, waits for the first, and rewrites what was said or
-// has a bias.  In place, y still has x where the mask allows.
-constexpr int LOGITS_WINDOW = 16384;
-
-template <class TX, class TY>
-__global__ void __launch_bounds__(1024, 2) logits_said_kernel(const LogitsParams p)
-{
-    constexpr int THREADS = 1024, AT_ONCE = 2;
-    extern __shared__ __align__(16) unsigned count[];      // [LOGITS_WINDOW], then the list's 16-bit places
-    uint16_t *list = reinterpret_cast<uint16_t *>(count + LOGITS_WINDOW);
-    __shared__ int listed;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int windows = (p.vocab + LOGITS_WINDOW - 1) / LOGITS_WINDOW;
-    const int row = blockIdx.x / windows, start = blockIdx.x % windows * LOGITS_WINDOW;
-    const unsigned tokens = min(p.vocab - start, LOGITS_WINDOW);
-    const int said = p.history ? p.history_len[row] : 0, prompt = p.history && p.prompt_len ? p.prompt_len[row] : 0;
-    const bool biased = p.bias_begin != nullptr;
-    const int b0 = biased ? max(p.bias_begin[row], 0) : 0, b1 = biased ? p.bias_begin[row + 1] : 0;
-    for (int i = threadIdx.x; i < LOGITS_WINDOW / 4 && 4 * i < (int)tokens; i += THREADS) reinterpret_cast<uint4 *>(count)[i] = make_uint4(0, 0, 0, 0);
-    if (threadIdx.x == 0) listed = 0;
-    __syncthreads();
+    if (!rewrite) return;
+    __syncthreads();                                         // counted and written
+    // (in place, y still has x where the mask allows)
+    auto allowed = [&](int v) { return !mask || __ldg(mask + (v >> 5)) >> (v & 31) & 1u; };
     if (p.history) {
-        const int *h = p.history + (long long)row * p.history_ld;
-        const int len = (int)min((long long)max(said, 0), p.history_ld), me = threadIdx.x;
-        auto seen = [&](int id) {
-            const unsigned at = (unsigned)id - (unsigned)start;
-            if (at < tokens) atomicOr(&count[at], SEEN);
-        };
-        auto generated = [&](int id) {
-            const unsigned at = (unsigned)id - (unsigned)start;
-            if (at < tokens) atomicAdd(&count[at], 1u);
-        };
-        auto tally = [&](int id, int i) {
-            if (i < min(prompt, len)) seen(id);
-            else if (i < len) generated(id);
-        };
-        const int lone = min(len, (int)(((16 - (reinterpret_cast<uintptr_t>(h) & 15)) & 15) / 4)), pieces = (len - lone) / 4;      // 16-byte pieces
-        if (me < lone) tally(h[me], me);
-        for (int q = me; q < pieces; q += AT_ONCE * THREADS) {
-            int4 ids[AT_ONCE];
+        for (int at = threadIdx.x * 8; at - lane * 8 < p.window; at += THREADS * 8) {
+            const unsigned marked = at < p.window ? count.said(at) : 0u;
+            const int mine = __popc(marked), all = __reduce_add_sync(0xffffffffu, mine);
+            if (all == 0) continue;
+            int to = mine;                                   // places up to and with this lane's
 #pragma unroll
-            for (int n = 0; n < AT_ONCE; n++)
-                if (q + n * THREADS < pieces) ids[n] = __ldg(reinterpret_cast<const int4 *>(h + lone) + q + n * THREADS);
-#pragma unroll
-            for (int n = 0; n < AT_ONCE; n++) {
-                if (q + n * THREADS >= pieces) break;
-                const int i = lone + 4 * (q + n * THREADS);
-                if (i >= prompt) {
-                    generated(ids[n].x);
-                    generated(ids[n].y);
-                    generated(ids[n].z);
-                    generated(ids[n].w);
-                } else if (i + 3 < prompt) {
-                    seen(ids[n].x);
-                    seen(ids[n].y);
-                    seen(ids[n].z);
-                    seen(ids[n].w);
-                } else {
-                    tally(ids[n].x, i);
-                    tally(ids[n].y, i + 1);
-                    tally(ids[n].z, i + 2);
-                    tally(ids[n].w, i + 3);
-                }
+            for (int o = 1; o < 32; o <<= 1) {
+                const int before = __shfl_up_sync(0xffffffffu, to, o);
+                if (lane >= o) to += before;
             }
-        }
-        const int rest = lone + 4 * pieces + me;
-        if (rest < len) tally(h[rest], rest);
-    }
-    for (int e = b0 + threadIdx.x; e < b1; e += THREADS) {
-        const unsigned at = (unsigned)p.bias_ids[e] - (unsigned)start;
-        if (at < tokens && (atomicOr(&count[at], BIASED) & BIASED)) atomicOr(&count[at], BIASED_AGAIN);
-    }
-    const float rep = p.repetition ? p.repetition[row] : 1.f, pres = p.presence ? p.presence[row] : 0.f, freq = p.frequency ? p.frequency[row] : 0.f;
-    const TX *x = static_cast<const TX *>(p.x) + (long long)row * p.x_ld + start;
-    TY *y = static_cast<TY *>(p.y) + (long long)row * p.y_ld + start;
-    const unsigned *mask = p.mask ? p.mask + (long long)row * p.mask_ld : nullptr;
-    auto allowed = [&](unsigned at) { return !mask || __ldg(mask + ((start + at) >> 5)) >> ((start + at) & 31) & 1u; };
-    __syncthreads();
-    if (p.history) {
-        for (int i = threadIdx.x; i < LOGITS_WINDOW / 4 && 4 * i < (int)tokens; i += THREADS) {
-            const uint4 c4 = reinterpret_cast<const uint4 *>(count)[i];
-            const unsigned c[4] = {c4.x, c4.y, c4.z, c4.w};
-            if ((c4.x | c4.y | c4.z | c4.w) == 0) continue;
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (c[k] && !(c[k] & BIASED)) list[atomicAdd(&listed, 1)] = (uint16_t)(4 * i + k);
+            int base = 0;
+            if (lane == 0) base = atomicAdd(&listed, all);
+            to += __shfl_sync(0xffffffffu, base, 0) - mine;
+            for (unsigned left = marked; left; left &= left - 1) list[to++] = (uint16_t)(at + __ffs(left) - 1);
         }
         __syncthreads();
-    }
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (int n = threadIdx.x; n < listed; n += THREADS) {
-        const unsigned at = list[n], c = count[at];
-        if (allowed(at)) store_f32(y + at, adjust(load_f32(x + at), c, NO_BIAS, rep, pres, freq));
+        for (int n = threadIdx.x; n < listed; n += THREADS) {
+            const int at = list[n], v = lo + at;
+            if (allowed(v)) store_f32(y + v, adjust(load_f32(x + v), count.get(at), 0.f, rep, pres, freq));
+        }
     }
     for (int e = b0 + threadIdx.x; e < b1; e += THREADS) {
         const int id = p.bias_ids[e];
         const unsigned at = (unsigned)id - (unsigned)start;
-        if (at >= tokens || !allowed(at)) continue;
+        if (at >= (unsigned)tokens || !allowed(id)) continue;
+        const unsigned c = count.get(lead + at);
         float bias = p.bias_values[e];
-        if ((count[at] & BIASED_AGAIN) && !sum_of_biases(p, b0, b1, e, id, bias)) continue;
-        store_f32(y + at, adjust(load_f32(x + at), count[at], bias_bits(bias), rep, pres, freq));
+        if ((c & BIASED_AGAIN) && !sum_of_biases(p, b0, b1, e, id, bias)) continue;
+        store_f32(y + id, adjust(load_f32(x + id), c, bias, rep, pres, freq));
     }
 }
 
-template <class TX, class TY>
-int launch_logits_two(LogitsParams p, cudaStream_t st)
+template <class TX, class TY, bool NARROW, int THREADS>
+int launch_logits(LogitsParams p, cudaStream_t st)
 {
-    constexpr int SLICE = 512 * 8 * MASK_GROUPS<TX>;
+    // Windows: as many as fill every SM at a time, of 2048 tokens at least, and of what 64 KB of counts hold at most.
+    constexpr int MOST = NARROW ? 32768 : 16384;
+    const long long room = (148ll * (THREADS == 512 ? 3 : 1) + p.rows - 1) / p.rows;
+    long long window = ((long long)p.vocab + room - 1) / room;
+    window = window < 2048 ? 2048 : window > MOST ? MOST : window;
+    p.window = (int)((window + 255) / 256 * 256);
+    // (a row that does not start on a 16-byte boundary of x or y has a part of a group in front)
     const bool even = aligned(p.x, 16) && aligned(p.y, 16) && p.x_ld % 8 == 0 && p.y_ld % 8 == 0;
-    p.slices = (int)(((long long)p.vocab + (even ? 0 : 8) + SLICE - 1) / SLICE);
-    const long long pieces = (long long)p.slices * p.rows, windows = ((long long)p.vocab + LOGITS_WINDOW - 1) / LOGITS_WINDOW * p.rows;
-    if (windows > 0x7fffffffll) return refuse("%d rows of %d are too many for one call", p.rows, p.vocab);
-    constexpr int SMEM = LOGITS_WINDOW * 6;
-    const bool rewrite = p.history || p.bias_begin;
-    if (rewrite) {
-        int rc = ask_for_shared(logits_said_kernel<TX, TY>, SMEM);
-        if (rc == 0) rc = ask_for_shared(logits_mask_kernel<TX, TY>, 0);
-        if (rc != 0) return rc;
-    }
-    launch_dependent(logits_mask_kernel<TX, TY>, dim3((unsigned)(pieces < 148 * 2 ? pieces : 148 * 2)), 512, 0, st, p);
-    const int rc = launched();
-    if (rc != 0 || !rewrite) return rc;
-    launch_dependent(logits_said_kernel<TX, TY>, dim3((unsigned)windows), 1024, SMEM, st, p);
+    p.windows = (int)(((long long)p.vocab + (even ? 0 : 8) + p.window - 1) / p.window);
+    const long long ctas = (long long)p.windows * p.rows;
+    if (ctas > 0x7fffffffll) return refuse("%d rows of %d are too many for one call", p.rows, p.vocab);
+    // warps that count before they write: half, or all where the history is longer than twice the window
+    p.counting_warps = !p.history && !p.bias_begin ? 0 : p.history && p.history_ld > 2ll * p.window ? THREADS / 32 : THREADS / 64;
+    const int listed = (int)(p.history_ld < p.window ? p.history_ld : p.window);       // more different tokens were not said
+    const int rc = ask_for_shared(logits_kernel<TX, TY, NARROW, THREADS>, MOST * ((NARROW ? 2 : 4) + 2));
+    if (rc != 0) return rc;
+    launch_dependent(logits_kernel<TX, TY, NARROW, THREADS>, dim3((unsigned)ctas), THREADS, p.window * (NARROW ? 2 : 4) + listed * 2, st, p);
     return launched();
 }
 
 template <class TX, class TY>
 int launch_logits_sized(const LogitsParams &p, cudaStream_t st)
 {
-    // slices of 2048 that do not give every SM more than four, and a history that each of them can go through
-    if ((long long)p.rows * p.vocab <= 148ll * 4 * 2048 && (!p.history || p.history_ld <= 8192)) return launch_logits<TX, TY>(p, st);
-    return launch_logits_two<TX, TY>(p, st);
+    // every window goes through the whole history: a long one has few windows, of more threads
+    if (p.history_ld < 8192) return launch_logits<TX, TY, true, 512>(p, st);
+    return launch_logits<TX, TY, false, 1024>(p, st);
 }
 
 template <class TX>
@@ -860,7 +696,7 @@ int gemm_logits(const GemmLogitsArgs *a)
         if (!aligned(w, 4)) return refuse("history, penalties, biases and mask must be 4-byte aligned");
     LogitsParams p = {};
     p.x = a->x; p.y = a->y; p.x_ld = a->x_ld; p.y_ld = a->y_ld;
-    p.history = a->history; p.history_ld = a->history_ld; p.history_len = a->history_len; p.prompt_len = a->prompt_len;
+    p.history = a->history; p.history_ld = a->history ? a->history_ld : 0; p.history_len = a->history_len; p.prompt_len = a->prompt_len;
     p.repetition = a->repetition; p.presence = a->presence; p.frequency = a->frequency;
     p.bias_ids = a->bias_ids; p.bias_values = a->bias_values; p.bias_begin = a->bias_begin;
     p.mask = a->mask; p.mask_ld = a->mask_ld;
