@@ -26,10 +26,17 @@
 // |x| is below 2^19 and some |x| of each row above 2^-40, else by row from its largest value.
 // Scales belong to (row, group) and are applied to the FP32 sums of a group, GPU = 1, 2 or 4 groups per unit.
 //
-// Work: CTA i takes the i-th share of the tiles of 16 rows, whole tiles (a part of a tile costs what a tile costs: shares of
-// exactly N / grid rows, the same bytes for every SM, took 27.3 us against 26.1 at 1 x 28672 x 8192).  Its 16 warps are WR groups over the tiles times WK slices over K in batches of two units; the WK
-// partial sums of a tile meet in shared memory and are added in the order of the slices -- no atomics, the same result
-// every run.  X is staged whole when it fits, else in passes over K with the partial sums kept.
+// Work: a cluster of 1, 2 or 4 CTAs takes its share of the tiles, whole tiles (a part of a tile costs what a tile costs: shares
+// of exactly N / grid rows, the same bytes for every SM, took 27.3 us against 26.1 at 1 x 28672 x 8192), and each of its CTAs a
+// part of K.  A CTA's warps (16; 8 for more than 8 rows of X, whose tiles are 32 rows) are WR groups over the tiles times WK
+// slices over its K in batches of two units.  The partial sums of a block of tiles meet in shared memory and are added, across
+// the cluster too, in the order of CTAs and slices -- no atomics, the same result every run.  X is staged whole when it fits,
+// else in passes over K with the partial sums kept.
+//
+// Measured (us, device time of back-to-back calls, weights from HBM; groups of 128, bf16): 28672 x 8192 by 1 / 4 / 8 / 9 / 16 rows
+// 26.7 / 29.5 / 30.5 / 39.7 / 51; 4096 x 14336 12.4 / 13.5 / 15.0 / 18.1 / 19.7; 8192 x 28672 31.2 / 31.5 / 32.9 / 47 / 56.
+// One row is bound by the bytes (slope 6.3 TB/s) and 5 us of start, staging and end; 16 rows by the tensor and logic
+// instructions that two warps per scheduler issue (the tcgen05 tiles of the bk128 plugins take 46, 19.4 and 46 us for any M).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -41,6 +48,7 @@ namespace sm100 {
 struct W4MatvecParams {
     int M, N, K;
     int group_shift;             // log2(group size)
+    int groups, zero_pitch;      // scales and bytes of zero points per row of W
     const void *X;               // [M][K]
     const uint8_t *W;            // [N][K/2]
     const void *scales;          // [N][K/G]
@@ -53,7 +61,7 @@ struct W4MatvecParams {
     int block_rows;              // rows of W whose partial sums shared memory holds
     int units_per_pass;          // units (128 K-elements) of X that shared memory holds
     int wk_shift;                // log2(WK)
-    int ring;                    // batches in flight per warp
+    int cluster;                 // CTAs that share tiles, each a part of K
     int part_at;                 // partial sums: byte offset in shared memory
     int scale_window, zero_window;       // scales / zero points reach the ring in words around them, else they are read when needed
     const uint8_t *scales_end, *zeros_end;
@@ -113,14 +121,14 @@ struct W4MatvecTraits {
     // tile is 32 rows of W, so that what is read of X is used twice; that takes the registers of 8 warps.
     static constexpr int SUBTILES = NB, TILE = 16 * SUBTILES, UNIT = 128;
     static constexpr int WARPS = NB == 1 ? 16 : 8, THREADS = 32 * WARPS;
-    static constexpr int MOST_RING = 3;              // batches of two units in flight per warp: 3, or 2 where X needs the room
+    static constexpr int RING = 2;                   // batches of two units in flight per warp (3 were no faster: X needs the room)
     static constexpr int UNIT_BYTES = TILE * UNIT / 2;
     static constexpr int AHEAD_ROWS = 32;            // rows of W asked into L2 before the grid before has ended
     // a batch in the ring: two units, then per row the scales of its 2 GPU groups and a word in front of them, then per row
     // two words around its zero points
     static __host__ __device__ constexpr int scale_pitch(int gpu) { return 8 * gpu; }
     static __host__ __device__ constexpr int slot_bytes(int gpu) { return 2 * UNIT_BYTES + TILE * scale_pitch(gpu) + TILE * 8; }
-    static __host__ __device__ constexpr int ring_bytes(int gpu, int ring) { return WARPS * ring * slot_bytes(gpu); }
+    static __host__ __device__ constexpr int ring_bytes(int gpu) { return WARPS * RING * slot_bytes(gpu); }
     static constexpr int ROW_BYTES = 256;            // per row of X: scaling, flags
     static constexpr int SMEM_ALLOC = 227 * 1024;    // ring, flags, staged X and its sums, partial sums
     // staged X: rows 64 bytes longer than their units, so that the eight lanes of a 16-byte access (two rows) reach all banks
@@ -191,6 +199,30 @@ __device__ __forceinline__ uint32_t w4_keep(uint32_t v)
 {
     asm volatile("" : "+r"(v));
     return v;
+}
+
+// this CTA's rank in its cluster; a float of CTA `rank`'s shared memory; a barrier over the cluster's CTAs
+__device__ __forceinline__ int w4_cluster_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return (int)r;
+}
+__device__ __forceinline__ uint32_t w4_shared_of(uint32_t addr, int rank)
+{
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float w4_load_cluster(uint32_t addr)
+{
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void w4_cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 __device__ __forceinline__ float w4_power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }      // -126 <= e <= 127
@@ -333,8 +365,8 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
     constexpr int GROUP_SUBS = 4 / GPU;                  // pieces of 32 k in a group
     constexpr int STEPS = GPU == 1 ? 2 : 4, SUBS = 8 / STEPS, GROUPS = 2 * GPU / STEPS;      // steps of a batch, pieces and groups of a step
     constexpr int SLOT = T::slot_bytes(GPU), SCALES_AT = 2 * T::UNIT_BYTES, SCALE_PITCH = T::scale_pitch(GPU), ZEROS_AT = SCALES_AT + TILE * SCALE_PITCH;
-    const int ring_slots = p.ring;
-    const uint32_t X_AT = T::ring_bytes(GPU, ring_slots) + T::ROW_BYTES;
+    constexpr int RING_BYTES = T::RING * SLOT;           // of a warp
+    constexpr uint32_t X_AT = T::ring_bytes(GPU) + T::ROW_BYTES;
     extern __shared__ __align__(16) uint8_t smem[];
     float *part = reinterpret_cast<float *>(smem + p.part_at);      // [WK][M][block_rows]
     W4Rows *xrows = reinterpret_cast<W4Rows *>(smem + X_AT - T::ROW_BYTES);
@@ -344,20 +376,24 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
     const int WK = 1 << p.wk_shift, WR = WARPS >> p.wk_shift;
     const int wk = warp & (WK - 1), wr = warp >> p.wk_shift;
     const int M = p.M, K = p.K;
-    const int groups = K >> p.group_shift;
-    const int zero_pitch = (groups + 1) >> 1;
-    const int units = (K + T::UNIT - 1) / T::UNIT;
+    const int groups = p.groups, zero_pitch = p.zero_pitch;
+    // this CTA's part of K, whole batches, and its cluster's share of the tiles
+    const int cluster = p.cluster, rank = w4_cluster_rank();
+    const int all_batches = (K + 2 * T::UNIT - 1) / (2 * T::UNIT);
+    const int unit_begin = (int)((long long)all_batches * rank / cluster) * 2;
+    const int unit_end = min((int)((long long)all_batches * (rank + 1) / cluster) * 2, (K + T::UNIT - 1) / T::UNIT);
     const uint32_t row_bytes = (uint32_t)K >> 1;
     const uint32_t sums_at = X_AT + M * T::x_row_bytes(p.units_per_pass);
     const long long all_tiles = (p.N + T::TILE - 1) / T::TILE;
-    const int row_begin = (int)(all_tiles * blockIdx.x / gridDim.x) * T::TILE, row_end = min((int)(all_tiles * (blockIdx.x + 1) / gridDim.x) * T::TILE, p.N);
+    const int share = blockIdx.x / cluster, shares = gridDim.x / cluster;
+    const int row_begin = (int)(all_tiles * share / shares) * T::TILE, row_end = min((int)(all_tiles * (share + 1) / shares) * T::TILE, p.N);
     const uint8_t *scales = static_cast<const uint8_t *>(p.scales);
     const uint32_t step_batch = WK * T::UNIT, step_w = WR * TILE * row_bytes, step_s = WR * TILE * groups * 2, step_z = WR * TILE * zero_pitch;      // K <= 2^24
 
     // The ring holds a unit as TILE rows of four 16-byte pieces; piece j of row r lies at (r, j ^ (r / 2 % 4)), so that the
     // eight rows of a matrix reach all banks.  Copies: lane (g, c) brings piece c of rows g, g + 8, ...  ldmatrix: lane l
     // names row l % 16 and piece l / 16 (then 2 more) of the four matrices (rows 0-7, 8-15) x (piece j, j + 1).
-    const uint32_t ring = smem_u32(smem) + warp * (ring_slots * SLOT);
+    const uint32_t ring = smem_u32(smem) + warp * RING_BYTES;
     const uint32_t put_at = g * 64 + ((c ^ (g >> 1 & 3)) << 4);
     const uint32_t get_at = (lane & 15) * 64 + (((lane >> 4) ^ (lane >> 1 & 3)) << 4);
     const uint32_t flip_lo = ZERO ? 0u : w4_keep(0x00080008u), flip_hi = ZERO ? 0u : w4_keep(0x00800080u);
@@ -369,15 +405,17 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
     // Launched as a programmatic dependent: up to here, and for this hint, the grid before may still be running.  The first
     // tiles are asked into L2 meanwhile (no data is read: what that grid still writes is seen all the same).
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (lane == 0)
-        for (int r = warp; r < T::AHEAD_ROWS && row_begin + r < row_end; r += WARPS) w4_prefetch(p.W + (size_t)(row_begin + r) * row_bytes, row_bytes);
+    if (lane == 0) {
+        const uint32_t ahead_at = unit_begin * (T::UNIT / 2), ahead = min(unit_end * (T::UNIT / 2), row_bytes) - ahead_at;
+        for (int r = warp; r < T::AHEAD_ROWS * cluster && row_begin + r < row_end; r += WARPS) w4_prefetch(p.W + (size_t)(row_begin + r) * row_bytes + ahead_at, ahead);
+    }
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
     for (int row0 = row_begin; row0 < row_end; row0 += p.block_rows) {
         const int rows = min(p.block_rows, row_end - row0);
         const int tiles = (rows + TILE - 1) / TILE;
-        for (int u0 = 0; u0 < units; u0 += p.units_per_pass) {
-            const int nu = min(p.units_per_pass, units - u0);       // units of this pass
+        for (int u0 = unit_begin; u0 < unit_end; u0 += p.units_per_pass) {
+            const int nu = min(p.units_per_pass, unit_end - u0);       // units of this pass
             const int batches = (nu + 1) >> 1;
             // A warp's share of the pass: of every WR-th tile every WK-th batch.
             // the batch that ends behind K, if one does: its missing pieces are zeros
@@ -457,19 +495,18 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
             if (wk >= batches) ld_tile = tiles;              // (a last pass of fewer batches than slices)
             int tile = ld_tile, batch = wk;                                 // computing side
             // X is staged while the first weights are on their way; the pass before has to be through with its own
-            const bool stage = units > p.units_per_pass || row0 == row_begin;
+            const bool stage = unit_end - unit_begin > p.units_per_pass || row0 == row_begin;
             if (stage) {
-                if (u0 != 0 || row0 != row_begin) __syncthreads();
+                if (u0 != unit_begin || row0 != row_begin) __syncthreads();
                 if (threadIdx.x < 16) {
                     xrows->ordinary[threadIdx.x] = 0;
                     xrows->down[threadIdx.x] = 1.f;
                 }
                 w4_copy_x<WARPS, T>(p, smem_u32(smem + X_AT), u0, 2 * batches, warp, lane);
             }
-            for (int d = 0; d < ring_slots; d++) load(d * SLOT);
+            for (int d = 0; d < T::RING; d++) load(d * SLOT);
             if (stage) {
-                if (ring_slots == 3) w4_copies_wait<3>();    // this thread's pieces of X
-                else w4_copies_wait<2>();
+                w4_copies_wait<T::RING>();           // this thread's pieces of X
                 __syncthreads();                     // the flags
 #pragma unroll 1
                 for (bool usual = true;; usual = false) {
@@ -494,30 +531,31 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
                     for (int i = 0; i < 4; i++) total[t][nb][i] = 0.f;
             // A STEP is the part of a batch whose sums are kept apart: a unit (GPU = 1), else half a unit, GPU / 2 groups.
             // scales of a step for row `row` of the tile, row ra of W: GROUPS times 16 bits
-            auto scales_of = [&](const uint8_t *slot, int row, size_t ra, int step) -> uint32_t {
+            auto scales_of = [&](const uint8_t *slot, int row, int ra, int step) -> uint32_t {
                 const int first = (u0 + 2 * batch) * GPU + step * GROUPS;          // the step's first group
                 if constexpr (WHOLE) {
                     const uint8_t *at = slot + SCALES_AT + row * SCALE_PITCH + step * (2 * GROUPS);
                     return GROUPS == 1 ? *reinterpret_cast<const uint16_t *>(at) : *reinterpret_cast<const uint32_t *>(at);
                 } else {
                     // (the window starts with the word that holds the batch's first scale; the array is 4-byte aligned)
-                    const uint16_t *at = p.scale_window ? reinterpret_cast<const uint16_t *>(slot + SCALES_AT + row * SCALE_PITCH + (ra * groups & 1) * 2) + step * GROUPS
-                                                        : reinterpret_cast<const uint16_t *>(scales) + ra * groups + first;
+                    const uint16_t *at = p.scale_window ? reinterpret_cast<const uint16_t *>(slot + SCALES_AT + row * SCALE_PITCH + (ra & groups & 1) * 2) + step * GROUPS
+                                                        : reinterpret_cast<const uint16_t *>(scales) + (size_t)ra * groups + first;
                     uint32_t v = first < groups ? at[0] : 0u;
                     if (GROUPS == 2 && first + 1 < groups) v |= (uint32_t)at[1] << 16;
                     return v;
                 }
             };
             // zero points of a step: GROUPS nibbles
-            auto zeros_of = [&](const uint8_t *slot, int row, size_t ra, int step) -> uint32_t {
+            auto zeros_of = [&](const uint8_t *slot, int row, int ra, int step) -> uint32_t {
                 if constexpr (WHOLE && GPU == 4) {
                     return slot[ZEROS_AT + row * 8 + step];
                 } else {
                     // byte of the batch's first group; its low bits say where the window starts
-                    const size_t z = ra * zero_pitch + (size_t)(u0 + 2 * batch) * GPU / 2;
+                    const int in_row = (u0 + 2 * batch) * GPU / 2;
+                    const uint32_t low = ra * (uint32_t)zero_pitch + in_row;
                     const int first = (u0 + 2 * batch) * GPU + step * GROUPS;
                     if (!WHOLE && !p.zero_window && first >= groups) return 0;     // (in the window are zeros or bytes of the array)
-                    const uint8_t *at = WHOLE || p.zero_window ? slot + ZEROS_AT + row * 8 + (z & 3) : p.zeros + z;
+                    const uint8_t *at = WHOLE || p.zero_window ? slot + ZEROS_AT + row * 8 + (low & 3) : p.zeros + (size_t)ra * zero_pitch + in_row;
                     return GROUPS == 2 ? at[step] : at[step >> 1] >> (4 * (step & 1));
                 }
             };
@@ -526,7 +564,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
 #pragma unroll
                 for (int t = 0; t < SUBTILES; t++) {
                     const int r = t * 16 + g;
-                    const size_t ra = row0 + min(tile * TILE + r, rows - 1), rb = row0 + min(tile * TILE + r + 8, rows - 1);
+                    const int ra = row0 + min(tile * TILE + r, rows - 1), rb = row0 + min(tile * TILE + r + 8, rows - 1);
                     sa[t] = scales_of(slot, r, ra, step);
                     sb[t] = scales_of(slot, r + 8, rb, step);
                     za[t] = ZERO ? zeros_of(slot, r, ra, step) : 0;
@@ -597,16 +635,15 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
             };
             uint32_t slot = 0;
             while (tile < tiles) {
-                if (ring_slots == 3) w4_copies_wait<2>();
-                else w4_copies_wait<1>();
+                w4_copies_wait<T::RING - 1>();
                 __syncwarp();                            // the other lanes' copies too
                 // one step after the other where the registers are short
                 constexpr int UNROLL = GPU == 1 && NB == 1 ? 2 : 1;
 #pragma unroll UNROLL
-                for (int step = 0; step < STEPS; step++) compute(smem + warp * (ring_slots * SLOT) + slot, ring + slot + get_at, step);
+                for (int step = 0; step < STEPS; step++) compute(smem + warp * RING_BYTES + slot, ring + slot + get_at, step);
                 __syncwarp();                            // every lane has read the slot
                 load(slot);
-                slot = slot == (ring_slots - 1) * SLOT ? 0 : slot + SLOT;
+                slot = slot == (T::RING - 1) * SLOT ? 0 : slot + SLOT;
                 batch += WK;
                 if (batch >= batches) {
                     // the warp's share of this tile is complete: its partial sums go to its own slot
@@ -621,7 +658,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
 #pragma unroll
                                 for (int k = 0; k < 2 * SUBTILES; k++) {
                                     const float v = total[k / 2][nb][2 * (k % 2) + i] * W4Type<E>::OUT * out;
-                                    to[8 * k] = u0 == 0 ? v : to[8 * k] + v;
+                                    to[8 * k] = u0 == unit_begin ? v : to[8 * k] + v;
                                 }
                             }
 #pragma unroll
@@ -633,14 +670,23 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
             }
             w4_copies_wait<0>();
         }
-        __syncthreads();
-        for (int i = threadIdx.x; i < rows * M; i += THREADS) {
+        // every CTA of the cluster adds up a part of the results: the slices of the first, of the second ...
+        const uint32_t part_addr = smem_u32(part), slice = M * p.block_rows * sizeof(float);
+        if (cluster > 1) w4_cluster_sync();
+        else __syncthreads();
+        for (int i = w4_cluster_rank() * THREADS + threadIdx.x; i < rows * M; i += cluster * THREADS) {
             const int m = i / rows, r = i - m * rows;
             float v = 0.f;
-            for (int w = 0; w < WK; w++) v += part[((size_t)w * M + m) * p.block_rows + r];
+            for (int j = 0; j < cluster; j++) {
+                uint32_t from = part_addr + (m * p.block_rows + r) * sizeof(float);
+                if (cluster > 1) from = w4_shared_of(from, j);
+#pragma unroll 4
+                for (int w = 0; w < WK; w++, from += slice) v += w4_load_cluster(from);
+            }
             w4_store<E, T::EPI>(p, m, row0 + r, v);
         }
-        __syncthreads();
+        if (cluster > 1) w4_cluster_sync();
+        else __syncthreads();
     }
 }
 
@@ -668,6 +714,8 @@ struct W4MatvecLauncher {
         W4MatvecParams p;
         p.M = a.M; p.N = a.N; p.K = a.K;
         p.group_shift = a.group_size == 32 ? 5 : a.group_size == 64 ? 6 : 7;
+        p.groups = a.K / a.group_size;
+        p.zero_pitch = (p.groups + 1) / 2;
         p.X = a.X;
         p.W = static_cast<const uint8_t *>(a.W);
         p.scales = a.w_scale;
@@ -681,37 +729,49 @@ struct W4MatvecLauncher {
         int sms = 0;
         int rc = sm_count(&sms);
         if (rc != GEMM_OK) return rc;
-        int grid = a.sm_limit > 0 && a.sm_limit < sms ? a.sm_limit : sms;
-        const int all_tiles = (a.N + T::TILE - 1) / T::TILE;
-        if (grid > all_tiles) grid = all_tiles;
-        const int gpu = T::UNIT >> p.group_shift, rows = (all_tiles + grid - 1) / grid * T::TILE, units = (a.K + T::UNIT - 1) / T::UNIT;
+        const int most_ctas = a.sm_limit > 0 && a.sm_limit < sms ? a.sm_limit : sms;
+        const int all_tiles = (a.N + T::TILE - 1) / T::TILE, all_batches = (a.K + 2 * T::UNIT - 1) / (2 * T::UNIT);
+        const int gpu = T::UNIT >> p.group_shift;
         // how scales and zero points come: with whole batches, else in words around them (base 4-byte aligned), else one by one
         // when they are needed
         const bool whole = a.K % (2 * T::UNIT) == 0 && bits(a.w_scale) % (4 * gpu) == 0 && bits(a.w_zero) % 4 == 0;
         p.scale_window = bits(a.w_scale) % 4 == 0;
         p.zero_window = bits(a.w_zero) % 4 == 0;
-        // The plan: WK slices of K leave WARPS / WK groups for the tiles, and WK partial sums of every result in shared memory,
-        // which the ring and X share (what does not fit of X goes in passes).  The one with the fewest rounds of batches is
-        // taken, counting a pass as 8 of them (its staging) and a ring of 2 batches instead of 3 as an eighth more; of equals
-        // the longest ring and the largest WK (a tile's bytes then arrive soonest).
+        // The plan.  A cluster of 1, 2 or 4 CTAs shares tiles, each CTA a part of K: every SM then stages a half or a quarter of
+        // X, which is what many rows and a long K cost most (us, clusters of 1 / 2 / 4: 16 x 4096 x 14336 37 / 26.6 / 20;
+        // 8 x 28672 x 8192 35.9 / 30.2 / 34.4), and adds the partial sums across the cluster (1 x 4096 x 4096 5.9 / 6.8; 4 of the
+        // 148 SMs cannot be in 37 clusters of 4, only 33 fit).  Then WK slices of the CTA's K leave WARPS / WK groups for the
+        // tiles, and WK partial sums of every result in shared memory, beside the ring and X (what does not fit of X goes in
+        // passes).  Costs are in eighths of the time of a round (a batch by every warp, ~1 us): 24 and WK per CTA for the sums
+        // of a block, 16 and 1 for 16 rows of a unit to stage X, 12 and 32 for clusters of 2 and 4.  Over 68 shapes and sizes
+        // that picks a plan 2 % (at most 8 %) behind the best of all.  Of equals the largest WK: a tile's bytes arrive soonest.
+        int clusters[2];
+        rc = clusters_at_once(clusters);
+        if (rc != GEMM_OK) return rc;
         long long best = -1;
-        for (int ring = T::MOST_RING; ring >= 2; ring--) {
-            const int fixed = T::ring_bytes(gpu, ring) + T::ROW_BYTES;
+        int grid = 0;
+        const int fixed = T::ring_bytes(gpu) + T::ROW_BYTES;
+        for (int cluster_shift = 0; cluster_shift <= 2; cluster_shift++) {
+            const int cluster = 1 << cluster_shift, shares = std::min(cluster == 1 ? most_ctas : std::min(most_ctas / cluster, clusters[cluster_shift - 1]), all_tiles);
+            if (shares == 0) continue;
+            const int rows = (all_tiles + shares - 1) / shares * T::TILE, units = (all_batches + cluster - 1) / cluster * 2;
             for (int shift = T::WARPS == 16 ? 4 : 3; shift >= 0; shift--) {
                 const int wk = 1 << shift, per_tile = wk * a.M * T::TILE * (int)sizeof(float);
                 const int most_rows = (T::SMEM_ALLOC - fixed) / 2 / per_tile * T::TILE;       // at most half of the rest
-                if (most_rows == 0) continue;
+                if (most_rows == 0 || wk > std::max(all_batches / cluster, 1)) continue;
                 const int blocks = (rows + most_rows - 1) / most_rows, block_rows = ((rows + blocks - 1) / blocks + T::TILE - 1) / T::TILE * T::TILE;
                 const int part_bytes = block_rows / T::TILE * per_tile;
                 const int most_units = (T::SMEM_ALLOC - fixed - part_bytes - a.M * 64) / (a.M * T::UNIT * 2 + gpu * T::NB * 32) / 2 * 2;
                 const int passes = (units + most_units - 1) / most_units, per_pass = ((units + passes - 1) / passes + 1) / 2 * 2;
-                if (per_pass < 2 * wk && wk > 1) continue;
+                if (per_pass < 2 * wk) continue;         // every slice has a part of the first pass
                 const int groups_of_tiles = T::WARPS / wk, tiles = block_rows / T::TILE;
                 const long long rounds = (long long)((tiles + groups_of_tiles - 1) / groups_of_tiles) * ((per_pass / 2 + wk - 1) / wk);
-                const long long cost = (long long)blocks * passes * (rounds * (11 - ring) + 8 * 8);
+                const long long stagings = passes > 1 ? (long long)blocks * passes : 1;
+                const long long cost = blocks * (passes * rounds * 8 + 24 + wk * cluster) + stagings * (16 + a.M * per_pass / 16) + (cluster == 1 ? 0 : cluster == 2 ? 12 : 32);
                 if (best >= 0 && cost >= best) continue;
                 best = cost;
-                p.ring = ring;
+                grid = shares * cluster;
+                p.cluster = cluster;
                 p.wk_shift = shift;
                 p.block_rows = block_rows;
                 p.units_per_pass = per_pass;
@@ -719,9 +779,8 @@ struct W4MatvecLauncher {
             }
         }
         const int smem = p.part_at + p.block_rows * a.M * (int)sizeof(float) * (1 << p.wk_shift);
-        const size_t groups = (size_t)a.K / a.group_size;
-        p.scales_end = static_cast<const uint8_t *>(a.w_scale) + (size_t)a.N * groups * 2;
-        p.zeros_end = a.w_zero ? p.zeros + (size_t)a.N * ((groups + 1) / 2) : nullptr;
+        p.scales_end = static_cast<const uint8_t *>(a.w_scale) + (size_t)a.N * p.groups * 2;
+        p.zeros_end = a.w_zero ? p.zeros + (size_t)a.N * p.zero_pitch : nullptr;
         if (a.x_dtype == GEMM_X_F16) return launch<__half>(p, whole, grid, smem, a.stream);
         return launch<__nv_bfloat16>(p, whole, grid, smem, a.stream);
     }
@@ -740,6 +799,41 @@ private:
         }
         *out = n;
         return GEMM_OK;
+    }
+
+    // how many clusters of 2 and of 4 CTAs, each with an SM of its own, the device runs side by side
+    static int clusters_at_once(int (&out)[2])
+    {
+        static std::atomic<int> counts[MAX_DEVICES][2];          // 1 more than the count: 0 is unknown
+        int dev = 0;
+        SM100_CUDA_TRY(cudaGetDevice(&dev));
+        if (dev < 0 || dev >= MAX_DEVICES) return set_error(GEMM_ERR_ARG, "device ordinal %d out of range", dev);
+        for (int i = 0; i < 2; i++) {
+            int n = counts[dev][i].load(std::memory_order_relaxed) - 1;
+            if (n < 0) {
+                auto *kernel = w4_matvec_kernel<__nv_bfloat16, 1, false, true, T>;
+                SM100_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::SMEM_ALLOC));
+                cudaLaunchAttribute attr = cluster_attribute(2 << i);
+                cudaLaunchConfig_t cfg = {};
+                cfg.gridDim = dim3(2 << i);
+                cfg.blockDim = dim3(T::THREADS);
+                cfg.dynamicSmemBytes = T::SMEM_ALLOC;
+                cfg.attrs = &attr;
+                cfg.numAttrs = 1;
+                SM100_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+                counts[dev][i].store(n + 1, std::memory_order_relaxed);
+            }
+            out[i] = n;
+        }
+        return GEMM_OK;
+    }
+    static cudaLaunchAttribute cluster_attribute(int ctas)
+    {
+        cudaLaunchAttribute a;
+        a.id = cudaLaunchAttributeClusterDimension;
+        a.val.clusterDim.x = ctas;
+        a.val.clusterDim.y = a.val.clusterDim.z = 1;
+        return a;
     }
 
     template <class E>
@@ -768,6 +862,9 @@ private:
         }
         cudaLaunchConfig_t cfg = dependent_launch_config(grid, T::THREADS, stream);
         cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attrs[2] = {cfg.attrs[0], cluster_attribute(p.cluster)};
+        cfg.attrs = attrs;
+        cfg.numAttrs = 2;
         SM100_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, p));
         return GEMM_OK;
     }

@@ -111,6 +111,77 @@ def test_matvec_long(registry, cuda_device, shape, zeros):
             check_matvec(matvec(matvec_plugin(registry, rows), X, W, sc, zp, group), X, Wd, group)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("shape", [(16, 2000, 14336 + 32, 32), (12, 31, 9 * 256 + 64, 64), (16, 301, 65536 - 128, 128), (8, 4000, 28672, 128), (9, 130, 3 * 256, 32), (4, 100, 5 * 256 + 96, 32),
+                                   (16, 16, 1 << 17, 128), (2, 5000, 1000 * 32, 32)])
+def test_matvec_shared_tiles(registry, cuda_device, shape, dtype):
+    """Sizes at which several SMs take a part of K each: parts of unequal length, cut batches, passes within a part; and the
+    same with few SMs, down to fewer than would share a tile."""
+    m, n, k, group = shape
+    W, sc, zp, Wd = w4_weights(n, k, group, T[dtype], True, seed=5)
+    X = torch.randn((m, k), device="cuda", generator=torch.Generator(device="cuda").manual_seed(6)).to(T[dtype])
+    C = torch.randn((m, n), device="cuda", generator=torch.Generator(device="cuda").manual_seed(7)).to(T[dtype])
+    for rows in (8, 16):
+        if m > rows:
+            continue
+        for limit in (0, 1, 2, 3, 6, 75):
+            Y = matvec(matvec_plugin(registry, rows), X, W, sc, zp, group, sm_limit=limit)
+            check_matvec(Y, X, Wd, group)
+        assert torch.equal(Y, matvec(matvec_plugin(registry, rows), X, W, sc, zp, group, sm_limit=75))
+        Y = matvec(matvec_plugin(registry, rows, 2), X, W, sc, zp, group, beta=1.0, C=C)
+        ref = X.double() @ Wd.t() + C.double()
+        tol = matvec_bound(X, Wd, group) + 2.0 ** -22 * (ref.abs() + C.double().abs()) + half_step(Y.dtype) * ref.abs() + tiny(Y.dtype)
+        assert ((Y.double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("shape", [(8, 100, 1024, 128), (8, 77, 1024 + 96, 32), (16, 300, 14336, 64), (16, 33, 65536, 128), (7, 200, 28672, 128)])
+def test_matvec_range(registry, cuda_device, shape, zeros):
+    """bf16 rows of X far from 1, which are staged by a scaling of their own: huge, tiny, subnormal, zero, mixed, some of them
+    only in one part of K; a row with an infinity or a NaN is NaN and leaves the others alone."""
+    m, n, k, group = shape
+    W, sc, zp, Wd = w4_weights(n, k, group, torch.bfloat16, zeros, seed=11)
+    base = torch.randn((m, k), device="cuda", generator=torch.Generator(device="cuda").manual_seed(12))
+    # u + z times the scale: what the sums of u * x and of z * x are made of, each rounded as the bound below says
+    u = torch.stack([W & 15, W >> 4], 2).view(n, -1, group).double()
+    if not zeros:
+        u = (u + 8) % 16
+    z = torch.stack([zp & 15, zp >> 4], 2).view(n, -1)[:, :k // group, None].double() if zeros else 8.0
+    parts = ((u + z) * sc.double()[:, :, None]).view(n, k)
+    for variant in range(4):
+        X = base.clone()
+        if variant == 0:
+            X[0] *= 2.0 ** 100
+            X[1] *= 2.0 ** -100
+            X[2] = 0
+            X[3] *= 2.0 ** -126                          # half of them subnormal
+            X[4, ::7] *= 2.0 ** 60
+        elif variant == 1:
+            X[:, k // 2:] *= 2.0 ** 30                   # every row, a later part of K only
+        elif variant == 2:
+            X[:, : k - 32] *= 2.0 ** -60                 # nothing ordinary in front of the last 32
+            X[5] = 0
+            X[5, 3] = 2.0 ** 110
+        else:
+            X[1, 17] = float("inf")
+            X[2, k - 1] = float("nan")
+            X[3, k // 3] = float("-inf")
+            X[4] *= 2.0 ** 40
+        X = X.bfloat16()
+        for rows in (8, 16):
+            if m > rows:
+                continue
+            Y = matvec(matvec_plugin(registry, rows), X, W, sc, zp, group)
+            good = [i for i in range(m) if variant < 3 or i not in (1, 2, 3)]
+            ref = X[good].double() @ Wd.t()
+            # a staged x may lose what is 2^-126 / 2^119 of its row's largest, far below FP32's share of it
+            tol = (k / 128 + 64) * 2.0 ** -22 * (X[good].double().abs() @ parts.t()) + half_step(Y.dtype) * ref.abs() + tiny(torch.bfloat16)
+            worst = ((Y[good].double() - ref).abs() / tol).max().item()
+            assert worst <= 1, (variant, rows, worst)
+            for i in set(range(m)) - set(good):
+                assert Y[i].isnan().all()
+
+
 def test_matvec_exact_integers(registry, cuda_device):
     """Small integers: every partial sum is exact in FP32, so the result is, whatever the order; 2^8 bounds it for bf16."""
     n, k = 77, 640
