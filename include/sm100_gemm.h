@@ -136,12 +136,14 @@ enum { GEMM_Y_BF16 = 0, GEMM_Y_E4M3 = 1 };
  * padded to a multiple of 128.  libsm100gemm_util.so converts a row-major [rows][K/32] array
  * into this layout (include/sm100_gemm_util.h).  Weights are converted once; K must be a multiple of 128 (MXFP8) / 256 (W4A4).
  *
- * Matrix-vector plugins (`w4a16_bm128_bn<8|16>_bk32_...`): 1 <= M <= bn rows of X against int4 weights, any N >= 1, K a
- * multiple of group_size (32, 64 or 128); X bf16 or fp16 (x_dtype), scales [N][K/group_size] of the same type, signed
+ * Matrix-vector plugins (`w4a16_bm128_bn<8|16>_bk32_...`): 1 <= M <= bn rows of X against int4 weights, N <= 2^30, K <= 2^24
+ * a multiple of group_size (32, 64 or 128); X bf16 or fp16 (x_dtype), scales [N][K/group_size] of the same type, signed
  * weights or zero points (w_zero).  X and W 16-byte aligned, every other pointer aligned to its elements.  They use no
  * workspace (gemm_workspace_bytes reports the family's figure, so that one workspace serves every W4A16 plugin) and the
  * first call may be made under stream capture.  `_e2`: with the output transform, in the type of X; y_dtype must be
- * GEMM_Y_BF16 (= "the type of X" here), amax NULL; C may be Y.  Sums are FP32, rounded once.
+ * GEMM_Y_BF16 (= "the type of X" here), amax NULL; C may be Y.  Sums are FP32, rounded once; their error is relative to
+ * the sum of (q + zero) * scale * |x| (zero = 8 for signed weights, q = w + 8).  An infinity or NaN in a row of X makes
+ * that row of Y NaN.
  */
 /* Returns GEMM_OK or an error code; asynchronous on success. */
 int gemm_run_ex(const GemmArgs *args);

@@ -77,7 +77,7 @@ typedef struct GemmRotaryArgs {
     int32_t layout;         /* GEMM_ROTARY_HALF / _INTERLEAVED                       */
     int32_t backward;       /* 0 / 1                                                 */
     int64_t tokens;         /* 0: nothing is done                                    */
-    int32_t heads, head_dim;
+    int32_t heads, head_dim;    /* heads * head_dim <= 2^30                              */
     int32_t rot_dim;        /* even, <= head_dim and <= 512                          */
     int32_t scaling;        /* GEMM_ROTARY_PLAIN ...                                 */
     const void *x;
@@ -103,13 +103,13 @@ typedef struct GemmLogitsArgs {
     uint32_t struct_size;   /* sizeof(GemmLogitsArgs), checked                                             */
     int32_t x_dtype, y_dtype;   /* GEMM_X_BF16, GEMM_X_F16 or GEMM_X_F32                                   */
     int32_t rows;           /* 0: nothing is done                                                          */
-    int32_t vocab;
+    int32_t vocab;          /* 1 .. 2^30                                                                   */
     int32_t reserved;       /* 0                                                                           */
     const void *x;
     void *y;
     int64_t x_ld, y_ld;     /* row pitches in elements, >= vocab                                           */
     const int32_t *history; /* [rows][history_ld], or NULL                                                 */
-    int64_t history_ld;
+    int64_t history_ld;     /* < 2^29                                                                      */
     const int32_t *history_len;     /* [rows], with history                                                */
     const int32_t *prompt_len;      /* [rows], or NULL: everything was generated                           */
     const float *repetition, *presence, *frequency;     /* [rows] each, or NULL: 1, 0, 0                   */

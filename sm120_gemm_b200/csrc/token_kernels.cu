@@ -640,6 +640,7 @@ int gemm_rotary(const GemmRotaryArgs *a)
     if (!is_type(a->dtype)) return refuse("unknown dtype %d", a->dtype);
     if (a->layout != GEMM_ROTARY_HALF && a->layout != GEMM_ROTARY_INTERLEAVED) return refuse("unknown layout %d", a->layout);
     if (a->tokens < 0 || a->heads < 1 || a->head_dim < 1) return refuse("%lld tokens, %d heads of %d", (long long)a->tokens, a->heads, a->head_dim);
+    if ((long long)a->heads * a->head_dim > 1ll << 30) return refuse("%d heads of %d: at most 2^30 values are wanted", a->heads, a->head_dim);
     if (a->rot_dim < 0 || a->rot_dim % 2 != 0 || a->rot_dim > a->head_dim || a->rot_dim > 2 * ROTARY_TABLE)
         return refuse("rot_dim %d: an even number up to head_dim = %d and %d is wanted", a->rot_dim, a->head_dim, 2 * ROTARY_TABLE);
     if (a->tokens == 0) return 0;
@@ -647,15 +648,16 @@ int gemm_rotary(const GemmRotaryArgs *a)
     const size_t e = type_bytes(a->dtype);
     if (!aligned(a->x, e) || !aligned(a->y, e) || !aligned(a->positions, 8)) return refuse("x, y and positions must be aligned to their elements");
     if (a->x == a->y && (a->x_token_stride != a->y_token_stride || a->x_head_stride != a->y_head_stride)) return refuse("in place, x and y have the same strides");
-    if (!(a->base > 0)) return refuse("base %g must be positive", a->base);
+    if (!(a->base > 0) || !isfinite(a->base)) return refuse("base %g must be positive and finite", a->base);
     RotaryKey key = {a->base, 1, 0, 1, 1, a->rot_dim, a->scaling};
     if (a->scaling != GEMM_ROTARY_PLAIN) {
         if (a->scaling < GEMM_ROTARY_PLAIN || a->scaling > GEMM_ROTARY_RAMP) return refuse("unknown scaling %d", a->scaling);
-        if (!(a->factor > 0)) return refuse("factor %g must be positive", a->factor);
+        if (!(a->factor > 0) || !isfinite(a->factor)) return refuse("factor %g must be positive and finite", a->factor);
         if (a->scaling == GEMM_ROTARY_NTK && a->rot_dim <= 2) return refuse("GEMM_ROTARY_NTK needs more than one pair");
         key.factor = a->factor;
         if (a->scaling == GEMM_ROTARY_RAMP) {
-            if (!(a->high_rotations > a->low_rotations) || !(a->original_length > 0)) return refuse("GEMM_ROTARY_RAMP needs high_rotations > low_rotations and original_length > 0");
+            if (!(a->high_rotations > a->low_rotations) || !(a->original_length > 0) || !isfinite(a->low_rotations) || !isfinite(a->high_rotations) || !isfinite(a->original_length))
+                return refuse("GEMM_ROTARY_RAMP needs high_rotations > low_rotations and original_length > 0, all finite");
             key.low = a->low_rotations;
             key.high = a->high_rotations;
             key.original = a->original_length;
@@ -681,7 +683,7 @@ int gemm_logits(const GemmLogitsArgs *a)
     g_message[0] = 0;
     if (!a || a->struct_size != sizeof(GemmLogitsArgs)) return refuse("GemmLogitsArgs is null or has the wrong struct_size");
     if (!is_type(a->x_dtype) || !is_type(a->y_dtype)) return refuse("unknown x_dtype %d or y_dtype %d", a->x_dtype, a->y_dtype);
-    if (a->rows < 0 || a->vocab < 1) return refuse("%d rows of %d", a->rows, a->vocab);
+    if (a->rows < 0 || a->vocab < 1 || a->vocab > 1 << 30) return refuse("%d rows of %d (1 to 2^30 are wanted)", a->rows, a->vocab);
     if (a->rows == 0) return 0;
     if (!a->x || !a->y) return refuse("null x or y");
     if (!aligned(a->x, type_bytes(a->x_dtype)) || !aligned(a->y, type_bytes(a->y_dtype))) return refuse("x and y must be aligned to their elements");

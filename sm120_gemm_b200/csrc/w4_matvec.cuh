@@ -121,7 +121,9 @@ struct W4MatvecTraits {
     // tile is 32 rows of W, so that what is read of X is used twice; that takes the registers of 8 warps.
     static constexpr int SUBTILES = NB, TILE = 16 * SUBTILES, UNIT = 128;
     static constexpr int WARPS = NB == 1 ? 16 : 8, THREADS = 32 * WARPS;
-    static constexpr int RING = 2;                   // batches of two units in flight per warp (3 were no faster: X needs the room)
+    // batches of two units in flight per warp; a batch is four 16-byte pieces per thread for every 16 rows, and STAGES the pieces
+    // (three batches were no faster, and X needs the room)
+    static constexpr int RING = STAGES / 4;
     static constexpr int UNIT_BYTES = TILE * UNIT / 2;
     static constexpr int AHEAD_ROWS = 32;            // rows of W asked into L2 before the grid before has ended
     // a batch in the ring: two units, then per row the scales of its 2 GPU groups and a word in front of them, then per row
@@ -135,6 +137,7 @@ struct W4MatvecTraits {
     static __host__ __device__ constexpr int x_row_bytes(int units) { return units * UNIT * 2 + 64; }
     static __host__ __device__ constexpr int staged_bytes(int M, int units, int gpu) { return M * x_row_bytes(units) + units * gpu * NB * 32; }
     static_assert(MPAD_ == 8 || MPAD_ == 16, "rows of X: up to 8 or 16");
+    static_assert(STAGES_ % 4 == 0 && STAGES_ >= 8, "whole batches, two at least");
 };
 
 // act(alpha * acc + beta * C + bias), rounded once to the type of Y
@@ -692,13 +695,13 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
 
 template <class T>
 struct W4MatvecLauncher {
-    static bool can_run(int M, int N, int K) { return M >= 1 && M <= T::MPAD && N >= 1 && K >= 32 && K % 32 == 0 && K <= 1 << 24; }
+    static bool can_run(int M, int N, int K) { return M >= 1 && M <= T::MPAD && N >= 1 && N <= 1 << 30 && K >= 32 && K % 32 == 0 && K <= 1 << 24; }
     // the family's figure, so that one workspace serves whichever W4A16 plugin is picked; nothing here touches it
     static size_t workspace_bytes(int, int, int) { return (size_t)2 * STREAMK_MAX_CTAS * 128 * 128 * sizeof(float); }
 
     static int run(const GemmArgs &a)
     {
-        if (!can_run(a.M, a.N, a.K)) return set_error(GEMM_ERR_SHAPE, "shape %dx%dx%d not supported (M <= %d, K a multiple of 32)", a.M, a.N, a.K, T::MPAD);
+        if (!can_run(a.M, a.N, a.K)) return set_error(GEMM_ERR_SHAPE, "shape %dx%dx%d not supported (M <= %d, N <= 2^30, K <= 2^24 a multiple of 32)", a.M, a.N, a.K, T::MPAD);
         if ((a.group_size != 32 && a.group_size != 64 && a.group_size != 128) || a.K % a.group_size != 0)
             return set_error(GEMM_ERR_ARG, "scale groups are 32, 64 or 128 K-elements that divide K = %d, got %d", a.K, a.group_size);
         if (a.x_dtype != GEMM_X_BF16 && a.x_dtype != GEMM_X_F16) return set_error(GEMM_ERR_ARG, "unknown x_dtype %d", a.x_dtype);
@@ -753,7 +756,7 @@ struct W4MatvecLauncher {
         const int fixed = T::ring_bytes(gpu) + T::ROW_BYTES;
         for (int cluster_shift = 0; cluster_shift <= 2; cluster_shift++) {
             const int cluster = 1 << cluster_shift, shares = std::min(cluster == 1 ? most_ctas : std::min(most_ctas / cluster, clusters[cluster_shift - 1]), all_tiles);
-            if (shares == 0) continue;
+            if (shares == 0 || cluster > all_batches) continue;      // (every CTA has a part of K)
             const int rows = (all_tiles + shares - 1) / shares * T::TILE, units = (all_batches + cluster - 1) / cluster * 2;
             for (int shift = T::WARPS == 16 ? 4 : 3; shift >= 0; shift--) {
                 const int wk = 1 << shift, per_tile = wk * a.M * T::TILE * (int)sizeof(float);

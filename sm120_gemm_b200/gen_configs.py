@@ -103,7 +103,7 @@ class GemmConfig:
         if M <= 0 or N <= 0 or K <= 0:
             return False
         if self.dt == "w4a16" and self.bk == 32:   # matrix-vector plugins (K must also be whole scale groups)
-            return M <= self.bn and K % 32 == 0 and K <= 1 << 24
+            return M <= self.bn and N <= 1 << 30 and K % 32 == 0 and K <= 1 << 24
         if self.dt == "w4a16":   # decode kernel: M fits the padded UMMA N, whole 128-element scale groups
             return M <= self.bn and N % 8 == 0 and K % 128 == 0
         if (K * ELEM_BITS[self.dt]) % 128 != 0 or N % 8 != 0:
@@ -209,7 +209,8 @@ def generate_w4a16(max_smem: int) -> list[GemmConfig]:
     """W4A16 decode kernels: operands swapped (ab=1), bn = M padded to 16/32/64/128, stream-K work split.
     bk128: dequantised weights go through tensor memory (A operand of the MMA read from TMEM), s = group slots;
     bk64: dequantised weights go through shared memory, s = group ring slots.
-    bk32: matrix-vector products (sk1: the whole K in one CTA), s = 16-byte weight loads in flight per thread."""
+    bk32: matrix-vector products; s = 16-byte weight loads in flight per thread for every 16 rows of W; sk1: the
+    parts of K meet inside the kernel."""
     out = []
     for rows in (8, 16):
         for epi in (0, 2):

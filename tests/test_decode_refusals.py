@@ -127,6 +127,35 @@ def test_logits_refusals(change, text):
     assert e.value.code == 6 and text in str(e.value)
 
 
+@pytest.mark.parametrize("change", [
+    dict(vocab=(1 << 30) + 1, x_ld=1 << 31, y_ld=1 << 31), dict(history=3 << 20, history_len=4 << 20, history_ld=1 << 29), dict(history_ld=1 << 40),
+])
+def test_logits_sizes(change):
+    with pytest.raises(g.GemmError, match="wanted"):
+        g.logits(logits_args(**change))
+
+
+@pytest.mark.parametrize("change", [
+    dict(heads=1 << 24, head_dim=128), dict(base=float("inf")), dict(scaling=1, factor=float("inf")),
+    dict(scaling=3, factor=2.0, low_rotations=float("-inf"), high_rotations=4, original_length=8192),
+    dict(scaling=3, factor=2.0, low_rotations=1, high_rotations=float("inf"), original_length=8192),
+    dict(scaling=3, factor=2.0, low_rotations=1, high_rotations=4, original_length=float("inf")),
+])
+def test_rotary_sizes_and_infinite_parameters(change):
+    with pytest.raises(g.GemmError, match="wanted|finite"):
+        g.rotary(rotary_args(**change))
+
+
+@pytest.mark.parametrize("n, k", [(16, (1 << 24) + 128), ((1 << 30) + 1, 128)])
+def test_matvec_sizes(registry, n, k):
+    a = g.GemmArgs()
+    a.M, a.N, a.K, a.group_size = 1, n, k, 128
+    a.X, a.W, a.Y, a.w_scale = 1 << 20, 2 << 20, 3 << 20, 4 << 20
+    for rows in (8, 16):
+        with pytest.raises(g.GemmError, match="not supported"):
+            g.dispatch_ex(registry.find(f"w4a16_bm128_bn{rows}_bk32_s8_cg1_sk1_ab1_e0"), a)
+
+
 def test_nothing_to_do_is_no_error():
     """No tokens, no rows: success without a launch (there is no GPU here to launch on)."""
     g.rotary(rotary_args(tokens=0, x=None, y=None, positions=None))

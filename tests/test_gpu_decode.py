@@ -601,6 +601,38 @@ def test_logits_special_values(cuda_device):
     assert math.isnan(y[0]) and y[1] == math.inf and y[2] == -math.inf and math.isfinite(y[3]) and y[4] == -math.inf and y[5] == -math.inf and y[6] == -1.0 and y[7] == -1.0
 
 
+@pytest.mark.parametrize("tx, ty", [("bf16", "f32"), ("f32", "f32"), ("f16", "bf16")])
+@pytest.mark.parametrize("shape", [(2, 40000, 9000, 50), (3, 5000, 20000, 10), (2, 300, 8192, 4), (1, 129280, 8191, 3000), (2, 33, 30000, 2)])
+def test_logits_histories_around_the_width_of_a_count(cuda_device, shape, tx, ty):
+    """A history of 8192 ids is the first whose counts take 32 bits; one token may be all of it."""
+    rows, vocab, hist, biases = shape
+    x, kw = logits_case(rows, vocab, hist, biases, True, seed=vocab, dtype=T[tx], pad=1)
+    kw["prompt"][0] = 0
+    kw["history"][0, 1:] = min(17, vocab - 1)
+    y = torch.full((rows, vocab), float("nan"), device="cuda", dtype=T[ty])
+    check_logits(logits(x, vocab, y, **kw), x, vocab, **kw)
+    if tx == ty:
+        in_place = x.clone()
+        logits(in_place, vocab, in_place, **kw)
+        assert torch.equal(in_place[:, :vocab], y) and torch.equal(in_place[:, vocab:], x[:, vocab:])
+
+
+def test_logits_biases_that_are_no_numbers(cuda_device):
+    """A bias may forbid a token or spoil its own logit, no other's; a masked token is -inf whatever its bias; without a generated
+    token the penalties are left out."""
+    vocab = 70
+    x = torch.linspace(-3, 3, vocab, device="cuda")[None].contiguous()
+    ids = torch.tensor([3, 9, 9, 40, 50, 50, 69], device="cuda", dtype=torch.int32)
+    values = torch.tensor([float("-inf"), 1.0, float("nan"), float("inf"), float("inf"), float("-inf"), float("nan")], device="cuda")
+    mask = torch.full((1, 3), -1, device="cuda", dtype=torch.int32)
+    mask[0, 2] = ~(1 << 5)                                           # 69 masked
+    y = logits(x, vocab, torch.empty_like(x), ids=ids, values=values, begin=torch.tensor([0, 7], device="cuda", dtype=torch.int32), mask=mask)[0]
+    assert y[3] == -math.inf and y[9].isnan() and y[40] == math.inf and y[50].isnan() and y[69] == -math.inf
+    rest = torch.ones(vocab, dtype=torch.bool, device="cuda")
+    rest[ids.long()] = False
+    assert torch.equal(y[rest], x[0][rest])
+
+
 def test_logits_lengths_beyond_the_row_and_negative(cuda_device):
     x, kw = logits_case(3, 500, 40, 0, False, seed=2)
     kw["length"] = torch.tensor([1 << 30, -5, 40], device="cuda", dtype=torch.int32)
