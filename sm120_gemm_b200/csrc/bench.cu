@@ -5,7 +5,7 @@
 //   bench --debug      fixed configurations called through the class templates, verbose checks
 // and one more for single measurements (profiling a kernel, sweeps):
 //   bench --kernel <config name> --shape M,N,K      time that one plugin
-//   bench --aux                                      the HBM-bound helper kernels alone (split-K reduce, quantisers, interleave) in GB/s
+//   bench --aux                                      the HBM-bound helper kernels alone (split-K reduce, quantisers, interleave, rotary positions, logits) in GB/s
 // Options: --dtype bf16|fp8|mxfp8|w4a4|w4a16 (default bf16)   --dir <plugin dir>   --cache <file>
 //          --shape M,N,K (repeatable, replaces the built-in list)   --json <file> (one JSON object per line)
 //          --peaks <MEASURED_PEAKS.json> (adds "% of measured" beside the nominal roofline fractions)
@@ -399,7 +399,7 @@ double time_comparator(Problem &p, cublasHandle_t handle, cudaStream_t stream, s
 }
 
 // bench --aux: the HBM-bound helper kernels on their own, as GB/s of algorithmic bytes: the split-K reduce kernel
-// (decode-sized and large), the quantisation kernels and the column-block interleave.  Small cases rotate over
+// (decode-sized and large), the quantisation kernels, the column-block interleave, rotary positions and logits.  Small cases rotate over
 // enough buffer sets to exceed twice the L2, like the GEMM timings.
 template <class F>
 void aux_line(const char *what, double bytes, F &&launch, cudaStream_t stream)
@@ -466,6 +466,67 @@ int aux_mode()
     DevBuf<bf16> blocked((size_t)R * K), y((size_t)R * K);
     if (!blocked.p || !y.p) return 1;
     aux_line("gemm_interleave_blocks 8 x [8192][1024] -> [8192][8192] bf16", n * 4, [&] { gemm_interleave_blocks(blocked.p, y.p, 8, R, (int)K / 8, 2, stream); }, stream);
+    {
+        // rotary positions of 64 heads of 128 of 8192 tokens, and the gradient's rotation of the same
+        DevBuf<int64_t> positions((size_t)R);
+        if (!positions.p) return 1;
+        std::vector<int64_t> h((size_t)R);
+        for (long long i = 0; i < R; i++) h[i] = i;
+        cudaMemcpy(positions.p, h.data(), h.size() * 8, cudaMemcpyHostToDevice);
+        GemmRotaryArgs r = {};
+        r.struct_size = sizeof r;
+        r.dtype = GEMM_X_BF16;
+        r.tokens = R;
+        r.heads = 64;
+        r.head_dim = r.rot_dim = 128;
+        r.x = x.p;
+        r.y = y.p;
+        r.x_token_stride = r.y_token_stride = K;
+        r.x_head_stride = r.y_head_stride = 128;
+        r.positions = positions.p;
+        r.base = 10000.0;
+        r.scale = 1.f;
+        r.stream = stream;
+        int rc = 0;
+        aux_line("gemm_rotary 8192 tokens x 64 heads of 128, bf16", n * 4, [&] { rc |= gemm_rotary(&r); }, stream);
+        r.backward = 1;
+        aux_line("gemm_rotary, backward", n * 4, [&] { rc |= gemm_rotary(&r); }, stream);
+        if (rc != 0) { std::printf("  gemm_rotary: %s\n", gemm_util_last_error_message()); return 1; }
+    }
+    {
+        // logits of 64 sequences over 131072 tokens, 4096 of them said, all allowed
+        const int rows = 64, vocab = 131072, said = 4096;
+        DevBuf<float> out((size_t)rows * vocab), penalty(rows);
+        DevBuf<int32_t> history((size_t)rows * said), length(rows);
+        DevBuf<uint32_t> mask((size_t)rows * vocab / 32);
+        if (!out.p || !penalty.p || !history.p || !length.p || !mask.p) return 1;
+        std::vector<int32_t> h((size_t)rows * said), len(rows, said);
+        for (size_t i = 0; i < h.size(); i++) h[i] = (int32_t)((i * 2654435761ull) >> 7) & (vocab - 1);
+        std::vector<float> pen(rows, 1.25f);
+        cudaMemcpy(history.p, h.data(), h.size() * 4, cudaMemcpyHostToDevice);
+        cudaMemcpy(length.p, len.data(), len.size() * 4, cudaMemcpyHostToDevice);
+        cudaMemcpy(penalty.p, pen.data(), pen.size() * 4, cudaMemcpyHostToDevice);
+        cudaMemset(mask.p, 255, (size_t)rows * vocab / 8);
+        GemmLogitsArgs l = {};
+        l.struct_size = sizeof l;
+        l.x_dtype = GEMM_X_BF16;
+        l.y_dtype = GEMM_X_F32;
+        l.rows = rows;
+        l.vocab = vocab;
+        l.x = x.p;
+        l.y = out.p;
+        l.x_ld = l.y_ld = vocab;
+        l.history = history.p;
+        l.history_ld = said;
+        l.history_len = length.p;
+        l.repetition = l.presence = l.frequency = penalty.p;
+        l.mask = mask.p;
+        l.mask_ld = vocab / 32;
+        l.stream = stream;
+        int rc = 0;
+        aux_line("gemm_logits 64 x 131072 bf16 -> fp32, 4096 said, mask", (double)rows * (vocab * (2 + 4 + 0.125) + said * 4), [&] { rc |= gemm_logits(&l); }, stream);
+        if (rc != 0) { std::printf("  gemm_logits: %s\n", gemm_util_last_error_message()); return 1; }
+    }
     return 0;
 }
 
