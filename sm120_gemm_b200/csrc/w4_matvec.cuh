@@ -63,8 +63,8 @@ struct W4MatvecParams {
     int wk_shift;                // log2(WK)
     int cluster;                 // CTAs that share tiles, each a part of K
     int part_at;                 // partial sums: byte offset in shared memory
-    int scale_window, zero_window;       // scales / zero points reach the ring in words around them, else they are read when needed
-    const uint8_t *scales_end, *zeros_end;
+    uint32_t step_batch, step_w, step_s, step_z;         // bytes from a warp's batch of W to its next; from a warp's tile to its next
+    const uint8_t *scales_end, *zeros_end;       // behind the word (4-byte aligned) that holds the last
 };
 
 // What depends on the 16-bit type: the matrix instruction m16n8k16 (D = A * B + C, C and D FP32), and the scaling of X.
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
     constexpr int NB = T::NB, WARPS = T::WARPS, THREADS = T::THREADS, SUBTILES = T::SUBTILES, TILE = T::TILE;
     constexpr int LANES_PER_ROW = 32 / TILE;             // that bring its scales and zero points
     constexpr int GROUP_SUBS = 4 / GPU;                  // pieces of 32 k in a group
-    constexpr int STEPS = GPU == 1 ? 2 : 4, SUBS = 8 / STEPS, GROUPS = 2 * GPU / STEPS;      // steps of a batch, pieces and groups of a step
+    constexpr int STEPS = GPU <= 2 ? 2 : 4, SUBS = 8 / STEPS, GROUPS = 2 * GPU / STEPS;      // steps of a batch, pieces and groups of a step
     constexpr int SLOT = T::slot_bytes(GPU), SCALES_AT = 2 * T::UNIT_BYTES, SCALE_PITCH = T::scale_pitch(GPU), ZEROS_AT = SCALES_AT + TILE * SCALE_PITCH;
     constexpr int RING_BYTES = T::RING * SLOT;           // of a warp
     constexpr uint32_t X_AT = T::ring_bytes(GPU) + T::ROW_BYTES;
@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
     const int share = blockIdx.x / cluster, shares = gridDim.x / cluster;
     const int row_begin = (int)(all_tiles * share / shares) * T::TILE, row_end = min((int)(all_tiles * (share + 1) / shares) * T::TILE, p.N);
     const uint8_t *scales = static_cast<const uint8_t *>(p.scales);
-    const uint32_t step_batch = WK * T::UNIT, step_w = WR * TILE * row_bytes, step_s = WR * TILE * groups * 2, step_z = WR * TILE * zero_pitch;      // K <= 2^24
+    const uint32_t step_batch = p.step_batch, step_w = p.step_w, step_s = p.step_s, step_z = p.step_z;
 
     // The ring holds a unit as TILE rows of four 16-byte pieces; piece j of row r lies at (r, j ^ (r / 2 % 4)), so that the
     // eight rows of a matrix reach all banks.  Copies: lane (g, c) brings piece c of rows g, g + 8, ...  ldmatrix: lane l
@@ -399,6 +399,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
     const uint32_t ring = smem_u32(smem) + warp * RING_BYTES;
     const uint32_t put_at = g * 64 + ((c ^ (g >> 1 & 3)) << 4);
     const uint32_t get_at = (lane & 15) * 64 + (((lane >> 4) ^ (lane >> 1 & 3)) << 4);
+    const uint32_t scales_odd = (uint32_t)reinterpret_cast<uintptr_t>(p.scales) >> 1 & 1, zeros_low = (uint32_t)reinterpret_cast<uintptr_t>(p.zeros);
     const uint32_t flip_lo = ZERO ? 0u : w4_keep(0x00080008u), flip_hi = ZERO ? 0u : w4_keep(0x00800080u);
     // this lane's column of B in column block nb is row m of X; columns behind the last repeat it (nobody reads their sums)
     uint32_t xbase[NB];
@@ -446,38 +447,40 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
             auto load = [&](uint32_t slot) {               // slot: byte offset in the ring
                 if (ld_tile < tiles) {
                     const uint32_t dst = ring + slot;
+                    if (WHOLE || ld_batch != cut) {
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const bool in_k = WHOLE || ld_batch != cut || (u0 + 2 * ld_batch + i) * T::UNIT + c * 32 < K;
+                        for (int i = 0; i < 2; i++)
 #pragma unroll
-                        for (int k = 0; k < 2 * SUBTILES; k++) {
-                            const uint8_t *from = wa + to_row[k] + i * (T::UNIT / 2);
-                            if (WHOLE) w4_copy16(dst + put_at + i * T::UNIT_BYTES + k * 512, from);
-                            else w4_copy16(dst + put_at + i * T::UNIT_BYTES + k * 512, in_k ? from : p.W, in_k ? 16 : 0);
+                            for (int k = 0; k < 2 * SUBTILES; k++) w4_copy16(dst + put_at + i * T::UNIT_BYTES + k * 512, wa + to_row[k] + i * (T::UNIT / 2));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            const bool in_k = (u0 + 2 * ld_batch + i) * T::UNIT + c * 32 < K;
+#pragma unroll
+                            for (int k = 0; k < 2 * SUBTILES; k++)
+                                w4_copy16(dst + put_at + i * T::UNIT_BYTES + k * 512, in_k ? wa + to_row[k] + i * (T::UNIT / 2) : p.W, in_k ? 16 : 0);
                         }
                     }
                     const uint32_t dst_s = dst + SCALES_AT + lane % TILE * SCALE_PITCH, dst_z = dst + ZEROS_AT + lane % TILE * 8;
                     if (WHOLE) {
                         if (lane < TILE) w4_copy_small<4 * GPU>(dst_s, ls);
-                    } else if (p.scale_window) {
-                        // words around them: from the word that holds the first, never behind the array's end
+                    } else {
+                        // the words that hold them: from the one of the first, none behind the array's last
                         const uint8_t *from = reinterpret_cast<const uint8_t *>(reinterpret_cast<uintptr_t>(ls) & ~(uintptr_t)3);
+                        const int left = (int)min((long long)(p.scales_end - from), 64ll);
 #pragma unroll
                         for (int w = 0; w <= GPU / LANES_PER_ROW; w++) {
                             const int word = w * LANES_PER_ROW + lane / TILE;
-                            const long long left = p.scales_end - (from + 4 * word);
-                            if (word <= GPU) w4_copy4(dst_s + 4 * word, left > 0 ? from + 4 * word : scales, left >= 4 ? 4 : left > 0 ? (int)left : 0);
+                            if (word <= GPU) w4_copy4(dst_s + 4 * word, 4 * word < left ? from + 4 * word : from, 4 * word < left ? 4 : 0);
                         }
                     }
                     if (ZERO && WHOLE && GPU == 4) {
                         if (lane < TILE) w4_copy_small<4>(dst_z, lz);
-                    } else if (ZERO && (WHOLE || p.zero_window)) {
+                    } else if (ZERO) {
+                        const uint8_t *from = reinterpret_cast<const uint8_t *>(reinterpret_cast<uintptr_t>(lz) & ~(uintptr_t)3);
+                        const bool both = p.zeros_end - from > 4;
 #pragma unroll
-                        for (int w = lane / TILE; w < 2; w += LANES_PER_ROW) {
-                            const uint8_t *from = reinterpret_cast<const uint8_t *>(reinterpret_cast<uintptr_t>(lz) & ~(uintptr_t)3) + 4 * w;
-                            const long long left = p.zeros_end - from;
-                            w4_copy4(dst_z + 4 * w, left > 0 ? from : p.zeros, left >= 4 ? 4 : left > 0 ? (int)left : 0);
-                        }
+                        for (int w = lane / TILE; w < 2; w += LANES_PER_ROW) w4_copy4(dst_z + 4 * w, w == 0 || both ? from + 4 * w : from, w == 0 || both ? 4 : 0);
                     }
                     ld_batch += WK;
                     wa += step_batch;
@@ -535,16 +538,19 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
             // A STEP is the part of a batch whose sums are kept apart: a unit (GPU = 1), else half a unit, GPU / 2 groups.
             // scales of a step for row `row` of the tile, row ra of W: GROUPS times 16 bits
             auto scales_of = [&](const uint8_t *slot, int row, int ra, int step) -> uint32_t {
-                const int first = (u0 + 2 * batch) * GPU + step * GROUPS;          // the step's first group
                 if constexpr (WHOLE) {
                     const uint8_t *at = slot + SCALES_AT + row * SCALE_PITCH + step * (2 * GROUPS);
                     return GROUPS == 1 ? *reinterpret_cast<const uint16_t *>(at) : *reinterpret_cast<const uint32_t *>(at);
                 } else {
-                    // (the window starts with the word that holds the batch's first scale; the array is 4-byte aligned)
-                    const uint16_t *at = p.scale_window ? reinterpret_cast<const uint16_t *>(slot + SCALES_AT + row * SCALE_PITCH + (ra & groups & 1) * 2) + step * GROUPS
-                                                        : reinterpret_cast<const uint16_t *>(scales) + (size_t)ra * groups + first;
-                    uint32_t v = first < groups ? at[0] : 0u;
-                    if (GROUPS == 2 && first + 1 < groups) v |= (uint32_t)at[1] << 16;
+                    // (the first of the batch is the lower or the upper half of its word)
+                    const uint16_t *at = reinterpret_cast<const uint16_t *>(slot + SCALES_AT + row * SCALE_PITCH) + ((ra & groups & 1) ^ scales_odd) + step * GROUPS;
+                    uint32_t v = at[0];
+                    if (GROUPS == 2) v |= (uint32_t)at[1] << 16;
+                    if (batch == cut) {              // behind K lies the next row's
+                        const int first = (u0 + 2 * batch) * GPU + step * GROUPS;
+                        if (first >= groups) v = 0;
+                        else if (GROUPS == 2 && first + 1 >= groups) v &= 0xffffu;
+                    }
                     return v;
                 }
             };
@@ -553,12 +559,8 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
                 if constexpr (WHOLE && GPU == 4) {
                     return slot[ZEROS_AT + row * 8 + step];
                 } else {
-                    // byte of the batch's first group; its low bits say where the window starts
-                    const int in_row = (u0 + 2 * batch) * GPU / 2;
-                    const uint32_t low = ra * (uint32_t)zero_pitch + in_row;
-                    const int first = (u0 + 2 * batch) * GPU + step * GROUPS;
-                    if (!WHOLE && !p.zero_window && first >= groups) return 0;     // (in the window are zeros or bytes of the array)
-                    const uint8_t *at = WHOLE || p.zero_window ? slot + ZEROS_AT + row * 8 + (low & 3) : p.zeros + (size_t)ra * zero_pitch + in_row;
+                    // the low bits of the address of the batch's first byte say where it is in its word
+                    const uint8_t *at = slot + ZEROS_AT + row * 8 + ((zeros_low + ra * (uint32_t)zero_pitch + (u0 + 2 * batch) * GPU / 2) & 3);
                     return GROUPS == 2 ? at[step] : at[step >> 1] >> (4 * (step & 1));
                 }
             };
@@ -581,7 +583,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
                     // piece 2 h of a unit lies where piece 0 does, bit 5 of the address flipped for h = 1
 #pragma unroll
                     for (int t = 0; t < SUBTILES; t++)
-                        w4_ldmatrix(q[t], (GPU == 1 ? (from + step * T::UNIT_BYTES) ^ (pair * 32) : (from + (step >> 1) * T::UNIT_BYTES) ^ ((step & 1) * 32)) + t * 1024);
+                        w4_ldmatrix(q[t], (STEPS == 2 ? (from + step * T::UNIT_BYTES) ^ (pair * 32) : (from + (step >> 1) * T::UNIT_BYTES) ^ ((step & 1) * 32)) + t * 1024);
 #pragma unroll
                     for (int sub = 0; sub < 2; sub++) {
                         const int j = 2 * pair + sub;    // piece of the step
@@ -640,8 +642,9 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
             while (tile < tiles) {
                 w4_copies_wait<T::RING - 1>();
                 __syncwarp();                            // the other lanes' copies too
-                // one step after the other where the registers are short
-                constexpr int UNROLL = GPU == 1 && NB == 1 ? 2 : 1;
+                // one step after the other where the registers are short (two side by side: 4 x 131072 x 4096 in groups of 32 64 us
+                // against 68)
+                constexpr int UNROLL = (GPU == 1 || WHOLE) && NB == 1 ? 2 : 1;
 #pragma unroll UNROLL
                 for (int step = 0; step < STEPS; step++) compute(smem + warp * RING_BYTES + slot, ring + slot + get_at, step);
                 __syncwarp();                            // every lane has read the slot
@@ -735,11 +738,8 @@ struct W4MatvecLauncher {
         const int most_ctas = a.sm_limit > 0 && a.sm_limit < sms ? a.sm_limit : sms;
         const int all_tiles = (a.N + T::TILE - 1) / T::TILE, all_batches = (a.K + 2 * T::UNIT - 1) / (2 * T::UNIT);
         const int gpu = T::UNIT >> p.group_shift;
-        // how scales and zero points come: with whole batches, else in words around them (base 4-byte aligned), else one by one
-        // when they are needed
+        // how scales and zero points come: with whole batches, else in the words that hold them
         const bool whole = a.K % (2 * T::UNIT) == 0 && bits(a.w_scale) % (4 * gpu) == 0 && bits(a.w_zero) % 4 == 0;
-        p.scale_window = bits(a.w_scale) % 4 == 0;
-        p.zero_window = bits(a.w_zero) % 4 == 0;
         // The plan.  A cluster of 1, 2 or 4 CTAs shares tiles, each CTA a part of K: every SM then stages a half or a quarter of
         // X, which is what many rows and a long K cost most (us, clusters of 1 / 2 / 4: 16 x 4096 x 14336 37 / 26.6 / 20;
         // 8 x 28672 x 8192 35.9 / 30.2 / 34.4), and adds the partial sums across the cluster (1 x 4096 x 4096 5.9 / 6.8; 4 of the
@@ -781,9 +781,15 @@ struct W4MatvecLauncher {
                 p.part_at = fixed + T::staged_bytes(a.M, per_pass, gpu);
             }
         }
+        const uint32_t tile_step = (T::WARPS >> p.wk_shift) * T::TILE;                // rows; K <= 2^24
+        p.step_batch = T::UNIT << p.wk_shift;
+        p.step_w = tile_step * ((uint32_t)a.K / 2);
+        p.step_s = tile_step * p.groups * 2;
+        p.step_z = tile_step * p.zero_pitch;
         const int smem = p.part_at + p.block_rows * a.M * (int)sizeof(float) * (1 << p.wk_shift);
-        p.scales_end = static_cast<const uint8_t *>(a.w_scale) + (size_t)a.N * p.groups * 2;
-        p.zeros_end = a.w_zero ? p.zeros + (size_t)a.N * p.zero_pitch : nullptr;
+        auto word_end = [&](const void *base, size_t bytes) { return reinterpret_cast<const uint8_t *>((bits(base) + bytes + 3) & ~(uintptr_t)3); };
+        p.scales_end = word_end(a.w_scale, (size_t)a.N * p.groups * 2);
+        p.zeros_end = word_end(a.w_zero, (size_t)a.N * p.zero_pitch);
         if (a.x_dtype == GEMM_X_F16) return launch<__half>(p, whole, grid, smem, a.stream);
         return launch<__nv_bfloat16>(p, whole, grid, smem, a.stream);
     }
