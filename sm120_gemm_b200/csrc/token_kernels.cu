@@ -322,9 +322,9 @@ struct LogitsParams {
 
 // A CTA has a window of a row's vocabulary.  Some of its warps count the row's history into shared memory, what is in the
 // window (integer atomics: the order does not matter); meanwhile the others write y = x under the mask for the window, chunk
-// by chunk, and the counting warps join them.  Then the few tokens that were said or have a bias are listed and rewritten:
+// by chunk, and the counting warps join them.  Then the few tokens that were said (listed meanwhile) or have a bias are rewritten:
 // whole warps do their arithmetic (a division among it), not every warp for the one lane in thirty that needs it.  Few bytes
-// (x once, y once), many instructions: 64 x 131072 with 4096 said takes 21 us, of which the masked copy is 13 (a plain copy 10.8).
+// (x once, y once), many instructions: 64 x 131072 with 4096 said takes 16.7 us, of which the masked copy is 13 (a plain copy 10.8).
 // What it must not do is wait: with the counting in front of the writing a CTA held its window up for four round trips to
 // memory, 29 us whatever the size of the windows; writing and rewriting in two kernels took 28.
 // a token's count: in the prompt; has a bias, several; how often it was generated.  16 bits hold it (the flags in the upper
@@ -334,7 +334,13 @@ template <bool NARROW>
 struct Counts {
     unsigned *words;
     static constexpr int BITS = NARROW ? 16 : 32, PER_WORD = 32 / BITS;
-    __device__ __forceinline__ void add(unsigned at) { atomicAdd(words + at / PER_WORD, 1u << at % PER_WORD * BITS % 32); }
+    // one more; returns what was there
+    __device__ __forceinline__ unsigned add(unsigned at)
+    {
+        const unsigned before = atomicAdd(words + at / PER_WORD, 1u << at % PER_WORD * BITS % 32);
+        if constexpr (NARROW) return wide(before >> at % 2 * 16 & 0xffffu);
+        else return before;
+    }
     // sets flag bits (of the 32-bit form); returns what was there
     __device__ __forceinline__ unsigned set(unsigned at, unsigned flag)
     {
@@ -342,22 +348,16 @@ struct Counts {
         else return atomicOr(words + at, flag);
     }
     static __device__ __forceinline__ unsigned wide(unsigned half) { return (half & 0xe000u) << 16 | (half & 0x1fffu); }
-    // which of the 8 tokens from `at` on (a multiple of 8) were said and have no bias
+    // which of the 8 tokens from `at` on (a multiple of 8) were said (32-bit counts)
     __device__ __forceinline__ unsigned said(unsigned at) const
     {
-        unsigned w[8 / PER_WORD], bits = 0;
+        unsigned bits = 0;
 #pragma unroll
-        for (int i = 0; i < 8 / PER_WORD; i += 4) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(words + at / PER_WORD + i);
-            w[i] = v.x;
-            w[i + 1] = v.y;
-            w[i + 2] = v.z;
-            w[i + 3] = v.w;
-        }
+        for (int i = 0; i < 8; i += 4) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(words + at + i);
+            const unsigned w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const unsigned c = w[k / PER_WORD] >> k % PER_WORD * BITS % 32 & (NARROW ? 0xffffu : 0xffffffffu);
-            bits |= c != 0 && !(c & (BIASED >> (32 - BITS))) ? 1u << k : 0u;
+            for (int k = 0; k < 4; k++) bits |= w[k] & (SEEN | GENERATED) ? 1u << (i + k) : 0u;
         }
         return bits;
     }
@@ -444,6 +444,9 @@ template <class TX, class TY, bool NARROW, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 3 : 1) logits_kernel(const LogitsParams p)
 {
     constexpr int G = sizeof(TX) == 4 ? 1 : 2, CHUNK = 32 * 8 * G;
+    // Said tokens are listed by who meets them first; where the history has more ids than the window has tokens, from the
+    // counts afterwards (us, listed first / afterwards: 64 x 131072 with 4096 said 16.5 / 21.3, 8 x 100003 with 60000 19.4 / 13.7).
+    constexpr bool LIST_AT_FIRST = NARROW;
     extern __shared__ __align__(16) unsigned shared[];     // the window's counts, then the list (16-bit places in the window)
     __shared__ int next_chunk, listed;
     after_the_grid_before();
@@ -468,50 +471,81 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 3 : 1) logits_kernel
         for (int i = threadIdx.x; i * 4 * count.PER_WORD < p.window; i += THREADS) reinterpret_cast<uint4 *>(count.words)[i] = make_uint4(0, 0, 0, 0);
     if (threadIdx.x == 0) next_chunk = listed = 0;
     __syncthreads();
+    // the places of a warp's `mine` entries each in the list: where this lane's begin
+    auto places = [&](int mine, int all) {
+        int to = mine;                                       // up to and with this lane's
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int lower = __shfl_up_sync(0xffffffffu, to, o);
+            if (lane >= o) to += lower;
+        }
+        int base = 0;
+        if (lane == 0) base = atomicAdd(&listed, all);
+        return __shfl_sync(0xffffffffu, base, 0) + to - mine;
+    };
     if (warp < p.counting_warps) {
         const int counting = p.counting_warps * 32, me = threadIdx.x;
         if (p.history) {
             const int len = (int)min((long long)max(said, 0), p.history_ld);
             const int *h = p.history + (long long)row * p.history_ld;
-            auto seen = [&](int id) {
+            // Counts an id, or marks it as the prompt's; what was there before.
+            auto count_one = [&](int id, int i) -> unsigned {
                 const unsigned at = (unsigned)id - (unsigned)start;
-                if (at < (unsigned)tokens) count.set(lead + at, SEEN);
+                if (at >= (unsigned)tokens) return SEEN;
+                return i < prompt ? count.set(lead + at, SEEN) : count.add(lead + at);
             };
-            auto generated = [&](int id) {
-                const unsigned at = (unsigned)id - (unsigned)start;
-                if (at < (unsigned)tokens) count.add(lead + at);
-            };
-            auto either = [&](int id, int i) {
-                if (i < prompt) seen(id);
-                else generated(id);
+            auto is_first = [](unsigned before) { return (before & (SEEN | GENERATED)) == 0; };
+            auto alone = [&](int id, int i) {
+                if (is_first(count_one(id, i)) && LIST_AT_FIRST) list[atomicAdd(&listed, 1)] = (uint16_t)(lead + id - start);
             };
             const int lone = min(len, (int)(((16 - (reinterpret_cast<uintptr_t>(h) & 15)) & 15) / 4)), pieces = (len - lone) / 4;      // 16-byte pieces
-            if (me < lone) either(h[me], me);
-            constexpr int AT_ONCE = 4;
-            for (int q = me; q < pieces; q += AT_ONCE * counting) {
+            if (me < lone) alone(h[me], me);
+            constexpr int AT_ONCE = 4, PART = 2;             // pieces on their way, pieces whose atomics are
+            for (int q0 = warp * 32; q0 < pieces; q0 += AT_ONCE * counting) {
+                const int q = q0 + lane;
                 int4 ids[AT_ONCE];
 #pragma unroll
                 for (int n = 0; n < AT_ONCE; n++)
                     if (q + n * counting < pieces) ids[n] = __ldg(reinterpret_cast<const int4 *>(h + lone) + q + n * counting);
+                if constexpr (!LIST_AT_FIRST) {
 #pragma unroll
-                for (int n = 0; n < AT_ONCE; n++) {
-                    if (q + n * counting >= pieces) break;
-                    const int i = lone + 4 * (q + n * counting);
-                    if (i >= prompt) {
-                        generated(ids[n].x);
-                        generated(ids[n].y);
-                        generated(ids[n].z);
-                        generated(ids[n].w);
-                    } else {
-                        either(ids[n].x, i);
-                        either(ids[n].y, i + 1);
-                        either(ids[n].z, i + 2);
-                        either(ids[n].w, i + 3);
+                    for (int n = 0; n < AT_ONCE; n++) {
+                        const int piece = q + n * counting, i = lone + 4 * piece;
+                        if (piece >= pieces) break;
+                        count_one(ids[n].x, i);
+                        count_one(ids[n].y, i + 1);
+                        count_one(ids[n].z, i + 2);
+                        count_one(ids[n].w, i + 3);
+                    }
+                    continue;
+                }
+#pragma unroll
+                for (int n0 = 0; n0 < AT_ONCE; n0 += PART) {
+                    if (q0 + n0 * counting >= pieces) break;
+                    unsigned before[4 * PART], firsts = 0;
+#pragma unroll
+                    for (int n = 0; n < PART; n++) {
+                        const int piece = q + (n0 + n) * counting, i = lone + 4 * piece;
+                        const int4 id = ids[n0 + n];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) before[4 * n + k] = piece < pieces ? count_one(k == 0 ? id.x : k == 1 ? id.y : k == 2 ? id.z : id.w, i + k) : SEEN;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4 * PART; k++) firsts |= is_first(before[k]) ? 1u << k : 0u;
+                    const int mine = __popc(firsts), all = __reduce_add_sync(0xffffffffu, mine);
+                    if (all == 0) continue;
+                    int to = places(mine, all);
+#pragma unroll
+                    for (int n = 0; n < PART; n++) {
+                        const int4 id = ids[n0 + n];
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            if (firsts >> (4 * n + k) & 1u) list[to++] = (uint16_t)(lead + (k == 0 ? id.x : k == 1 ? id.y : k == 2 ? id.z : id.w) - start);
                     }
                 }
             }
             const int rest = lone + 4 * pieces + me;
-            if (rest < len) either(h[rest], rest);
+            if (rest < len) alone(h[rest], rest);
         }
         for (int e = b0 + me; e < b1; e += counting) {
             const unsigned at = (unsigned)p.bias_ids[e] - (unsigned)start;
@@ -555,28 +589,22 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 3 : 1) logits_kernel
     __syncthreads();                                         // counted and written
     // (in place, y still has x where the mask allows)
     auto allowed = [&](int v) { return !mask || __ldg(mask + (v >> 5)) >> (v & 31) & 1u; };
-    if (p.history) {
+    if (p.history && !LIST_AT_FIRST) {
         for (int at = threadIdx.x * 8; at - lane * 8 < p.window; at += THREADS * 8) {
             const unsigned marked = at < p.window ? count.said(at) : 0u;
             const int mine = __popc(marked), all = __reduce_add_sync(0xffffffffu, mine);
             if (all == 0) continue;
-            int to = mine;                                   // places up to and with this lane's
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int before = __shfl_up_sync(0xffffffffu, to, o);
-                if (lane >= o) to += before;
-            }
-            int base = 0;
-            if (lane == 0) base = atomicAdd(&listed, all);
-            to += __shfl_sync(0xffffffffu, base, 0) - mine;
+            int to = places(mine, all);
             for (unsigned left = marked; left; left &= left - 1) list[to++] = (uint16_t)(at + __ffs(left) - 1);
         }
         __syncthreads();
+    }
+    if (p.history)
         for (int n = threadIdx.x; n < listed; n += THREADS) {
             const int at = list[n], v = lo + at;
-            if (allowed(v)) store_f32(y + v, adjust(load_f32(x + v), count.get(at), 0.f, rep, pres, freq));
+            const unsigned c = count.get(at);
+            if (!(c & BIASED) && allowed(v)) store_f32(y + v, adjust(load_f32(x + v), c, 0.f, rep, pres, freq));
         }
-    }
     for (int e = b0 + threadIdx.x; e < b1; e += THREADS) {
         const int id = p.bias_ids[e];
         const unsigned at = (unsigned)id - (unsigned)start;
