@@ -73,7 +73,7 @@ struct GemmConfig {
     bool is_valid_for(int M, int N, int K) const
     {
         if (M <= 0 || N <= 0 || K <= 0) return false;
-        if (dt == GEMM_DT_W4A16 && bk == 32) return M <= bn && K % 32 == 0 && K <= 1 << 24;      // matrix-vector plugins (K must also be whole scale groups)
+        if (dt == GEMM_DT_W4A16 && bk == 32) return M <= bn && K % 32 == 0 && K <= 1 << 24 && N <= 1 << 30;      // matrix-vector plugins (K must also be whole scale groups)
         if (dt == GEMM_DT_W4A16) return M <= bn && N % 8 == 0 && K % 128 == 0;   // decode kernel, bn = padded M
         if (((long long)K * sm100::elem_bits(dt)) % 128 != 0 || N % 8 != 0) return false;
         if ((dt == GEMM_DT_MXFP8 || dt == GEMM_DT_W4A4) && K % bk != 0) return false;

@@ -182,6 +182,34 @@ def test_matvec_range(registry, cuda_device, shape, zeros):
                 assert Y[i].isnan().all()
 
 
+@pytest.mark.parametrize("rows", [8, 16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("k", [512, 2048 + 128, 128 * 9])
+def test_matvec_scales_and_zero_points_anywhere(registry, cuda_device, rows, group, k):
+    """Scales on any element and zero points on any byte, NaN around the scales: a row whose scales are NaN is NaN in its own
+    column alone, the first row, the last row and one behind a cut batch among them."""
+    n, t = 83, torch.bfloat16
+    for zeros in (False, True):
+        W, sc, zp, Wd = w4_weights(n, k, group, t, zeros, seed=k + group)
+        X = torch.randn((rows - 1, k), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(t)
+        for at in range(4):
+            buf = torch.full((sc.numel() + 16,), float("nan"), device="cuda", dtype=t)
+            s = buf[at:at + sc.numel()].view_as(sc)
+            s.copy_(sc)
+            z = None
+            if zeros:
+                zbuf = torch.full((zp.numel() + 16,), 255, device="cuda", dtype=torch.uint8)
+                z = zbuf[at:at + zp.numel()].view_as(zp)
+                z.copy_(zp)
+            check_matvec(matvec(matvec_plugin(registry, rows), X, W, s, z, group), X, Wd, group)
+            bad = [0, 17, 40, n - 1]
+            s[bad] = float("nan")
+            Y = matvec(matvec_plugin(registry, rows), X, W, s, z, group)
+            assert Y[:, bad].isnan().all()
+            good = [i for i in range(n) if i not in bad]
+            check_matvec(Y[:, good], X, Wd[good], group)
+
+
 def test_matvec_exact_integers(registry, cuda_device):
     """Small integers: every partial sum is exact in FP32, so the result is, whatever the order; 2^8 bounds it for bf16."""
     n, k = 77, 640
