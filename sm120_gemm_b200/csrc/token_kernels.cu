@@ -31,10 +31,14 @@ int refuse(const char *fmt, ...)
 
 bool aligned(const void *p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
-int launched()
+// The answer to a call whose CUDA call `what` said e.  Only that call's own status counts: the thread's last error may be an
+// older one of somebody else's, and this one does not stay behind for whoever asks next.
+int answer(cudaError_t e, const char *what)
 {
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) snprintf(g_message, sizeof(g_message), "launch failed: %s", cudaGetErrorString(e));
+    if (e != cudaSuccess) {
+        snprintf(g_message, sizeof(g_message), "%s failed: %s", what, cudaGetErrorString(e));
+        (void)cudaGetLastError();
+    }
     return (int)e;
 }
 
@@ -47,7 +51,7 @@ __device__ __forceinline__ void after_the_grid_before()
 }
 
 template <class... P, class... A>
-void launch_dependent(void (*kernel)(P...), dim3 grid, unsigned threads, unsigned smem, cudaStream_t st, const A &...args)
+int launch_dependent(void (*kernel)(P...), dim3 grid, unsigned threads, unsigned smem, cudaStream_t st, const A &...args)
 {
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -59,7 +63,7 @@ void launch_dependent(void (*kernel)(P...), dim3 grid, unsigned threads, unsigne
     cfg.stream = st;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, kernel, args...);       // its error, if any, is cudaGetLastError's: launched() reports it
+    return answer(cudaLaunchKernelEx(&cfg, kernel, args...), "launch");
 }
 
 // more shared memory than a kernel gets unasked (48 KB), once per kernel and device
@@ -83,8 +87,7 @@ int ask_for_shared(void (*kernel)(P...), int bytes)
             }
         if (e == cudaSuccess) return 0;      // (no place left to remember it)
     }
-    snprintf(g_message, sizeof(g_message), "cudaFuncSetAttribute failed: %s", cudaGetErrorString(e));
-    return (int)e;
+    return answer(e, "cudaFuncSetAttribute");
 }
 
 __device__ __forceinline__ float load_f32(const float *p) { return *p; }
@@ -225,11 +228,11 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p, const
 }
 
 template <class T, int P>
-void launch_rotary(RotaryParams p, int layout, const RotaryTable &table, cudaStream_t st)
+int launch_rotary(RotaryParams p, int layout, const RotaryTable &table, cudaStream_t st)
 {
     p.turned = p.rot / 2 / P;
     p.units = p.turned + (p.x == p.y ? 0 : (p.dim - p.rot + 2 * P - 1) / (2 * P));
-    if (p.units == 0) return;
+    if (p.units == 0) return 0;
     // heads per thread: as many as still leave 2048 threads for each SM, at most 10
     const double threads = (double)p.tokens * p.heads * p.units;
     int each = (int)fmin(fmax(threads / (148.0 * 2048), 1.0), 10.0);
@@ -240,13 +243,13 @@ void launch_rotary(RotaryParams p, int layout, const RotaryTable &table, cudaStr
     if (slice > (unsigned long long)p.tokens) slice = (unsigned long long)p.tokens;
     p.per_slice = (unsigned)slice;
     const dim3 grid((unsigned)((slice * row + 255) / 256), (unsigned)((p.tokens + slice - 1) / slice));
-    if (layout == GEMM_ROTARY_INTERLEAVED) launch_dependent(rotary_kernel<T, P, true>, grid, 256, 0, st, p, table);
-    else launch_dependent(rotary_kernel<T, P, false>, grid, 256, 0, st, p, table);
+    if (layout == GEMM_ROTARY_INTERLEAVED) return launch_dependent(rotary_kernel<T, P, true>, grid, 256, 0, st, p, table);
+    return launch_dependent(rotary_kernel<T, P, false>, grid, 256, 0, st, p, table);
 }
 
 // the widest pieces that every row, every head and both halves of the pairs are aligned to
 template <class T>
-void launch_rotary_wide(const RotaryParams &p, int layout, const RotaryTable &table, cudaStream_t st)
+int launch_rotary_wide(const RotaryParams &p, int layout, const RotaryTable &table, cudaStream_t st)
 {
     const size_t bits = reinterpret_cast<uintptr_t>(p.x) | reinterpret_cast<uintptr_t>(p.y) |
                         (size_t)(p.x_token | p.x_head | p.y_token | p.y_head) * sizeof(T);
@@ -254,9 +257,9 @@ void launch_rotary_wide(const RotaryParams &p, int layout, const RotaryTable &ta
     auto fits = [&](int n) { return bits % (n * sizeof(T)) == 0 && each % n == 0; };
     if constexpr (sizeof(T) == 2)
         if (fits(8)) return launch_rotary<T, 8>(p, layout, table, st);
-    if (fits(4)) launch_rotary<T, 4>(p, layout, table, st);
-    else if (fits(2)) launch_rotary<T, 2>(p, layout, table, st);
-    else launch_rotary<T, 1>(p, layout, table, st);
+    if (fits(4)) return launch_rotary<T, 4>(p, layout, table, st);
+    if (fits(2)) return launch_rotary<T, 2>(p, layout, table, st);
+    return launch_rotary<T, 1>(p, layout, table, st);
 }
 
 // The frequency table of a set of parameters, kept per thread (the last few sets): a value of its key alone.
@@ -635,8 +638,7 @@ int launch_logits(LogitsParams p, cudaStream_t st)
     const int listed = (int)(p.history_ld < p.window ? p.history_ld : p.window);       // more different tokens were not said
     const int rc = ask_for_shared(logits_kernel<TX, TY, NARROW, THREADS>, MOST * ((NARROW ? 2 : 4) + 2));
     if (rc != 0) return rc;
-    launch_dependent(logits_kernel<TX, TY, NARROW, THREADS>, dim3((unsigned)ctas), THREADS, p.window * (NARROW ? 2 : 4) + listed * 2, st, p);
-    return launched();
+    return launch_dependent(logits_kernel<TX, TY, NARROW, THREADS>, dim3((unsigned)ctas), THREADS, p.window * (NARROW ? 2 : 4) + listed * 2, st, p);
 }
 
 template <class TX, class TY>
@@ -702,10 +704,9 @@ int gemm_rotary(const GemmRotaryArgs *a)
     p.scale = a->scale;
     const RotaryTable &table = *rotary_table(key);
     cudaStream_t st = static_cast<cudaStream_t>(a->stream);
-    if (a->dtype == GEMM_X_BF16) launch_rotary_wide<__nv_bfloat16>(p, a->layout, table, st);
-    else if (a->dtype == GEMM_X_F16) launch_rotary_wide<__half>(p, a->layout, table, st);
-    else launch_rotary_wide<float>(p, a->layout, table, st);
-    return launched();
+    if (a->dtype == GEMM_X_BF16) return launch_rotary_wide<__nv_bfloat16>(p, a->layout, table, st);
+    if (a->dtype == GEMM_X_F16) return launch_rotary_wide<__half>(p, a->layout, table, st);
+    return launch_rotary_wide<float>(p, a->layout, table, st);
 }
 
 int gemm_logits(const GemmLogitsArgs *a)
