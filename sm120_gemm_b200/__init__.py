@@ -226,16 +226,22 @@ class KernelRegistry:
                 return k
         return None
 
-    def heuristic(self, M: int, N: int, K: int, dt: str = "bf16") -> LoadedKernel | None:
-        """The loaded plugin with the smallest modelled time for the shape (no measurement, no cache)."""
-        c = heuristic_config([k.config for k in self.kernels], dt, M, N, K)
+    def heuristic(self, M: int, N: int, K: int, dt: str = "bf16", *, group_size: int = 0, x_dtype: int = X_BF16, zero_points: bool = False,
+                  transform: bool = False) -> LoadedKernel | None:
+        """The loaded plugin with the smallest modelled time for the shape (no measurement, no cache) that takes a call of
+        this kind: ``group_size`` (0: not said), ``x_dtype``, zero points and an output transform as in ``GemmArgs``; None
+        when there is none."""
+        c = heuristic_config([k.config for k in self.kernels], dt, M, N, K, group_size=group_size, x_dtype=x_dtype, zero_points=zero_points, transform=transform)
         return self.find(c.name()) if c else None
 
-    def select(self, cache: "AutotuneCache", M: int, N: int, K: int, dt: str = "bf16", gpus: int = 1) -> LoadedKernel | None:
-        """Dispatch without autotuning: the cache entry when there is one (and its plugin is loaded), else the heuristic pick."""
+    def select(self, cache: "AutotuneCache", M: int, N: int, K: int, dt: str = "bf16", gpus: int = 1, *, group_size: int = 0, x_dtype: int = X_BF16,
+               zero_points: bool = False, transform: bool = False) -> LoadedKernel | None:
+        """Dispatch without autotuning: the cache entry when there is one (and its plugin is loaded and takes a call of this
+        kind), else the heuristic pick."""
+        kind = dict(group_size=group_size, x_dtype=x_dtype, zero_points=zero_points, transform=transform)
         hit = cache.lookup(M, N, K, dt, gpus)
         k = self.find(hit[0].name()) if hit else None
-        return k or self.heuristic(M, N, K, dt)
+        return k if k and k.config.takes(K, **kind) else self.heuristic(M, N, K, dt, **kind)
 
 
 class AutotuneCache:

@@ -39,6 +39,15 @@ inline int dtype_from_name(const char *s)
 inline int elem_bits(int dt) { return dt == GEMM_DT_BF16 || dt == GEMM_DT_W4A16 ? 16 : dt == GEMM_DT_W4A4 ? 4 : 8; }
 }  // namespace sm100
 
+// What a call is beyond its shape, where the plugins of a data type differ in what they take (GemmArgs.group_size, x_dtype,
+// w_zero, and whether alpha / beta / C / bias / activation / y_dtype / amax are used).
+struct GemmCallKind {
+    int group_size = 0;               // W4A16; 0: not said, whatever the plugin's
+    int x_dtype = GEMM_X_BF16;
+    bool zero_points = false;
+    bool transform = false;
+};
+
 struct GemmConfig {
     int dt = GEMM_DT_BF16;  // GEMM_DT_*
     int bm = 128, bn = 128, bk = 64, num_stages = 4;
@@ -79,6 +88,16 @@ struct GemmConfig {
         if ((dt == GEMM_DT_MXFP8 || dt == GEMM_DT_W4A4) && K % bk != 0) return false;
         if (split_k > 1 && (K % bk != 0 || (K / bk) % split_k != 0)) return false;
         return true;
+    }
+
+    // Whether the plugin takes calls of this kind (with any reduction length the shape rules allow, when no group is said).
+    bool takes(const GemmCallKind &kind, int K) const
+    {
+        if (kind.transform && epi != 2) return false;
+        if (dt == GEMM_DT_W4A16 && bk == 32 && (kind.x_dtype == GEMM_X_BF16 || kind.x_dtype == GEMM_X_F16))
+            return kind.group_size == 0 || ((kind.group_size == 32 || kind.group_size == 64 || kind.group_size == 128) && K % kind.group_size == 0);
+        if (kind.x_dtype != GEMM_X_BF16 || kind.zero_points) return false;
+        return dt != GEMM_DT_W4A16 || kind.group_size == 0 || kind.group_size == 128;
     }
 
     // Dynamic shared memory of the dense kernel (must equal UmmaGemmTraits::SMEM_ALLOC;
@@ -359,15 +378,15 @@ inline double heuristic_ms(const GemmConfig &c, int M, int N, int K, int sms = 1
     return (t + launch_us * 1e-6) * 1e3;
 }
 
-// The loaded plugin of data type `dt` with the smallest modelled time for the shape (fused-transform plugins
-// are left out: they compute the same product and are asked for by name); nullptr when none can run it.
-inline const LoadedKernel *heuristic_kernel(const KernelRegistry &reg, int dt, int M, int N, int K, int sms = 148)
+// The loaded plugin of data type `dt` with the smallest modelled time for the shape, among those that take a call of this
+// kind (fused-transform plugins for calls with a transform, the others for calls without); nullptr when there is none.
+inline const LoadedKernel *heuristic_kernel(const KernelRegistry &reg, int dt, int M, int N, int K, int sms = 148, const GemmCallKind &kind = {})
 {
     const LoadedKernel *best = nullptr;
     double best_ms = 0;
     std::string best_name;
     for (const auto &k : reg.kernels) {
-        if (k.config.dt != dt || k.config.epi == 2 || !k.can_run(M, N, K)) continue;
+        if (k.config.dt != dt || (k.config.epi == 2) != kind.transform || !k.config.takes(kind, K) || !k.can_run(M, N, K)) continue;
         const double ms = heuristic_ms(k.config, M, N, K, sms);
         const std::string name = k.config.name();
         if (!best || ms < best_ms || (ms == best_ms && name < best_name)) { best = &k; best_ms = ms; best_name = name; }
@@ -375,10 +394,11 @@ inline const LoadedKernel *heuristic_kernel(const KernelRegistry &reg, int dt, i
     return best;
 }
 
-// dispatch for callers that do not autotune: the cache entry when there is one, else the heuristic pick
-inline const LoadedKernel *select_kernel(const KernelRegistry &reg, const AutotuneCache &cache, int dt, int M, int N, int K, int gpus = 1)
+// dispatch for callers that do not autotune: the cache entry when there is one and its plugin takes the call, else the
+// heuristic pick
+inline const LoadedKernel *select_kernel(const KernelRegistry &reg, const AutotuneCache &cache, int dt, int M, int N, int K, int gpus = 1, const GemmCallKind &kind = {})
 {
     if (auto hit = cache.lookup(M, N, K, dt, gpus))
-        if (const LoadedKernel *k = reg.find(hit->config.name())) return k;
-    return heuristic_kernel(reg, dt, M, N, K);
+        if (const LoadedKernel *k = reg.find(hit->config.name()); k && k->config.takes(kind, K)) return k;
+    return heuristic_kernel(reg, dt, M, N, K, 148, kind);
 }

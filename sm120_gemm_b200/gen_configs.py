@@ -115,6 +115,16 @@ class GemmConfig:
                 return False
         return True
 
+    def takes(self, K: int, group_size: int = 0, x_dtype: int = 0, zero_points: bool = False, transform: bool = False) -> bool:
+        """Whether the plugin takes calls of this kind (GemmConfig::takes of csrc/gemm_config.h; group_size 0: not said)."""
+        if transform and self.epi != 2:
+            return False
+        if self.dt == "w4a16" and self.bk == 32 and x_dtype in (0, 1):
+            return group_size == 0 or (group_size in (32, 64, 128) and K % group_size == 0)
+        if x_dtype != 0 or zero_points:
+            return False
+        return self.dt != "w4a16" or group_size in (0, 128)
+
     def defines(self) -> list[str]:
         return [f"-DGEMM_DT={DT_IDS[self.dt]}", f"-DGEMM_BN={self.bn}", f"-DGEMM_STAGES={self.num_stages}",
                 f"-DGEMM_CG={self.cg}", f"-DGEMM_SK={self.split_k}", f"-DGEMM_AB={self.swap_ab}",
@@ -166,12 +176,13 @@ def heuristic_ms(c: GemmConfig, M: int, N: int, K: int, sms: int = 148) -> float
     return (t + launch_us * 1e-6) * 1e3
 
 
-def heuristic_config(configs, dt: str, M: int, N: int, K: int, sms: int = 148):
-    """The configuration of `configs` with the smallest modelled time for the shape, for callers that do not
-    autotune (the reference skips shapes that are missing from its cache, src/bench.cu:455-458)."""
+def heuristic_config(configs, dt: str, M: int, N: int, K: int, sms: int = 148, **kind):
+    """The configuration of `configs` with the smallest modelled time for the shape among those that take a call of this
+    kind (GemmConfig.takes), for callers that do not autotune (the reference skips shapes that are missing from its
+    cache, src/bench.cu:455-458)."""
     best = None
     for c in configs:
-        if c.dt != dt or c.epi == 2 or not c.is_valid_for(M, N, K):
+        if c.dt != dt or (c.epi == 2) != kind.get("transform", False) or not c.takes(K, **kind) or not c.is_valid_for(M, N, K):
             continue
         key = (heuristic_ms(c, M, N, K, sms), c.name())
         if best is None or key < best[0]:
