@@ -95,9 +95,10 @@ inline int device_info(DeviceInfo **out)
             SM100_CUDA_TRY(cudaDeviceGetAttribute(&d.cc_major, cudaDevAttrComputeCapabilityMajor, dev));
             if (d.cc_major != 10)
                 return set_error(GEMM_ERR_CUDA, "device %d is compute capability %d.x; this library runs on sm_100 only", dev, d.cc_major);
+            // (a module's variables are zero when it is loaded: a memset here would be a legacy-stream operation, which a
+            // call that is the first under stream capture may not make)
             void *p = nullptr;
             SM100_CUDA_TRY(cudaGetSymbolAddress(&p, g_status_block));
-            SM100_CUDA_TRY(cudaMemset(p, 0, sizeof(uint32_t) * 4));
             d.status = static_cast<uint32_t *>(p);
             SM100_CUDA_TRY(cudaGetSymbolAddress(&p, g_wave_sync));
             d.wave_sync = static_cast<uint32_t *>(p);

@@ -37,12 +37,15 @@
 // Measured (us, device time of back-to-back calls, weights from HBM; groups of 128, bf16): 28672 x 8192 by 1 / 4 / 8 / 9 / 16 rows
 // 26.7 / 29.5 / 30.5 / 39.7 / 51; 4096 x 14336 12.4 / 13.5 / 15.0 / 18.1 / 19.7; 8192 x 28672 31.2 / 31.5 / 32.9 / 47 / 56.
 // One row is bound by the bytes (slope 6.3 TB/s) and 5 us of start, staging and end; 16 rows by the tensor and logic
-// instructions that two warps per scheduler issue (the tcgen05 tiles of the bk128 plugins take 46, 19.4 and 46 us for any M).
+// instructions that two warps per scheduler issue (the tcgen05 tiles of the bk128 plugins take 46, 19.4 and 46 us for any M:
+// calls that those take, and that give the workspace, are handed to them, w4_choice.h).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include "bf16_gemm.cuh"
+#include "w4_choice.h"
+#include "w4a16_tmem_gemm.cuh"
 
 namespace sm100 {
 
@@ -705,7 +708,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
 template <class T>
 struct W4MatvecLauncher {
     static bool can_run(int M, int N, int K) { return M >= 1 && M <= T::MPAD && N >= 1 && N <= 1 << 30 && K >= 32 && K % 32 == 0 && K <= 1 << 24; }
-    // the family's figure, so that one workspace serves whichever W4A16 plugin is picked; nothing here touches it
+    // the family's figure, so that one workspace serves whichever W4A16 plugin is picked
     static size_t workspace_bytes(int, int, int) { return (size_t)2 * STREAMK_MAX_CTAS * 128 * 128 * sizeof(float); }
 
     static int run(const GemmArgs &a)
@@ -723,6 +726,18 @@ struct W4MatvecLauncher {
             return set_error(GEMM_ERR_ARG, "alpha / beta*C / bias / activation need a fused-epilogue configuration (e2)");
         if (a.activation < ACT_NONE || a.activation > ACT_SILU) return set_error(GEMM_ERR_ARG, "unknown activation %d", a.activation);
         if (a.beta != 0.f && !a.C) return set_error(GEMM_ERR_ARG, "beta != 0 needs C");
+        // What the tensor-memory kernel does faster goes to it where the call is one that its plugins take, workspace included.
+        if constexpr (T::MPAD > 8 && T::EPI != EPI_FUSED) {
+            using Other = W4A16TmemLauncher<W4A16TmemTraits<16, 6>>;
+            if (a.x_dtype == GEMM_X_BF16 && !a.w_zero && a.group_size == 128 && a.workspace && bits(a.workspace) % 16 == 0 &&
+                (a.workspace_bytes == 0 || a.workspace_bytes >= workspace_bytes(a.M, a.N, a.K)) && Other::can_run(a.M, a.N, a.K)) {
+                int sms = 0;
+                const int rc = sm_count(&sms);
+                if (rc != GEMM_OK) return rc;
+                if (w4_tensor_memory_wins(a.M, a.N, a.K, a.sm_limit > 0 && a.sm_limit < sms ? a.sm_limit : sms))
+                    return Other::run(a.M, a.N, a.K, a.X, a.W, a.Y, a.w_scale, a.group_size, static_cast<float *>(a.workspace), a.workspace_bytes, a.sm_limit, a.stream);
+            }
+        }
         W4MatvecParams p;
         p.M = a.M; p.N = a.N; p.K = a.K;
         p.group_shift = a.group_size == 32 ? 5 : a.group_size == 64 ? 6 : 7;

@@ -1,0 +1,94 @@
+"""Calls of up to 16 rows that the tensor-memory W4A16 plugins take too -- bf16, signed weights in groups of 128, the family's
+workspace -- through the dispatcher: no slower and no different from what those plugins give."""
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+import sm120_gemm_b200 as g
+from test_gpu_decode import check_matvec, matvec, w4_weights
+from test_gpu_decode_rows import graph_us
+
+pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+TM = "w4a16_bm128_bn16_bk128_s6_cg1_sk0_ab1_e0"
+
+
+def workspace():
+    return torch.empty(2 * 160 * 128 * 128, device="cuda")
+
+
+@pytest.mark.parametrize("m, n, k", [(16, 28672, 8192), (13, 28672, 8192), (9, 8192, 28672), (12, 12568, 15232), (16, 14336, 4096)])
+def test_large_plain_calls_give_what_the_tensor_memory_plugin_gives(registry, cuda_device, m, n, k):
+    W, sc, _, Wd = w4_weights(n, k, 128, torch.bfloat16, False, seed=1)
+    X = torch.randn((m, k), device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).bfloat16()
+    ws = workspace()
+    ref = matvec(registry.find(TM), X, W, sc, None, 128, workspace=ws, workspace_bytes=ws.numel() * 4)
+    pick = registry.heuristic(m, n, k, "w4a16")
+    assert torch.equal(matvec(pick, X, W, sc, None, 128, workspace=ws, workspace_bytes=ws.numel() * 4), ref)
+    assert torch.equal(matvec(pick, X, W, sc, None, 128, workspace=ws), ref)                  # a size of 0 is not checked
+    said = registry.heuristic(m, n, k, "w4a16", group_size=128)
+    assert torch.equal(matvec(said, X, W, sc, None, 128, workspace=ws), ref)
+    # without a workspace, or with one that is too small, and for every other kind: the matrix-vector kernel
+    check_matvec(matvec(pick, X, W, sc, None, 128), X, Wd, 128)
+    check_matvec(matvec(pick, X, W, sc, None, 128, workspace=ws, workspace_bytes=1024), X, Wd, 128)
+    for kw, group, t in (({}, 64, torch.bfloat16), ({}, 128, torch.float16)):
+        W2, sc2, zp2, Wd2 = w4_weights(n, k, group, t, True, seed=3)
+        check_matvec(matvec(pick, X.to(t), W2, sc2, zp2, group, workspace=ws), X.to(t), Wd2, group)
+        del W2, Wd2
+
+
+@pytest.mark.parametrize("limit", [1, 40])
+def test_few_sms(registry, cuda_device, limit):
+    m, n, k = 14, 4096, 2048
+    W, sc, _, Wd = w4_weights(n, k, 128, torch.bfloat16, False, seed=1)
+    X = torch.randn((m, k), device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).bfloat16()
+    check_matvec(matvec(registry.heuristic(m, n, k, "w4a16"), X, W, sc, None, 128, workspace=workspace(), sm_limit=limit), X, Wd, 128)
+
+
+@pytest.mark.parametrize("m, n, k", [(16, 28672, 8192), (16, 8192, 28672), (13, 5056, 24704), (16, 4096, 14336), (16, 4096, 4096), (9, 28672, 8192)])
+def test_plain_calls_are_no_slower_than_before(registry, cuda_device, m, n, k):
+    """Against the plugin that such calls had before the matrix-vector plugins: ranked by the name alone, these took up to 1.46
+    times as long (13 x 5056 x 24704).  Weights from memory: four matrices in turn; 1.12: the rule's own 10 %, and the clock."""
+    Ws = [w4_weights(n, k, 128, torch.bfloat16, False, seed=s)[:2] for s in range(4 if n * k < 1 << 27 else 2)]
+    X = torch.randn((m, k), device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).bfloat16()
+    Y, ws = torch.empty((m, n), device="cuda", dtype=torch.bfloat16), workspace()
+
+    def turn(plugin):
+        return lambda: [matvec(plugin, X, W, sc, None, 128, Y=Y, workspace=ws) for W, sc in Ws]
+
+    before, now, said = (graph_us(turn(p), 10) for p in (registry.find(TM), registry.heuristic(m, n, k, "w4a16"), registry.heuristic(m, n, k, "w4a16", group_size=128)))
+    assert now <= 1.12 * before and said <= 1.12 * before, (before, now, said)
+
+
+FIRST_CALL = """
+import sys, torch
+sys.path[:0] = [{root!r}, {tests!r}]
+import sm120_gemm_b200 as g
+from test_gpu_decode import matvec, w4_weights
+reg = g.KernelRegistry()
+reg.load_dir(dt="w4a16")
+m, n, k = 16, 28672, 8192
+W, sc, _, _ = w4_weights(n, k, 128, torch.bfloat16, False, seed=1)
+X = torch.randn((m, k), device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).bfloat16()
+Y, ws = torch.zeros((m, n), device="cuda", dtype=torch.bfloat16), torch.empty(2 * 160 * 128 * 128, device="cuda")
+kernel = reg.heuristic(m, n, k, "w4a16")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    matvec(kernel, X, W, sc, None, 128, Y=Y, workspace=ws if {with_workspace} else None)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(Y, matvec(kernel, X, W, sc, None, 128, workspace=ws if {with_workspace} else None)) and Y.abs().sum() > 0
+kernel.check_status()
+"""
+
+
+@pytest.mark.parametrize("with_workspace", [True, False])
+def test_the_first_call_may_be_captured(cuda_device, with_workspace):
+    """In a process of its own: nothing has been called before the capture begins."""
+    script = FIRST_CALL.format(root=ROOT, tests=os.path.join(ROOT, "tests"), with_workspace=with_workspace)
+    r = subprocess.run([sys.executable, "-c", script], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
