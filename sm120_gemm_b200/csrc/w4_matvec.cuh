@@ -69,6 +69,7 @@ struct W4MatvecParams {
     int part_at;                 // partial sums: byte offset in shared memory
     uint32_t step_batch, step_w, step_s, step_z;         // bytes from a warp's batch of W to its next; from a warp's tile to its next
     const uint8_t *scales_end, *zeros_end;       // behind the word (4-byte aligned) that holds the last
+    int infinities;              // an infinite x gives w * x (bf16, signed, groups of 128); else it makes its row NaN
 };
 
 // What depends on the 16-bit type: the matrix instruction m16n8k16 (D = A * B + C, C and D FP32), and the scaling of X.
@@ -239,7 +240,7 @@ struct W4Rows {
     float up[16];        // staged x = x * up * 2^K_USUAL
     float down[16];      // 1 / up
     int ordinary[16];    // some |x| is at least 2^-40 (bf16)
-    int top[16];         // largest finite exponent field
+    int top[16];         // largest finite exponent field; then whether the row has an infinity that was left out
 };
 
 // Staging of `nu` units of X from unit u0 on ([m][unit][32 k][c]: 8 values, 16 bytes; x behind K is 0).  A thread copies its
@@ -268,7 +269,7 @@ __device__ __forceinline__ void w4_copy_x(const W4MatvecParams &p, uint32_t xs, 
 // Returns what this thread saw of X that the usual scaling may not do for (bf16): an |x| of 2^19 or more; a row that is not
 // zero and whose |x| are all below 2^-40, as far as this thread sees it.
 constexpr unsigned W4_FAR = 1, W4_TINY = 2;
-template <class E, int WARPS, class T>
+template <class E, int WARPS, bool INFINITIES, class T>
 __device__ __forceinline__ unsigned w4_order_x(const W4MatvecParams &p, uint8_t *xs, W4Rows *rows, int nu, bool usual, int warp, int lane)
 {
     constexpr int AT_ONCE = 4;                       // rows side by side: each piece is a round trip to shared memory
@@ -294,7 +295,14 @@ __device__ __forceinline__ unsigned w4_order_x(const W4MatvecParams &p, uint8_t 
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         most[j] = W4Type<E>::max_abs2(most[j], q[i]);
-                        if (!usual) q[i] = W4Type<E>::mul2(q[i], up[j]);
+                        if (!usual) {
+                            if (INFINITIES && p.infinities) {        // w4_add_infinities sees to them
+                                const uint32_t low = (q[i] & 0x7fffu) == 0x7f80u ? 0xffffu : 0u, high = (q[i] & 0x7fff0000u) == 0x7f800000u ? 0xffff0000u : 0u;
+                                if (low | high) rows->top[m0 + j] = 1;
+                                q[i] &= ~(low | high);
+                            }
+                            q[i] = W4Type<E>::mul2(q[i], up[j]);
+                        }
                         q[i] = W4Type<E>::mul2(q[i], W4Type<E>::TWO_K_USUAL);
                     }
                 }
@@ -340,7 +348,7 @@ __device__ __forceinline__ void w4_sum_x(const uint8_t *smem, const uint32_t (&x
 }
 
 // The rows' scaling from their largest finite values in this pass (bf16 only; rare): brings them to 2^119 .. 2^120.
-template <class E, int THREADS, class T>
+template <class E, int THREADS, bool INFINITIES, class T>
 __device__ __forceinline__ void w4_rescale_rows(const W4MatvecParams &p, W4Rows *rows, int u0, int nu)
 {
     if (threadIdx.x < 16) rows->top[threadIdx.x] = 0;
@@ -361,8 +369,39 @@ __device__ __forceinline__ void w4_rescale_rows(const W4MatvecParams &p, W4Rows 
         const int e = max(rows->top[threadIdx.x], 1) - 127, k = min(119 - e, 190) - W4Type<E>::K_USUAL;
         rows->up[threadIdx.x] = w4_power_of_two(k);
         rows->down[threadIdx.x] = w4_power_of_two(-k);
+        if (INFINITIES) rows->top[threadIdx.x] = 0;
     }
     __syncthreads();
+}
+
+// What the infinities of this pass's X give, w * x each (0 * inf is NaN), into the partial sums of the first slice: the sums
+// themselves are of u * x and 8 x, which for an infinity have no difference.  Signed weights in groups of 128, any row of
+// X that is flagged; every thread looks through the row again for its own rows of W.
+template <int THREADS, class T>
+__device__ __forceinline__ void w4_add_infinities(const W4MatvecParams &p, const W4Rows *rows, float *part, int row0, int count, int u0, int nu)
+{
+    const int first = u0 * T::UNIT / 8, last = min(first + nu * T::UNIT / 8, p.K / 8);        // pieces of 8 x
+    for (int m = 0; m < p.M; m++) {
+        if (!rows->top[m]) continue;
+        const uint4 *X = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p.X) + (size_t)m * p.K);
+        for (int r = threadIdx.x; r < count; r += THREADS) {
+            const size_t n = row0 + r;
+            float sum = 0.f;
+            for (int at = first; at < last; at++) {
+                const uint4 v = X[at];
+                const uint32_t q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const uint32_t x = q[i / 2] << (i % 2 ? 0 : 16) & 0xffff0000u;
+                    if ((x & 0x7fff0000u) != 0x7f800000u) continue;
+                    const int k = at * 8 + i;
+                    const int w = (int)((p.W[n * (p.K / 2) + k / 2] >> 4 * (k % 2) & 15) ^ 8) - 8;
+                    sum = fmaf(__bfloat162float(static_cast<const __nv_bfloat16 *>(p.scales)[n * p.groups + k / 128]), (float)w * __uint_as_float(x), sum);
+                }
+            }
+            part[m * p.block_rows + r] += sum;
+        }
+    }
 }
 
 // WHOLE: K is whole batches and the scales and zero points are aligned like them, so that nothing is cut and every row's
@@ -373,6 +412,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
     constexpr int NB = T::NB, WARPS = T::WARPS, THREADS = T::THREADS, SUBTILES = T::SUBTILES, TILE = T::TILE;
     constexpr int LANES_PER_ROW = 32 / TILE;             // that bring its scales and zero points
     constexpr int GROUP_SUBS = 4 / GPU;                  // pieces of 32 k in a group
+    constexpr bool INFINITIES = W4Type<E>::RESCALE && GPU == 1 && !ZERO && T::EPI != EPI_FUSED;        // that calls may ask for
     constexpr int STEPS = GPU <= 2 ? 2 : 4, SUBS = 8 / STEPS, GROUPS = 2 * GPU / STEPS;      // steps of a batch, pieces and groups of a step
     constexpr int SLOT = T::slot_bytes(GPU), SCALES_AT = 2 * T::UNIT_BYTES, SCALE_PITCH = T::scale_pitch(GPU), ZEROS_AT = SCALES_AT + TILE * SCALE_PITCH;
     constexpr int RING_BYTES = T::RING * SLOT;           // of a warp
@@ -514,6 +554,7 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
                 if (threadIdx.x < 16) {
                     xrows->ordinary[threadIdx.x] = 0;
                     xrows->down[threadIdx.x] = 1.f;
+                    if (INFINITIES) xrows->top[threadIdx.x] = 0;
                 }
                 w4_copy_x<WARPS, T>(p, smem_u32(smem + X_AT), u0, 2 * batches, warp, lane);
             }
@@ -523,14 +564,14 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
                 __syncthreads();                     // the flags
 #pragma unroll 1
                 for (bool usual = true;; usual = false) {
-                    const unsigned unusual = w4_order_x<E, WARPS, T>(p, smem + X_AT, xrows, 2 * batches, usual, warp, lane);
+                    const unsigned unusual = w4_order_x<E, WARPS, INFINITIES, T>(p, smem + X_AT, xrows, 2 * batches, usual, warp, lane);
                     bool again = __syncthreads_or(unusual) && W4Type<E>::RESCALE && usual;
                     if (again && !__syncthreads_or(unusual & W4_FAR)) {
                         again = false;
                         for (int m = 0; m < M; m++) again = again || !xrows->ordinary[m];
                     }
                     if (!again) break;
-                    w4_rescale_rows<E, THREADS, T>(p, xrows, u0, nu);
+                    w4_rescale_rows<E, THREADS, INFINITIES, T>(p, xrows, u0, nu);
                     w4_copy_x<WARPS, T>(p, smem_u32(smem + X_AT), u0, 2 * batches, warp, lane);
                     w4_copies_wait<0>();
                 }
@@ -684,6 +725,10 @@ __global__ void __launch_bounds__(T::THREADS, 1) w4_matvec_kernel(const W4Matvec
                 }
             }
             w4_copies_wait<0>();
+            if (INFINITIES && __any_sync(0xffffffffu, xrows->top[lane & 15])) {
+                __syncthreads();                         // the partial sums
+                w4_add_infinities<THREADS, T>(p, xrows, part, row0, rows, u0, nu);
+            }
         }
         // every CTA of the cluster adds up a part of the results: the slices of the first, of the second ...
         const uint32_t part_addr = smem_u32(part), slice = M * p.block_rows * sizeof(float);
@@ -727,10 +772,12 @@ struct W4MatvecLauncher {
         if (a.activation < ACT_NONE || a.activation > ACT_SILU) return set_error(GEMM_ERR_ARG, "unknown activation %d", a.activation);
         if (a.beta != 0.f && !a.C) return set_error(GEMM_ERR_ARG, "beta != 0 needs C");
         // What the tensor-memory kernel does faster goes to it where the call is one that its plugins take, workspace included.
+        // Whichever kernel does it, an infinite x then gives what it gives there.
+        using Other = W4A16TmemLauncher<W4A16TmemTraits<16, 6>>;
+        const bool common = T::EPI != EPI_FUSED && a.x_dtype == GEMM_X_BF16 && !a.w_zero && a.group_size == 128 && a.workspace && bits(a.workspace) % 16 == 0 &&
+                            (a.workspace_bytes == 0 || a.workspace_bytes >= workspace_bytes(a.M, a.N, a.K)) && Other::can_run(a.M, a.N, a.K);
         if constexpr (T::MPAD > 8 && T::EPI != EPI_FUSED) {
-            using Other = W4A16TmemLauncher<W4A16TmemTraits<16, 6>>;
-            if (a.x_dtype == GEMM_X_BF16 && !a.w_zero && a.group_size == 128 && a.workspace && bits(a.workspace) % 16 == 0 &&
-                (a.workspace_bytes == 0 || a.workspace_bytes >= workspace_bytes(a.M, a.N, a.K)) && Other::can_run(a.M, a.N, a.K)) {
+            if (common) {
                 int sms = 0;
                 const int rc = sm_count(&sms);
                 if (rc != GEMM_OK) return rc;
@@ -739,6 +786,7 @@ struct W4MatvecLauncher {
             }
         }
         W4MatvecParams p;
+        p.infinities = common;
         p.M = a.M; p.N = a.N; p.K = a.K;
         p.group_shift = a.group_size == 32 ? 5 : a.group_size == 64 ? 6 : 7;
         p.groups = a.K / a.group_size;

@@ -81,3 +81,46 @@ def test_zero_rows_take_no_longer(registry, cuda_device, m, pad, n, k):
     plugin = matvec_plugin(registry, 8 if m <= 8 else 16)
     full, padded = (graph_us(lambda x=x: matvec(plugin, x, W, sc, zp, 128, Y=Y)) for x in (X, P))
     assert padded <= 1.25 * full, (padded, full)
+
+
+@pytest.mark.parametrize("m, n, k", [(1, 4096, 4096), (7, 200, 28672), (8, 1000, 1024 + 128), (5, 8, 128), (3, 30000, 640), (16, 304, 65536), (12, 4096, 3968), (9, 64, 131072), (16, 4096, 8192)])
+def test_infinities_in_calls_that_the_tensor_memory_plugin_takes(registry, cuda_device, m, n, k):
+    """bf16, signed weights in groups of 128, the family's workspace: an infinite x gives the sum of w * x, as it did before these
+    plugins -- infinities of either sign, NaN where a weight or a scale is 0 or two signs meet -- and leaves the other rows alone."""
+    rows = 8 if m <= 8 else 16
+    W, sc, _, Wd = w4_weights(n, k, 128, torch.bfloat16, False, seed=31)
+    sc[3] = 0
+    Wd[3] = 0
+    X = torch.randn((m, k), device="cuda", generator=torch.Generator(device="cuda").manual_seed(32)).bfloat16()
+    plain = X.clone()
+    inf = float("inf")
+    X[0, k // 2] = inf
+    if m > 2:
+        X[1, k - 1], X[2, 0], X[2, k - 1] = -inf, inf, inf
+    if m > 4:
+        X[3, :] = inf
+        X[4, 64], X[4, 65] = inf, float("nan")
+    if m > 6:
+        X[5] *= 2.0 ** 60                # finite, by its own scaling; row 6 is ordinary
+    if m > 8:
+        X[7, k // 3], X[8] = inf, 0
+    ws = torch.empty(2 * 160 * 128 * 128, device="cuda")
+    Y = matvec(matvec_plugin(registry, rows), X, W, sc, None, 128, workspace=ws, workspace_bytes=ws.numel() * 4)
+    before = matvec(registry.find("w4a16_bm128_bn16_bk128_s6_cg1_sk0_ab1_e0"), X, W, sc, None, 128, workspace=ws)
+    good = []
+    for r in range(m):
+        x = X[r].double()
+        far = (~x.isfinite()).nonzero().flatten()
+        if len(far) == 0:
+            good.append(r)
+            continue
+        want = (Wd[:, far] * x[far]).sum(1)
+        assert not want.isfinite().any() and torch.equal(Y[r].double().nan_to_num(7.0), want.nan_to_num(7.0)), r
+        assert torch.equal(before[r].double().nan_to_num(7.0), want.nan_to_num(7.0)), r
+    if good:
+        check_rows(Y[good], X[good], Wd, sc, 128, False)
+    # without a workspace such a row is NaN, as the header says; with one, finite rows are what they are without
+    assert matvec(matvec_plugin(registry, rows), X, W, sc, None, 128)[0].isnan().all()
+    a, b = (matvec(matvec_plugin(registry, rows), plain, W, sc, None, 128, workspace=w) for w in (ws, None))
+    if rows == 8 or registry.heuristic(m, n, k, "w4a16", group_size=128).config.bk == 32:
+        assert torch.equal(a, b)
