@@ -62,7 +62,8 @@ const char *gemm_util_last_error_message(void);
  * is padding: its heads are passed through unchanged.  backward = 1 turns the gradient of y into that of x (the transposed
  * map; its rows are addressed as x -> y too).  Angles are exact modulo a turn at every position.
  * Strides are in elements, so that q and k are turned in place inside a fused QKV result: heads = q + k heads,
- * token stride = the row of the whole result. */
+ * token stride = the row of the whole result.  Strides of x may be 0 (one head for many); heads and tokens of y do not
+ * overlap. */
 enum { GEMM_ROTARY_HALF = 0, GEMM_ROTARY_INTERLEAVED = 1 };
 enum {
     GEMM_ROTARY_PLAIN = 0,

@@ -680,6 +680,8 @@ int gemm_rotary(const GemmRotaryArgs *a)
     const size_t e = type_bytes(a->dtype);
     if (!aligned(a->x, e) || !aligned(a->y, e) || !aligned(a->positions, 8)) return refuse("x, y and positions must be aligned to their elements");
     if (a->x == a->y && (a->x_token_stride != a->y_token_stride || a->x_head_stride != a->y_head_stride)) return refuse("in place, x and y have the same strides");
+    auto on_top = [&](int64_t stride) { return stride > -a->head_dim && stride < a->head_dim; };
+    if ((a->heads > 1 && on_top(a->y_head_stride)) || (a->tokens > 1 && on_top(a->y_token_stride))) return refuse("heads or tokens of y overlap");
     if (!(a->base > 0) || !isfinite(a->base)) return refuse("base %g must be positive and finite", a->base);
     RotaryKey key = {a->base, 1, 0, 1, 1, a->rot_dim, a->scaling};
     if (a->scaling != GEMM_ROTARY_PLAIN) {

@@ -47,3 +47,18 @@ def test_a_failed_call_is_no_refusal(no_gpu):
         assert rc not in (0, INVALID_VALUE) and b"launch failed" in lib.gemm_util_last_error_message()
         rc = failing_logits()
         assert rc not in (0, INVALID_VALUE) and b"failed" in lib.gemm_util_last_error_message()
+
+
+@pytest.mark.parametrize("change", [dict(y_head_stride=0), dict(y_head_stride=63), dict(y_head_stride=-63), dict(y_token_stride=0), dict(y_token_stride=32), dict(y_token_stride=-1)])
+def test_heads_or_tokens_of_y_on_top_of_each_other(change):
+    """Broadcast strides are for x: a y whose heads or tokens share elements is refused (they would be written in any order)."""
+    a = rotary_args(64, 2 << 20)
+    for k, v in change.items():
+        setattr(a, k, v)
+    with pytest.raises(g.GemmError, match="overlap") as e:
+        g.rotary(a)
+    assert e.value.code == 6
+    a.x = a.y                                    # in place too
+    a.x_head_stride, a.x_token_stride = a.y_head_stride, a.y_token_stride
+    with pytest.raises(g.GemmError, match="overlap"):
+        g.rotary(a)
