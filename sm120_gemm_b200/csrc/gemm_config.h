@@ -27,7 +27,6 @@
 #include <vector>
 
 #include "../../include/sm100_gemm.h"
-#include "w4_choice.h"
 
 namespace sm100 {
 inline const char *const kDtypeNames[] = {"bf16", "fp8", "mxfp8", "w4a16", "w4a4"};
@@ -344,7 +343,7 @@ inline double heuristic_ms(const GemmConfig &c, int M, int N, int K, int sms = 1
     const double eb = sm100::elem_bits(c.dt) / 8.0;                         // bytes per operand element
     const double wb = c.dt == GEMM_DT_W4A16 ? 0.5 : eb;
     const double alg_bytes = (double)M * K * eb + (double)N * K * wb + (double)M * N * 2.0;
-    if (c.dt == GEMM_DT_W4A16)    // the narrowest padded M that fits, then the deeper ring
+    if (c.dt == GEMM_DT_W4A16)    // the narrowest padded M that fits, then the deeper ring (matrix-vector plugins hand on what tensor memory does faster)
         return alg_bytes / hbm * 1e3 + c.bn * 1e-4 - c.num_stages * 1e-6;
     const double slots = (double)(sms / c.cg);
     const double tiles = std::ceil((double)M / c.bm) * std::ceil((double)N / c.bn);
@@ -386,12 +385,9 @@ inline const LoadedKernel *heuristic_kernel(const KernelRegistry &reg, int dt, i
     const LoadedKernel *best = nullptr;
     double best_ms = 0;
     std::string best_name;
-    // (nothing said about the groups: the matrix-vector plugin, which takes every kind and hands on what another kernel does faster)
-    const bool plain_w4 = dt == GEMM_DT_W4A16 && kind.group_size == 128 && kind.x_dtype == GEMM_X_BF16 && !kind.zero_points && !kind.transform;
     for (const auto &k : reg.kernels) {
         if (k.config.dt != dt || (k.config.epi == 2) != kind.transform || !k.config.takes(kind, K) || !k.can_run(M, N, K)) continue;
-        double ms = heuristic_ms(k.config, M, N, K, sms);
-        if (plain_w4 && k.config.bk == 32 && sm100::w4_tensor_memory_wins(M, N, K, sms)) ms += 1.0;      // behind the other W4A16 plugins
+        const double ms = heuristic_ms(k.config, M, N, K, sms);
         const std::string name = k.config.name();
         if (!best || ms < best_ms || (ms == best_ms && name < best_name)) { best = &k; best_ms = ms; best_name = name; }
     }

@@ -38,13 +38,14 @@
 // 26.7 / 29.5 / 30.5 / 39.7 / 51; 4096 x 14336 12.4 / 13.5 / 15.0 / 18.1 / 19.7; 8192 x 28672 31.2 / 31.5 / 32.9 / 47 / 56.
 // One row is bound by the bytes (slope 6.3 TB/s) and 5 us of start, staging and end; 16 rows by the tensor and logic
 // instructions that two warps per scheduler issue (the tcgen05 tiles of the bk128 plugins take 46, 19.4 and 46 us for any M:
-// calls that those take, and that give the workspace, are handed to them, w4_choice.h).
+// calls that those take, and that give the workspace, are handed to them).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <cmath>
+
 #include "bf16_gemm.cuh"
-#include "w4_choice.h"
 #include "w4a16_tmem_gemm.cuh"
 
 namespace sm100 {
@@ -771,20 +772,11 @@ struct W4MatvecLauncher {
             return set_error(GEMM_ERR_ARG, "alpha / beta*C / bias / activation need a fused-epilogue configuration (e2)");
         if (a.activation < ACT_NONE || a.activation > ACT_SILU) return set_error(GEMM_ERR_ARG, "unknown activation %d", a.activation);
         if (a.beta != 0.f && !a.C) return set_error(GEMM_ERR_ARG, "beta != 0 needs C");
-        // What the tensor-memory kernel does faster goes to it where the call is one that its plugins take, workspace included.
-        // Whichever kernel does it, an infinite x then gives what it gives there.
+        // A call that the tensor-memory plugins take, workspace included: what their kernel does faster goes to it, and whichever does
+        // it, an infinite x gives what it gives there.
         using Other = W4A16TmemLauncher<W4A16TmemTraits<16, 6>>;
         const bool common = T::EPI != EPI_FUSED && a.x_dtype == GEMM_X_BF16 && !a.w_zero && a.group_size == 128 && a.workspace && bits(a.workspace) % 16 == 0 &&
                             (a.workspace_bytes == 0 || a.workspace_bytes >= workspace_bytes(a.M, a.N, a.K)) && Other::can_run(a.M, a.N, a.K);
-        if constexpr (T::MPAD > 8 && T::EPI != EPI_FUSED) {
-            if (common) {
-                int sms = 0;
-                const int rc = sm_count(&sms);
-                if (rc != GEMM_OK) return rc;
-                if (w4_tensor_memory_wins(a.M, a.N, a.K, a.sm_limit > 0 && a.sm_limit < sms ? a.sm_limit : sms))
-                    return Other::run(a.M, a.N, a.K, a.X, a.W, a.Y, a.w_scale, a.group_size, static_cast<float *>(a.workspace), a.workspace_bytes, a.sm_limit, a.stream);
-            }
-        }
         W4MatvecParams p;
         p.infinities = common;
         p.M = a.M; p.N = a.N; p.K = a.K;
@@ -822,6 +814,7 @@ struct W4MatvecLauncher {
         if (rc != GEMM_OK) return rc;
         long long best = -1;
         int grid = 0;
+        double us = 0;
         const int fixed = T::ring_bytes(gpu) + T::ROW_BYTES;
         for (int cluster_shift = 0; cluster_shift <= 2; cluster_shift++) {
             const int cluster = 1 << cluster_shift, shares = std::min(cluster == 1 ? most_ctas : std::min(most_ctas / cluster, clusters[cluster_shift - 1]), all_tiles);
@@ -848,8 +841,12 @@ struct W4MatvecLauncher {
                 p.block_rows = block_rows;
                 p.units_per_pass = per_pass;
                 p.part_at = fixed + T::staged_bytes(a.M, per_pass, gpu);
+                if constexpr (T::MPAD > 8) us = matvec_us(a, blocks * passes * rounds, stagings, per_pass, blocks * block_rows, cluster);
             }
         }
+        if constexpr (T::MPAD > 8 && T::EPI != EPI_FUSED)
+            if (common && tensor_memory_us(a, most_ctas) < us)
+                return Other::run(a.M, a.N, a.K, a.X, a.W, a.Y, a.w_scale, a.group_size, static_cast<float *>(a.workspace), a.workspace_bytes, a.sm_limit, a.stream);
         const uint32_t tile_step = (T::WARPS >> p.wk_shift) * T::TILE;                // rows; K <= 2^24
         p.step_batch = T::UNIT << p.wk_shift;
         p.step_w = tile_step * ((uint32_t)a.K / 2);
@@ -864,6 +861,25 @@ struct W4MatvecLauncher {
     }
 
 private:
+    // What the two kernels take for 9 to 16 rows of bf16 against signed weights in groups of 128 (us, back to back, weights from
+    // HBM), to tell which is faster.  Of the plan: rounds of batches by every warp, which are longer where a pass is; stagings of
+    // per_pass units of X; weights; results that an SM writes; what a cluster costs.  The tensor-memory kernel, whose time is the same for all
+    // these M: units of 128 rows x 128 k of an SM, and the parts of the tiles that meet in the workspace.  Fitted to 1240 sizes:
+    // what is picked is 0.4 % slower on average than the faster of the two (always this kernel: 3.7 %, always the other:
+    // 10.3 %); 33 of them are more than 3 % slower than the tensor-memory kernel (at most 10 %; of this kernel alone 317, at most 56 %),
+    // 25 more than 3 % slower than this one (at most 16 %).  this / tensor memory: 16 x 28672 x 8192 50.3 / 45.9, 16 x 8192 x 28672 54.0 /
+    // 46.2, 13 x 5056 x 24704 42.3 / 29.4; but 9 x 28672 x 8192 39.7 / 45.7, 16 x 131072 x 4096 86.0 / 95.0, 16 x 4096 x 4096 11.3 / 12.1.
+    static double matvec_us(const GemmArgs &a, long long rounds, long long stagings, int per_pass, long long rows, int cluster)
+    {
+        return 1.5 + rounds * (0.753 + 0.00234 * per_pass) + stagings * (3.2 + 0.00604 * a.M * per_pass) + 3.33e-8 * a.N * a.K + 0.00068 * rows * a.M +
+               (cluster == 1 ? 0.0 : cluster == 2 ? 1.4 : 3.1);
+    }
+    static double tensor_memory_us(const GemmArgs &a, int ctas)
+    {
+        const double tiles = (a.N + 127) / 128, units = tiles * (a.K / 128) / ctas;
+        return 5.2 + 0.329 * units + 0.42 * ctas / tiles + 0.83 * std::sqrt(units);
+    }
+
     static int sm_count(int *out)
     {
         static std::atomic<int> counts[MAX_DEVICES];

@@ -176,22 +176,15 @@ def heuristic_ms(c: GemmConfig, M: int, N: int, K: int, sms: int = 148) -> float
     return (t + launch_us * 1e-6) * 1e3
 
 
-def w4_tensor_memory_wins(M: int, N: int, K: int, sms: int = 148) -> bool:
-    """The rule of csrc/w4_choice.h (see there)."""
-    return -(-N // 128) * (K // 128) >= 8 * sms and M >= (9 if K >= 10240 else 10 if K >= 6144 else 14)
-
-
 def heuristic_config(configs, dt: str, M: int, N: int, K: int, sms: int = 148, **kind):
     """The configuration of `configs` with the smallest modelled time for the shape among those that take a call of this
     kind (GemmConfig.takes), for callers that do not autotune (the reference skips shapes that are missing from its
     cache, src/bench.cu:455-458)."""
     best = None
-    plain_w4 = dt == "w4a16" and kind.get("group_size") == 128 and not (kind.get("x_dtype") or kind.get("zero_points") or kind.get("transform"))
     for c in configs:
         if c.dt != dt or (c.epi == 2) != kind.get("transform", False) or not c.takes(K, **kind) or not c.is_valid_for(M, N, K):
             continue
-        behind = plain_w4 and c.bk == 32 and w4_tensor_memory_wins(M, N, K, sms)
-        key = (heuristic_ms(c, M, N, K, sms) + (1.0 if behind else 0.0), c.name())
+        key = (heuristic_ms(c, M, N, K, sms), c.name())
         if best is None or key < best[0]:
             best = (key, c)
     return best[1] if best else None

@@ -104,16 +104,3 @@ def test_cpp_dispatcher_picks_the_same(tmp_path, registry, cache):
         kind = dict(group_size=int(group), x_dtype=int(x), zero_points=bool(int(z)), transform=bool(int(t)))
         for mine, theirs in ((registry.heuristic(int(m), int(n), int(k), dt, **kind), heuristic), (registry.select(cache, int(m), int(n), int(k), dt, **kind), select)):
             assert (mine.config.name() if mine else "-") == theirs, (dt, m, n, k, kind)
-
-
-@pytest.mark.parametrize("m, n, k, tensor_memory", [
-    (16, 28672, 8192, True), (13, 28672, 8192, True), (9, 28672, 8192, False), (9, 8192, 28672, True), (16, 8192, 28672, True), (8, 8192, 28672, False),
-    (16, 14336, 4096, True), (13, 14336, 4096, False), (16, 4096, 4096, False), (1, 28672, 8192, False), (13, 5056, 24704, True),
-])
-def test_plain_calls_go_to_the_faster_kernel(registry, m, n, k, tensor_memory):
-    """Symmetric bf16 weights in groups of 128, 9 to 16 rows: the tensor-memory plugin where it is the faster one (as measured,
-    csrc/w4_choice.h); the other kinds stay where they are done at all."""
-    pick = registry.heuristic(m, n, k, "w4a16", group_size=128).config
-    assert pick.bk == (128 if tensor_memory else 32) and pick.bn == (8 if m <= 8 else 16)
-    assert registry.heuristic(m, n, k, "w4a16", group_size=64).config.bk == 32
-    assert registry.heuristic(m, n, k, "w4a16", group_size=128, zero_points=True).config.bk == 32

@@ -122,5 +122,5 @@ def test_infinities_in_calls_that_the_tensor_memory_plugin_takes(registry, cuda_
     # without a workspace such a row is NaN, as the header says; with one, finite rows are what they are without
     assert matvec(matvec_plugin(registry, rows), X, W, sc, None, 128)[0].isnan().all()
     a, b = (matvec(matvec_plugin(registry, rows), plain, W, sc, None, 128, workspace=w) for w in (ws, None))
-    if rows == 8 or registry.heuristic(m, n, k, "w4a16", group_size=128).config.bk == 32:
-        assert torch.equal(a, b)
+    # (above 8 rows the call may be handed to the tensor-memory kernel)
+    assert torch.equal(a, b) or rows == 16 and torch.equal(a, matvec(registry.find("w4a16_bm128_bn16_bk128_s6_cg1_sk0_ab1_e0"), plain, W, sc, None, 128, workspace=ws))
