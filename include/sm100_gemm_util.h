@@ -96,7 +96,8 @@ int gemm_rotary(const GemmRotaryArgs *args);
 /* Logits of `rows` sequences before sampling, y[r][v] from x[r][v], in FP32, rounded once to the type of y:
  *     l = x;  token v in the row's history:  l = l > 0 ? l / repetition : l * repetition
  *     c = how often v was generated, c > 0:  l -= frequency * c + presence
- *     v listed in the row's biases:          l += the sum of its listed values, in the order of the list
+ *     v listed in the row's biases:          l += the sum of its listed values, in the order of the list (an id that is listed
+ *                                            more than once costs a walk over the row's list: fine for some hundred entries)
  *     mask bit of v is 0:                    l = -inf (whatever it was; a row that allows nothing is all -inf)
  * History: the first history_len[r] tokens of row r (at most history_ld), the first prompt_len[r] of which are the prompt:
  * they count as seen, not as generated; without a history (history NULL, a first token) no penalty applies.  Ids outside [0, vocab) are ignored, in the history and in the biases. */

@@ -430,17 +430,20 @@ __device__ __forceinline__ float adjust(float l, unsigned c, float bias, float r
 }
 
 // An id that is listed more than once: its values are added in the order of the list, by the thread of the first entry (true).
+// The others look as far as that entry: a list of one id is walked through once, not once for each of its entries.
 __device__ __forceinline__ bool sum_of_biases(const LogitsParams &p, int b0, int b1, int e, int id, float &sum)
 {
-    bool first = true;
-    sum = 0.f;
-#pragma unroll 8
-    for (int d = b0; d < b1; d++) {
-        const bool same = p.bias_ids[d] == id;
-        first = first && !(same && d < e);
-        if (same) sum = d == e ? p.bias_values[d] : sum + p.bias_values[d];
+    for (int d = b0; d < e; d += 8) {
+        bool earlier = false;
+#pragma unroll
+        for (int i = 0; i < 8; i++) earlier = earlier || (d + i < e && p.bias_ids[d + i] == id);
+        if (earlier) return false;
     }
-    return first;
+    sum = p.bias_values[e];
+#pragma unroll 8
+    for (int d = e + 1; d < b1; d++)
+        if (p.bias_ids[d] == id) sum += p.bias_values[d];
+    return true;
 }
 
 template <class TX, class TY, bool NARROW, int THREADS>
