@@ -60,7 +60,8 @@ const char *gemm_util_last_error_message(void);
  * f_i = base^(-2 i / rot_dim), scaled for contexts longer than trained (`scaling`).  Pairs: (i, i + rot_dim / 2) or
  * (2 i, 2 i + 1) of the head's first rot_dim elements; elements behind them are copied.  A token with a negative position
  * is padding: its heads are passed through unchanged.  backward = 1 turns the gradient of y into that of x (the transposed
- * map; its rows are addressed as x -> y too).  Angles are exact modulo a turn at every position.
+ * map; its rows are addressed as x -> y too).  An angle is off by at
+ * most 2^-65 of a turn per position, before its sine is taken (within 2^-22; 2^-20.6 for 16-bit data).
  * Strides are in elements, so that q and k are turned in place inside a fused QKV result: heads = q + k heads,
  * token stride = the row of the whole result.  Strides of x may be 0 (one head for many); heads and tokens of y do not
  * overlap. */
@@ -70,7 +71,9 @@ enum {
     GEMM_ROTARY_LINEAR = 1,  /* f_i / factor                                                                          */
     GEMM_ROTARY_NTK = 2,     /* base * factor^(rot_dim / (rot_dim - 2)) in the place of base                          */
     GEMM_ROTARY_RAMP = 3     /* f_i * w + f_i / factor * (1 - w), w = (original_length * f_i / 2 pi - low_rotations)  */
-                             /* / (high_rotations - low_rotations), clamped to [0, 1]                                 */
+                             /* / (high_rotations - low_rotations), clamped to [0, 1]: linear in the rotations over   */
+                             /* the original length.  Models whose ramp is linear in i between two pairs get other    */
+                             /* frequencies from this one                                                             */
 };
 typedef struct GemmRotaryArgs {
     uint32_t struct_size;   /* sizeof(GemmRotaryArgs), checked                       */
@@ -100,7 +103,8 @@ int gemm_rotary(const GemmRotaryArgs *args);
  *                                            more than once costs a walk over the row's list: fine for some hundred entries)
  *     mask bit of v is 0:                    l = -inf (whatever it was; a row that allows nothing is all -inf)
  * History: the first history_len[r] tokens of row r (at most history_ld), the first prompt_len[r] of which are the prompt:
- * they count as seen, not as generated; without a history (history NULL, a first token) no penalty applies.  Ids outside [0, vocab) are ignored, in the history and in the biases. */
+ * they count as seen, not as generated (history_ld of 8192 or more takes a form made for long histories, whatever the lengths);
+ * without a history (history NULL, a first token) no penalty applies.  Ids outside [0, vocab) are ignored, in the history and in the biases. */
 typedef struct GemmLogitsArgs {
     uint32_t struct_size;   /* sizeof(GemmLogitsArgs), checked                                             */
     int32_t x_dtype, y_dtype;   /* GEMM_X_BF16, GEMM_X_F16 or GEMM_X_F32                                   */

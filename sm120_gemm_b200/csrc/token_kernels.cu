@@ -101,9 +101,9 @@ size_t type_bytes(int t) { return t == GEMM_X_F32 ? 4 : 2; }
 
 // ------------------------------------------------------------------------------------------------------------ rotary
 // The pair (a, b) number i of a head at position t is turned by the angle t * f_i.  Angles are kept in turns, as 64-bit
-// fractions: freq[i] = f_i / (2 pi) * 2^64, and the low 64 bits of t * freq[i] are the angle modulo one turn -- exact for
-// every position, where a 32-bit product is off by radians a million tokens into a context (the table's own rounding,
-// 2^-65 of a turn per position, is the whole error).
+// fractions: freq[i] = f_i / (2 pi) * 2^64, and the low 64 bits of t * freq[i] are the angle modulo one turn, off by no more
+// than the table's own rounding, 2^-65 of a turn per position: less than FP32's share up to some 2^41, where a 32-bit product
+// is off by radians a million tokens into a context.
 constexpr int ROTARY_TABLE = 256;      // pairs of one head that the launch's parameters have room for
 
 struct RotaryTable {
@@ -122,8 +122,8 @@ struct RotaryParams {
     unsigned per_slice;          // tokens of one grid.y
 };
 
-// cos and sin (times scale) of `phase` / 2^64 turns.  16-bit data: the hardware's sine of the nearest half turn either way,
-// off by at most 2^-21.4, and 2^-22.3 from the angle's conversion.
+// cos and sin (times scale) of `phase` / 2^64 turns.  16-bit data: the hardware's cosine and sine of the nearest half turn either
+// way, off by at most 2^-21.19 and 2^-21.41, and by 2^-22.3 from the angle's conversion: 2^-20.6 together.
 template <class T>
 __device__ __forceinline__ float2 cos_sin(unsigned long long phase, float scale)
 {
@@ -151,7 +151,7 @@ struct alignas(N * sizeof(T)) Pack {
 
 // A unit is P pairs of one head (two pieces of P elements) or, behind the pairs, 2 P elements that are copied; a thread has
 // one unit of a token in every `slots`-th head, so that the sines, which cost more than the turning, are taken once for
-// several heads.  HBM-bound: 2 * heads * dim elements per token.  8192 tokens of 48 heads of 128, bf16: 32.3 us (5.2 TB/s; one
+// several heads.  HBM-bound: 2 * heads * dim elements per token.  8192 tokens of 40 heads of 128, bf16: 32.2 us (5.2 TB/s; one
 // head per thread, a sine each and 2-byte accesses took 182); 16 tokens 2.6 us in a graph.
 template <class T, int P, bool INTERLEAVED>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p, const __grid_constant__ RotaryTable table)

@@ -35,9 +35,9 @@
 // else in passes over K with the partial sums kept.
 //
 // Measured (us, device time of back-to-back calls, weights from HBM; groups of 128, bf16): 28672 x 8192 by 1 / 4 / 8 / 9 / 16 rows
-// 26.7 / 29.5 / 30.5 / 39.7 / 51; 4096 x 14336 12.4 / 13.5 / 15.0 / 18.1 / 19.7; 8192 x 28672 31.2 / 31.5 / 32.9 / 47 / 56.
-// One row is bound by the bytes (slope 6.3 TB/s) and 5 us of start, staging and end; 16 rows by the tensor and logic
-// instructions that two warps per scheduler issue (the tcgen05 tiles of the bk128 plugins take 46, 19.4 and 46 us for any M:
+// 26.4 / 28.8 / 30.2 / 39.7 / 50.3; 4096 x 14336 11.4 / 12.4 / 13.7 / 17.0 / 19.3; 8192 x 28672 30.9 / 31.0 / 32.4 / 45.8 / 54.0.
+// One row is bound by the bytes (slope 6.3 TB/s) and 5 us of start, staging and end; 16 rows by two warps per scheduler, with
+// issue slots at 38 % and the tensor pipe at 27 %: by the latency of their instructions (the tcgen05 tiles of the bk128 plugins take 46, 19.4 and 46 us for any M:
 // calls that those take, and that give the workspace, are handed to them).
 #pragma once
 #include <cuda_bf16.h>
