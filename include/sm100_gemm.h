@@ -140,14 +140,14 @@ enum { GEMM_Y_BF16 = 0, GEMM_Y_E4M3 = 1 };
  * a multiple of group_size (32, 64 or 128); X bf16 or fp16 (x_dtype), scales [N][K/group_size] of the same type, signed
  * weights or zero points (w_zero).  X and W 16-byte aligned, every other pointer aligned to its elements.  They need no
  * workspace; gemm_workspace_bytes reports the family's figure, so that one workspace serves every W4A16 plugin, and a call
- * that gives one (not `_e2`) is done in it by the family's tensor-memory kernel where that takes the call (bf16, signed
+ * that gives one of that size (not `_e2`) is done in it by the family's tensor-memory kernel where that takes the call (bf16, signed
  * weights, groups of 128, N a multiple of 8) and is faster (more than 8 rows): such calls then may not share it at the same
  * time.  The first call may be made under stream capture.  `_e2`: with the output transform, in the type of X; y_dtype must be
  * GEMM_Y_BF16 (= "the type of X" here), amax NULL; C may be Y.  Sums are FP32, rounded once; their error is relative to
  * the sum of (q + zero) * scale * |x| (zero = 8 for signed weights, q = w + 8), for bf16 no smaller than 2^-116 a term.
- * Scales and zero points are read in whole aligned 4-byte words, up to 3 bytes around their arrays.  An infinity or NaN in a row of X makes
- * that row of Y NaN; in a call that gives the workspace and that the tensor-memory kernel takes, an infinity gives what it
- * gives there (the sum of w * x: infinities, NaN where a weight is 0).
+ * Scales and zero points are read in whole aligned 4-byte words, up to 3 bytes around their arrays.  An infinity or NaN in a
+ * row of X makes that row of Y NaN; in a call that gives the workspace and that the tensor-memory kernel takes, an infinity
+ * gives what it gives there (the sum of w * x: infinities, NaN where a weight is 0).
  */
 /* Returns GEMM_OK or an error code; asynchronous on success. */
 int gemm_run_ex(const GemmArgs *args);

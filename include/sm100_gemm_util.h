@@ -60,8 +60,8 @@ const char *gemm_util_last_error_message(void);
  * f_i = base^(-2 i / rot_dim), scaled for contexts longer than trained (`scaling`).  Pairs: (i, i + rot_dim / 2) or
  * (2 i, 2 i + 1) of the head's first rot_dim elements; elements behind them are copied.  A token with a negative position
  * is padding: its heads are passed through unchanged.  backward = 1 turns the gradient of y into that of x (the transposed
- * map; its rows are addressed as x -> y too).  An angle is off by at
- * most 2^-65 of a turn per position, before its sine is taken (within 2^-22; 2^-20.6 for 16-bit data).
+ * map; its rows are addressed as x -> y too).  An angle is off by at most 2^-65 of a turn per position, before its sine is
+ * taken (within 2^-22; 2^-20.6 for 16-bit data).
  * Strides are in elements, so that q and k are turned in place inside a fused QKV result: heads = q + k heads,
  * token stride = the row of the whole result.  Strides of x may be 0 (one head for many); heads and tokens of y do not
  * overlap. */

@@ -83,7 +83,8 @@ def test_zero_rows_take_no_longer(registry, cuda_device, m, pad, n, k):
     assert padded <= 1.25 * full, (padded, full)
 
 
-@pytest.mark.parametrize("m, n, k", [(1, 4096, 4096), (7, 200, 28672), (8, 1000, 1024 + 128), (5, 8, 128), (3, 30000, 640), (16, 304, 65536), (12, 4096, 3968), (9, 64, 131072), (16, 4096, 8192)])
+@pytest.mark.parametrize("m, n, k", [(1, 4096, 4096), (7, 200, 28672), (8, 1000, 1024 + 128), (5, 8, 128), (3, 30000, 640), (16, 304, 65536), (12, 4096, 3968), (9, 64, 131072), (16, 4096, 8192),
+                                     (8, 2600, 65536), (8, 400000, 256)])
 def test_infinities_in_calls_that_the_tensor_memory_plugin_takes(registry, cuda_device, m, n, k):
     """bf16, signed weights in groups of 128, the family's workspace: an infinite x gives the sum of w * x, as it did before these
     plugins -- infinities of either sign, NaN where a weight or a scale is 0 or two signs meet -- and leaves the other rows alone."""
@@ -106,6 +107,7 @@ def test_infinities_in_calls_that_the_tensor_memory_plugin_takes(registry, cuda_
         X[7, k // 3], X[8] = inf, 0
     ws = torch.empty(2 * 160 * 128 * 128, device="cuda")
     Y = matvec(matvec_plugin(registry, rows), X, W, sc, None, 128, workspace=ws, workspace_bytes=ws.numel() * 4)
+    one_sm = matvec(matvec_plugin(registry, rows), X, W, sc, None, 128, workspace=ws, sm_limit=1)        # blocks of tiles, passes over K
     before = matvec(registry.find("w4a16_bm128_bn16_bk128_s6_cg1_sk0_ab1_e0"), X, W, sc, None, 128, workspace=ws)
     good = []
     for r in range(m):
@@ -117,8 +119,10 @@ def test_infinities_in_calls_that_the_tensor_memory_plugin_takes(registry, cuda_
         want = (Wd[:, far] * x[far]).sum(1)
         assert not want.isfinite().any() and torch.equal(Y[r].double().nan_to_num(7.0), want.nan_to_num(7.0)), r
         assert torch.equal(before[r].double().nan_to_num(7.0), want.nan_to_num(7.0)), r
+        assert torch.equal(one_sm[r].double().nan_to_num(7.0), want.nan_to_num(7.0)), r
     if good:
         check_rows(Y[good], X[good], Wd, sc, 128, False)
+        check_rows(one_sm[good], X[good], Wd, sc, 128, False)
     # without a workspace such a row is NaN, as the header says; with one, finite rows are what they are without
     assert matvec(matvec_plugin(registry, rows), X, W, sc, None, 128)[0].isnan().all()
     a, b = (matvec(matvec_plugin(registry, rows), plain, W, sc, None, 128, workspace=w) for w in (ws, None))
